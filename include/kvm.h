@@ -519,6 +519,148 @@ kvm_status kvm_quantize_rows(kvm_stream stream, int32_t type, const void *d_src,
 kvm_status kvm_quantize_rows_noalloc(kvm_stream stream, int32_t type, const void *d_src,
                                      uint64_t n_rows, uint32_t n_embd, void *d_dst);
 
+/* ---------------------------------- the attention layer around a window -- */
+
+/*
+ * Sessionless calls for the layer that uses a window: the step's cell map, the
+ * norm and rotation of its queries and keys, the rows into and out of the
+ * window, and the attention over it.  They launch on `stream` without a host
+ * wait, allocate nothing, keep nothing between calls, and may be captured into
+ * a CUDA graph.  The first pointer of a call decides the device: the work runs
+ * there whatever device is current, and `stream` must belong to it (NULL: that
+ * device's legacy default stream).  A bad argument is KVM_EINVAL, with the
+ * reason in kvm_last_error(NULL), before anything is launched.  What only the
+ * device sees -- lengths, table entries, cells -- is bounds-checked there:
+ * nothing outside the named buffers is read or written, and each call says
+ * what it makes of a bad value.
+ */
+
+/*
+ * One layer's cache as these calls see it: n_slots blocks of block_tokens rows
+ * ("cells"; cell c = slot * block_tokens + offset, as
+ * src/adapter/llama-kvmem-batch.cpp:5-58 maps positions), each row
+ * n_head_kv * head_dim values of type_k / type_v.  A session's window is such a
+ * cache with n_slots = kvm_window_slots.  d_k / d_v: 4-byte aligned (16 bytes
+ * are faster).  head_dim: a multiple of 32; n_slots * block_tokens < 2^31.
+ */
+typedef struct kvm_cache {
+    void *d_k;
+    void *d_v;
+    int32_t type_k;
+    int32_t type_v;
+    uint32_t n_head_kv;
+    uint32_t head_dim;
+    uint32_t block_tokens;
+    uint32_t n_slots;
+} kvm_cache;
+
+/*
+ * The step's block tables and cell map from the requests' lengths, on the
+ * device (no counterpart in the reference, which serves one sequence:
+ * alloc_slot, src/adapter/llama-memory-kvmem.cpp:693-700, for many).  Request i
+ * holds d_past[i] tokens in the blocks d_table[i][0 .. ceil(past/T)) and brings
+ * d_new[i] more; T = block_tokens.  In request order, each takes the slots its
+ * new blocks need from the front of d_free and d_table[i] gets them behind the
+ * held ones.  A request whose need reaches past n_free waits, and so does every
+ * later one that needs a slot; requests that need none go ahead.  A request
+ * with a negative length, more than table_cols blocks, or rows past n_rows is
+ * refused too, and takes part in the free list as one that needs nothing.
+ * Outputs: q_start[i] the first row of request i (q_start[n_seq] the rows of
+ * all, at most n_rows); kv_len[i] = past + new, 0 for a request that waits or
+ * is refused; per row r < n_rows its cell (-1 when its request does not run,
+ * or when a held table entry is negative), position and request, and behind
+ * the last request -1, 0, -1; info = {slots taken, rows of all requests,
+ * requests that do not run, tokens of those that do}.  n_seq <= 4096.
+ */
+typedef struct kvm_batch_map {
+    const int32_t *d_past;
+    const int32_t *d_new;
+    const int32_t *d_free;
+    int32_t *d_table;
+    uint64_t table_stride;     /* entries between two requests' rows, >= table_cols */
+    uint32_t table_cols;
+    uint32_t n_seq;
+    uint32_t n_free;
+    uint32_t block_tokens;
+    uint32_t n_rows;
+    uint32_t reserved0;
+    int32_t *d_q_start;        /* [n_seq + 1] */
+    int32_t *d_kv_len;         /* [n_seq] */
+    int64_t *d_cells;          /* [n_rows] */
+    int32_t *d_pos;            /* [n_rows] */
+    int32_t *d_seq;            /* [n_rows] */
+    int32_t *d_info;           /* [4] */
+} kvm_batch_map;
+kvm_status kvm_map_batch(kvm_stream stream, const kvm_batch_map *m);
+
+/*
+ * RMS norm of every head of q and k and the NeoX rotation at the row's
+ * position (kvmem::rope_neox_apply, kvmem/src/host/rope.cpp:8-45), one pass:
+ *     y = x / sqrt(mean(x^2) + eps) * weight,
+ *     (y[i], y[i + n_rot/2]) turned by d_pos[row] * d_freqs[i], i < n_rot/2.
+ * The angle is formed and reduced in 64 bits, the rest in 32, and rounded once.
+ * d_q_weight / d_k_weight: [head_dim] F32, NULL = 1.  n_rot: a multiple of 16
+ * up to head_dim, 0 = no rotation.  head_dim: a multiple of 16 up to 512.
+ * All tensors have one type (F32, F16 or BF16).  k and k_out may be NULL
+ * (queries only).  An output may be its input (the same data and strides);
+ * any other overlap is undefined.
+ */
+kvm_status kvm_qk_norm_rope(kvm_stream stream, uint32_t n, const kvm_rows *q, const kvm_rows *k,
+                            const float *d_q_weight, const float *d_k_weight, float eps,
+                            const float *d_freqs, uint32_t n_rot, const int32_t *d_pos,
+                            const kvm_rows *q_out, const kvm_rows *k_out);
+
+/*
+ * Quantize row i of k and v (F32, F16 or BF16) into cell d_cells[i], with the
+ * arithmetic and bytes of ggml's quantize_row_*_ref in 32 bits
+ * (kvm_quantize_rows for F16 rows).  A cell outside [0, n_slots*block_tokens)
+ * skips the row.  k or v may be NULL.  Rows that share a cell leave a mixture
+ * of their blocks there.
+ */
+kvm_status kvm_write_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
+                          const int64_t *d_cells, const kvm_rows *k, const kvm_rows *v);
+/* The inverse: row i of k_out / v_out (F32, F16 or BF16; either may be NULL)
+ * gets the values that cell d_cells[i] stands for, code * scale in 32 bits and
+ * rounded once; zeros for a cell outside the cache. */
+kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
+                         const int64_t *d_cells, const kvm_rows *k_out, const kvm_rows *v_out);
+
+/*
+ * Attention of a step's queries over one layer's cache, straight from its
+ * rows.  Request s owns rows d_q_start[s] .. d_q_start[s+1] of q and out, and
+ * its keys j < d_kv_len[s] lie at cell d_table[s][j / T] * T + j % T.
+ *     out = softmax(scale * q k^T) v   over the keys a row sees:
+ * all of them, or with KVM_ATTEND_CAUSAL key j of row i (of n) when
+ * j <= kv_len - n + i.  A row that sees no key is 0.  Keys beyond the table's
+ * columns and keys of a block whose entry is outside [0, n_slots) are not seen.
+ * What hidden keys hold -- stale bytes, infinities, NaN -- reaches no output.
+ * Rows of q_start outside [0, n_rows) are skipped, and rows of out that belong
+ * to no request stay as they were.  Query head h reads KV head
+ * h / (n_head / n_head_kv).  q and out: F16 or BF16, head_dim 64, 128 or 256.
+ * Scores, maxima and sums are F32; the weights enter the second product in F16.
+ * max_new: the most rows of a request, as far as the caller knows (it picks the
+ * kernel; a wrong value costs time, not correctness).
+ * d_work: KVM_ATTEND_WORK_BYTES of device memory, 16-byte aligned, that no
+ * other call running at the same time uses; its contents need no preparation
+ * and mean nothing afterwards.
+ */
+#define KVM_ATTEND_CAUSAL 1u
+#define KVM_ATTEND_WORK_BYTES 33554432u
+typedef struct kvm_attend_batch {
+    const int32_t *d_table;
+    uint64_t table_stride;     /* entries between two requests' rows */
+    uint32_t table_cols;
+    uint32_t n_seq;
+    const int32_t *d_q_start;  /* [n_seq + 1] */
+    const int32_t *d_kv_len;   /* [n_seq] */
+    uint32_t n_rows;           /* rows of q and out */
+    uint32_t max_new;
+    uint32_t flags;
+    float scale;
+} kvm_attend_batch;
+kvm_status kvm_attend(kvm_stream stream, const kvm_cache *cache, const kvm_attend_batch *batch,
+                      const kvm_rows *q, const kvm_rows *out, void *d_work, uint64_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

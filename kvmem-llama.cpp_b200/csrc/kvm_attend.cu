@@ -1,0 +1,105 @@
+// kvm_attend.cu -- kvm_attend: argument checks and the choice of kernel.
+#include <cmath>
+
+#include "kvm_attend.cuh"
+#include "kvm_layer.cuh"
+
+namespace kvm {
+
+template <int D, int KT>
+cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st);
+
+namespace {
+
+template <int D>
+cudaError_t split_d(const AttendArgs &a, int kt, int vt, int nt, uint32_t grid, cudaStream_t st) {
+    switch (kt) {
+        case KVM_TYPE_Q4_0: return launch_attend_split<D, KVM_TYPE_Q4_0>(a, vt, nt, grid, st);
+        case KVM_TYPE_Q5_0: return launch_attend_split<D, KVM_TYPE_Q5_0>(a, vt, nt, grid, st);
+        case KVM_TYPE_Q8_0: return launch_attend_split<D, KVM_TYPE_Q8_0>(a, vt, nt, grid, st);
+        default: return launch_attend_split<D, KVM_TYPE_F16>(a, vt, nt, grid, st);
+    }
+}
+
+AttendRows rows_of(const kvm_rows *r) {
+    return AttendRows{static_cast<const uint8_t *>(r->data), r->nb_dim, r->nb_head, r->nb_tok,
+                      r->type == KVM_TYPE_BF16 ? 1 : 0};
+}
+
+}  // namespace
+}  // namespace kvm
+
+using namespace kvm;
+
+extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kvm_attend_batch *b, const kvm_rows *q,
+                                 const kvm_rows *out, void *d_work, uint64_t work_bytes) {
+    const char *me = "kvm_attend";
+    kvm_status r = cache_check(c, me);
+    if (r != KVM_OK) return r;
+    if (!b || !q || !out) return layer_fail(KVM_EINVAL, "%s: null argument", me);
+    const uint32_t D = c->head_dim;
+    if (D != 64u && D != 128u && D != 256u) return layer_fail(KVM_EINVAL, "%s: head_dim must be 64, 128 or 256", me);
+    if (q->n_head == 0 || q->n_head % c->n_head_kv || q->n_head > 65535u)
+        return layer_fail(KVM_EINVAL, "%s: query heads must be a multiple of the %u KV heads", me, c->n_head_kv);
+    if (b->n_seq == 0 || b->n_rows == 0) return KVM_OK;
+    if ((r = rows_check(q, q->n_head, D, "kvm_attend q")) != KVM_OK) return r;
+    if ((r = rows_check(out, q->n_head, D, "kvm_attend out")) != KVM_OK) return r;
+    if (q->type == KVM_TYPE_F32 || out->type == KVM_TYPE_F32)
+        return layer_fail(KVM_EINVAL, "%s: q and out must be F16 or BF16", me);
+    if (b->flags & ~KVM_ATTEND_CAUSAL) return layer_fail(KVM_EINVAL, "%s: unknown flags", me);
+    if (!std::isfinite(b->scale)) return layer_fail(KVM_EINVAL, "%s: scale must be finite", me);
+    if (b->n_seq > 65535u) return layer_fail(KVM_EINVAL, "%s: at most 65535 requests", me);
+    if (static_cast<uint64_t>(b->n_rows) * (q->n_head / c->n_head_kv) > 0x7fffffffull || b->table_cols > 0x7fffffffu)
+        return layer_fail(KVM_EINVAL, "%s: too many rows or columns", me);
+    if (b->n_seq > 1 && b->table_stride < b->table_cols) return layer_fail(KVM_EINVAL, "%s: table_stride < table_cols", me);
+    if (b->n_seq && (!b->d_q_start || !b->d_kv_len || (b->table_cols && !b->d_table)))
+        return layer_fail(KVM_EINVAL, "%s: null buffer", me);
+    if ((reinterpret_cast<uintptr_t>(b->d_table) | reinterpret_cast<uintptr_t>(b->d_q_start) |
+         reinterpret_cast<uintptr_t>(b->d_kv_len)) & 3u)
+        return layer_fail(KVM_EINVAL, "%s: table, q_start and kv_len must be 4-byte aligned", me);
+    if (!d_work || work_bytes < KVM_ATTEND_WORK_BYTES || (reinterpret_cast<uintptr_t>(d_work) & 15u))
+        return layer_fail(KVM_EINVAL, "%s: workspace must be %u bytes, 16-byte aligned", me, KVM_ATTEND_WORK_BYTES);
+    PointerDevice dev(c->d_k, me);
+    if (dev.status() != KVM_OK) return dev.status();
+
+    AttendArgs a{};
+    const uint32_t width = c->n_head_kv * D;
+    a.k = static_cast<const uint8_t *>(c->d_k);
+    a.v = static_cast<const uint8_t *>(c->d_v);
+    a.row_k = kvm_row_bytes(c->type_k, width);
+    a.row_v = kvm_row_bytes(c->type_v, width);
+    a.table = b->d_table;
+    a.table_stride = b->table_stride;
+    a.table_cols = b->table_cols;
+    a.q_start = b->d_q_start;
+    a.kv_len = b->d_kv_len;
+    a.n_seq = b->n_seq;
+    a.n_rows = b->n_rows;
+    a.n_head_kv = c->n_head_kv;
+    a.group = q->n_head / c->n_head_kv;
+    a.block_tokens = c->block_tokens;
+    a.n_slots = c->n_slots;
+    a.scale_log2 = b->scale * 1.4426950408889634f;
+    a.causal = (b->flags & KVM_ATTEND_CAUSAL) ? 1u : 0u;
+    a.q = rows_of(q);
+    a.out = rows_of(out);
+    a.work = static_cast<uint8_t *>(d_work);
+    a.align16 = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.row_k | a.row_v) & 15u) == 0;
+    a.min_rows = 1;
+    a.max_rows = 0xffffffffu;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    // row tiles of 8 when every request fits one, else of 16
+    const int nt = static_cast<uint64_t>(b->max_new) * a.group <= 8u ? 1 : 2;
+    // no more CTAs than a warp's step each can fill
+    const uint64_t tiles = static_cast<uint64_t>(b->n_rows) * a.group / (8u * nt) + b->n_seq;
+    const uint64_t steps = (static_cast<uint64_t>(b->table_cols) * c->block_tokens + kAttendStep - 1) / kAttendStep + 1;
+    const uint64_t most = static_cast<uint64_t>(num_sms());
+    uint64_t grid = most;
+    if (tiles * c->n_head_kv <= 8u * most) grid = std::min<uint64_t>(most, (tiles * c->n_head_kv * std::min<uint64_t>(steps, 1u << 24) + 7) / 8);
+    grid = std::max<uint64_t>(1, std::min<uint64_t>(grid, kAttendMaxCtas));
+    cudaError_t e;
+    if (D == 64u) e = split_d<64>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
+    else if (D == 128u) e = split_d<128>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
+    else e = split_d<256>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
+    return layer_cuda(e, me);
+}

@@ -1,0 +1,163 @@
+// kvm_attend.cuh -- arguments and device pieces of kvm_attend: attention of a
+// step's queries over one layer's window of ggml rows.
+//
+//   out[r] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_r . k_j - max)
+//
+// over the keys j that row r sees.  k and v stay in their blocks of 32 values
+// (code * d, d the block's f16 scale); codes enter the tensor cores as exact
+// small integers and the scales are applied outside the products.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kvm_internal.cuh"
+#include "kvm_quant.cuh"
+
+namespace kvm {
+
+// One activation tensor of an attend call (kvm_rows, 16-bit types).
+struct AttendRows {
+    const uint8_t *p;
+    uint64_t nb_dim, nb_head, nb_tok;
+    int32_t bf16;              // 1 = BF16, 0 = F16
+};
+
+struct AttendArgs {
+    const uint8_t *k, *v;      // one layer's cache
+    uint64_t row_k, row_v;     // bytes of a cache row (all heads)
+    const int32_t *table;
+    uint64_t table_stride;     // entries between two sequences' rows
+    uint32_t table_cols;
+    const int32_t *q_start;    // [n_seq + 1]
+    const int32_t *kv_len;     // [n_seq]
+    uint32_t n_seq, n_rows, n_head_kv, group, block_tokens, n_slots;
+    float scale_log2;          // scale * log2(e)
+    uint32_t causal;
+    AttendRows q, out;
+    uint8_t *work;             // split descriptors, then partial results
+    uint32_t align16;          // cache bases and row bytes are multiples of 16
+    uint32_t min_rows, max_rows;   // query rows (tokens * group) a sequence needs to be taken by this launch
+};
+
+// A sequence as the kernels see it; nothing read from device memory is trusted
+// to stay inside the tables.
+struct AttendSeq {
+    int32_t row0;              // first row of q / out
+    int32_t n_new;             // rows of this sequence inside [0, n_rows)
+    int32_t shift;             // causal: row i sees keys below shift + i + 1
+    int32_t keys;              // keys held by the table
+};
+
+__device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, uint32_t s) {
+    AttendSeq q;
+    const int64_t lo = a.q_start[s], hi = a.q_start[s + 1];
+    const int64_t kv = max(a.kv_len[s], 0);
+    const int64_t cap = static_cast<int64_t>(a.table_cols) * a.block_tokens;
+    const int64_t n = hi - lo;
+    q.row0 = static_cast<int32_t>(lo);
+    q.n_new = (lo < 0 || n <= 0 || lo >= a.n_rows)
+                  ? 0 : static_cast<int32_t>(min(n, static_cast<int64_t>(a.n_rows) - lo));
+    q.shift = static_cast<int32_t>(max(kv - n, static_cast<int64_t>(-0x40000000)));
+    q.keys = static_cast<int32_t>(min(kv, min(cap, static_cast<int64_t>(0x7fffff00))));
+    return q;
+}
+
+// Keys that row token i of the sequence sees.
+__device__ __forceinline__ int32_t attend_limit(const AttendArgs &a, const AttendSeq &q, int32_t i) {
+    if (!a.causal) return q.keys;
+    return max(0, min(q.keys, static_cast<int32_t>(min(static_cast<int64_t>(q.shift) + i + 1,
+                                                       static_cast<int64_t>(0x7fffff00)))));
+}
+
+__device__ __forceinline__ float load16(const uint8_t *p, int32_t bf16) {
+    const uint16_t u = *reinterpret_cast<const uint16_t *>(p);
+    return bf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(__ushort_as_half(u));
+}
+
+__device__ __forceinline__ void store16(uint8_t *p, float x, int32_t bf16) {
+    *reinterpret_cast<uint16_t *>(p) = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x))
+                                            : __half_as_ushort(__float2half_rn(x));
+}
+
+// D += A B on f16 operands with F32 accumulation, A 16x16, B 16x8.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                        const float (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
+                   "f"(c[2]), "f"(c[3]));
+}
+
+// Transpose of an 8x8 matrix of 16-bit values held two a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------- split bookkeeping --
+// The keys of every (sequence, row tile, KV head) are cut into steps of 16;
+// all steps of the call form one line that the CTAs share evenly, so ragged
+// batches balance without the host knowing a length.  A segment that one CTA
+// holds whole is written to `out`; one that several CTAs share leaves partial
+// results (max, sum, unnormalised output in F32) that attend_join_kernel adds
+// in CTA order.
+constexpr int kAttendStep = 16;
+constexpr uint32_t kAttendMaxCtas = 592;      // descriptors in the workspace
+constexpr uint32_t kAttendDescBytes = 32;
+struct AttendDesc {                           // segment that starts in CTA c and goes on in c + 1 ...
+    uint32_t parts;                           // 0 = none
+    int32_t row0;                             // first token row of the tile
+    uint32_t head;                            // KV head
+    uint32_t first;                           // first (token, group) row of the tile in the sequence
+    uint32_t rows;                            // rows of the tile
+    uint32_t pad[3];
+};
+static_assert(sizeof(AttendDesc) == kAttendDescBytes, "AttendDesc");
+
+template <int D, int NT>
+constexpr uint32_t attend_part_floats() { return 8u * NT * (D + 2u); }
+
+template <int D, int NT>
+__device__ __forceinline__ float *attend_part(uint8_t *work, uint32_t slot) {
+    return reinterpret_cast<float *>(work + kAttendMaxCtas * kAttendDescBytes) +
+           static_cast<uint64_t>(slot) * attend_part_floats<D, NT>();
+}
+
+// ------------------------------------------------------------ block codes --
+// Geometry of a head's slice of a row, by cache type.
+template <int T, int D>
+struct Slice {
+    static constexpr int kBlock = T == KVM_TYPE_F16 ? 64 : block_bytes(T);
+    static constexpr int kBytes = D / 32 * kBlock;
+    // shared-memory stride: an odd multiple of 16 bytes, so that eight rows'
+    // words fall into different banks
+    static constexpr int kUp = (kBytes + 15) / 16;
+    static constexpr int kStride = (kUp | 1) * 16;
+    static constexpr bool kNibble = T == KVM_TYPE_Q4_0 || T == KVM_TYPE_Q5_0;
+    // codes are stored unsigned; the value is (code - kOffset) * d
+    static constexpr int kOffset = T == KVM_TYPE_Q4_0 ? 8 : T == KVM_TYPE_Q5_0 ? 16 : T == KVM_TYPE_Q8_0 ? 128 : 0;
+    static constexpr int kOffsetLog = T == KVM_TYPE_Q4_0 ? 3 : T == KVM_TYPE_Q5_0 ? 4 : 7;
+};
+
+}  // namespace kvm

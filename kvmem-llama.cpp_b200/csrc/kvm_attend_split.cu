@@ -1,0 +1,40 @@
+// kvm_attend_split.cu -- the instances of attend_split_kernel for one head size
+// and K type (compiled once for each pair of KVM_ATTEND_D, KVM_ATTEND_KT).
+#include "kvm_attend_split.cuh"
+
+namespace kvm {
+namespace {
+
+template <int D, int KT, int VT, int NT>
+cudaError_t launch(const AttendArgs &a, uint32_t grid, cudaStream_t st) {
+    static std::atomic<uint64_t> attr{0};
+    constexpr int smem = attend_split_smem<D, KT, VT, NT>();
+    static_assert(smem <= 227 * 1024, "shared memory");
+    if (!attr_once(attr, reinterpret_cast<const void *>(attend_split_kernel<D, KT, VT, NT>), smem))
+        return cudaErrorInvalidValue;
+    attend_split_kernel<D, KT, VT, NT><<<grid, SplitGeom<D, KT, VT>::kThreads, smem, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || grid == 1) return e;
+    return launch_after_prev(attend_join_kernel<D, NT>, dim3(grid, 8 * NT), dim3(D), 0, st, a);
+}
+
+template <int D, int KT, int VT>
+cudaError_t launch_nt(const AttendArgs &a, int nt, uint32_t grid, cudaStream_t st) {
+    return nt == 1 ? launch<D, KT, VT, 1>(a, grid, st) : launch<D, KT, VT, 2>(a, grid, st);
+}
+
+}  // namespace
+
+template <int D, int KT>
+cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st) {
+    switch (vt) {
+        case KVM_TYPE_Q4_0: return launch_nt<D, KT, KVM_TYPE_Q4_0>(a, nt, grid, st);
+        case KVM_TYPE_Q5_0: return launch_nt<D, KT, KVM_TYPE_Q5_0>(a, nt, grid, st);
+        case KVM_TYPE_Q8_0: return launch_nt<D, KT, KVM_TYPE_Q8_0>(a, nt, grid, st);
+        default: return launch_nt<D, KT, KVM_TYPE_F16>(a, nt, grid, st);
+    }
+}
+template cudaError_t launch_attend_split<KVM_ATTEND_D, KVM_ATTEND_KT>(const AttendArgs &, int, int, uint32_t,
+                                                                      cudaStream_t);
+
+}  // namespace kvm

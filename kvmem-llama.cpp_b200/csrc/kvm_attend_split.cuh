@@ -1,0 +1,768 @@
+// kvm_attend_split.cuh -- attend_split_kernel: attention for few query rows a
+// sequence (decode steps, drafted tokens), bound by reading the window once.
+//
+// Mathematics.  With c the unsigned code of an element, o the type's offset and
+// d the scale of its block of 32 (q4_0: o = 8, q5_0: 16, q8_0: 128),
+//   q . k = sum_b d_b (sum_{e in b} q_e c_e) - o sum_b d_b (sum_{e in b} q_e)
+//   o_e   = sum_j (p_j d_jb) c_je - o sum_j (p_j d_jb)
+// so the tensor cores see the codes themselves and nothing is rounded by
+// dequantizing.  A code enters as the F16 bit pattern of its integer -- the
+// subnormal c * 2^-24, exact -- which costs one AND a pair of values and no
+// conversion; the factor 2^24 is taken out again in F32.  The second term of
+// q . k is one more product, scales (16 keys x blocks) times block sums of q
+// (an F16 value and its remainder); that of o_e a second product with the
+// constant -o for A.
+//
+// Rounding: q enters in F16, scaled by a power of two a row so that its largest
+// element is near the top of the range (exact for F16 and BF16 inputs but for
+// elements 2^17 below the row's largest); p and p*d are rounded to F16 (2^-11
+// relative, as the output type), sums and statistics are F32.  To use F16's
+// range, p is carried times 2^14 (which cancels in the quotient) and the scales
+// of V times the power of two that brings the largest met so far to [1, 2):
+// weights keep all bits down to 2^-28 of the row's largest.
+//
+// Layout.  S^T = K Q^T with 16 keys as M and 8 query rows as N, then
+// O^T = V^T P^T with dims as M: the few rows fill N = 8, codes are the A operand
+// straight from the rows' bytes, and P^T goes from the accumulators to the B
+// operand by one 8x8 transpose a half.  Which 16 elements of a block form one
+// K = 16 product is free as long as q agrees, so every lane takes the bytes of
+// one word.  A warp streams its own keys (16 a step) through its own
+// cp.async ring and keeps its own running maximum, sum and output; the warps
+// of a CTA meet once a segment.
+#pragma once
+
+#include "kvm_attend.cuh"
+
+namespace kvm {
+
+template <int D, int KT, int VT>
+struct SplitGeom {
+    using K = Slice<KT, D>;
+    using V = Slice<VT, D>;
+    static constexpr int kStage = kAttendStep * (K::kStride + V::kStride);
+    // eight warps unless two stages of each no longer fit
+    static constexpr int kWarps = 16 * kStage <= 210 * 1024 ? 8 : 4;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kBudget = 196 * 1024 / (kWarps * kStage);
+    static constexpr int kStages = kBudget > 6 ? 6 : kBudget < 2 ? 2 : kBudget;
+    static constexpr int kScaleBytes = 1024;      // per warp: K f16, K f32, V f16
+    static constexpr int kRing = kWarps * kStages * kStage;
+};
+
+template <int D, int NT>
+constexpr int attend_merge_bytes(int warps) { return warps * 8 * NT * (D + 4 + 2) * 4; }
+
+template <int D, int KT, int VT, int NT>
+constexpr int attend_split_smem() {
+    using G = SplitGeom<D, KT, VT>;
+    const int merge = attend_merge_bytes<D, NT>(G::kWarps), big = G::kRing > merge ? G::kRing : merge;
+    return big + G::kWarps * (G::kScaleBytes + G::kStages * 4) + 64;
+}
+
+__device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
+__device__ __forceinline__ uint32_t lds16(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
+
+__device__ __forceinline__ uint32_t pack_half2(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// The codes that lane (g, t) supplies of a row's block pair `p` as A operands
+// of K: w[b][m] holds the two registers (k = 2t.. and k = 2t+8..) of block
+// 2p + b, product m.  Elements (q4_0, q5_0): m = 0: 4t, 4t+2 | 4t+1, 4t+3;
+// m = 1: the same + 16, times 16.  (q8_0, F16): m: 8t+4m, +1 | +2, +3.
+template <int KT>
+__device__ __forceinline__ void k_codes(const uint8_t *pair, int t, uint32_t (&w)[2][2][2]) {
+    constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+    if constexpr (KT == KVM_TYPE_Q4_0) {
+        const uint32_t x0 = __byte_perm(lds32(pair + 4 * t), lds32(pair + 4 * t + 4), 0x5432);
+        const uint32_t x1 = lds32(pair + 20 + 4 * t);
+        w[0][0][0] = x0 & kLo; w[0][0][1] = (x0 >> 8) & kLo;
+        w[0][1][0] = x0 & kHi; w[0][1][1] = (x0 >> 8) & kHi;
+        w[1][0][0] = x1 & kLo; w[1][0][1] = (x1 >> 8) & kLo;
+        w[1][1][0] = x1 & kHi; w[1][1][1] = (x1 >> 8) & kHi;
+    } else if constexpr (KT == KVM_TYPE_Q5_0) {
+        const uint32_t h[2] = {__byte_perm(lds32(pair), lds32(pair + 4), 0x5432) >> (4 * t),
+                               lds32(pair + 24) >> (4 * t)};
+        const uint32_t x[2] = {__byte_perm(lds32(pair + 4 + 4 * t), lds32(pair + 8 + 4 * t), 0x5432),
+                               lds32(pair + 28 + 4 * t)};
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint32_t hl = h[b], hh = h[b] >> 16;
+            // bit i of the low half-word is element 4t + i's fifth bit: spread
+            // bits 0, 2 (and 1, 3) to bits 4 and 20, those of +16 to 8 and 24
+            w[b][0][0] = (x[b] & kLo) | (((hl & 5u) * 0x00040010u) & 0x00100010u);
+            w[b][0][1] = ((x[b] >> 8) & kLo) | (((hl & 10u) * 0x00020008u) & 0x00100010u);
+            w[b][1][0] = (x[b] & kHi) | (((hh & 5u) * 0x00400100u) & 0x01000100u);
+            w[b][1][1] = ((x[b] >> 8) & kHi) | (((hh & 10u) * 0x00200080u) & 0x01000100u);
+        }
+    } else if constexpr (KT == KVM_TYPE_Q8_0) {
+        const uint32_t a0 = lds32(pair + 8 * t), a1 = lds32(pair + 8 * t + 4), a2 = lds32(pair + 8 * t + 8);
+        const uint32_t x[2][2] = {{__byte_perm(a0, a1, 0x5432) ^ 0x80808080u, __byte_perm(a1, a2, 0x5432) ^ 0x80808080u},
+                                  {lds32(pair + 36 + 8 * t) ^ 0x80808080u, lds32(pair + 40 + 8 * t) ^ 0x80808080u}};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                w[b][m][0] = __byte_perm(x[b][m], 0u, 0x4140);
+                w[b][m][1] = __byte_perm(x[b][m], 0u, 0x4342);
+            }
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(pair + 64 * b + 16 * t);
+            w[b][0][0] = x.x; w[b][0][1] = x.y; w[b][1][0] = x.z; w[b][1][1] = x.w;
+        }
+    }
+}
+
+// Element of a 32-block that register r (0..3: product r >> 1, register r & 1)
+// holds in half i, for lane t of a K row.
+template <int KT>
+__device__ __forceinline__ constexpr int k_elem(int t, int r, int i) {
+    return Slice<KT, 64>::kNibble ? 4 * t + 2 * i + (r & 1) + 16 * (r >> 1) : 8 * t + 2 * r + i;
+}
+
+// V: lane (g, t) supplies dims of rows g and g + 8 of two M = 16 tiles of block
+// b for the keys 2t, 2t+1 (x0, x1) packed in one register: r[tile][half].
+// Dims (q4_0, q5_0): 2g, 2g+1 | 16+2g, 16+2g+1 (times 16); (q8_0, F16): 4g .. 4g+3.
+template <int VT>
+__device__ __forceinline__ void v_codes(const uint8_t *row0, const uint8_t *row1, int b, int g, uint32_t (&r)[2][2]) {
+    constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+    constexpr int kB = Slice<VT, 64>::kBlock;
+    const uint8_t *p0 = row0 + b * kB, *p1 = row1 + b * kB;
+    if constexpr (VT == KVM_TYPE_Q4_0 || VT == KVM_TYPE_Q5_0) {
+        const uint32_t u = lds16(p0 + kB - 16 + 2 * g) | (lds16(p1 + kB - 16 + 2 * g) << 16);
+        r[0][0] = u & kLo;
+        r[0][1] = (u >> 8) & kLo;
+        r[1][0] = u & kHi;
+        r[1][1] = (u >> 8) & kHi;
+        if constexpr (VT == KVM_TYPE_Q5_0) {
+            const uint32_t l = (lds16(p0 + 2) >> (2 * g)) | ((lds16(p1 + 2) >> (2 * g)) << 16);
+            const uint32_t h = (lds16(p0 + 4) >> (2 * g)) | ((lds16(p1 + 4) >> (2 * g)) << 16);
+            r[0][0] |= (l << 4) & 0x00100010u;
+            r[0][1] |= (l << 3) & 0x00100010u;
+            r[1][0] |= (h << 8) & 0x01000100u;
+            r[1][1] |= (h << 7) & 0x01000100u;
+        }
+    } else if constexpr (VT == KVM_TYPE_Q8_0) {
+        const uint32_t l = (lds16(p0 + 2 + 4 * g) | (lds16(p1 + 2 + 4 * g) << 16)) ^ 0x80808080u;
+        const uint32_t h = (lds16(p0 + 4 + 4 * g) | (lds16(p1 + 4 + 4 * g) << 16)) ^ 0x80808080u;
+        r[0][0] = l & 0x00ff00ffu;
+        r[0][1] = (l >> 8) & 0x00ff00ffu;
+        r[1][0] = h & 0x00ff00ffu;
+        r[1][1] = (h >> 8) & 0x00ff00ffu;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p0 + 8 * g), y = *reinterpret_cast<const uint2 *>(p1 + 8 * g);
+        r[0][0] = __byte_perm(x.x, y.x, 0x5410);
+        r[0][1] = __byte_perm(x.x, y.x, 0x7632);
+        r[1][0] = __byte_perm(x.y, y.y, 0x5410);
+        r[1][1] = __byte_perm(x.y, y.y, 0x7632);
+    }
+}
+
+// Dim of block b that tile `tile`, row half `h` holds for lane g.
+template <int VT>
+__device__ __forceinline__ constexpr int v_dim(int b, int tile, int h, int g) {
+    return 32 * b + (Slice<VT, 64>::kNibble ? 16 * tile + 2 * g + h : 4 * g + 2 * tile + h);
+}
+
+// One value of a row slice in shared memory, by its definition.
+template <int T>
+__device__ __forceinline__ float row_value(const uint8_t *row, int e) {
+    if constexpr (T == KVM_TYPE_F16) {
+        return __half2float(*reinterpret_cast<const __half *>(row + 2 * e));
+    } else {
+        constexpr int kB = Slice<T, 64>::kBlock;
+        const uint8_t *p = row + e / 32 * kB;
+        const float d = __half2float(*reinterpret_cast<const __half *>(p));
+        const int i = e % 32;
+        if constexpr (T == KVM_TYPE_Q8_0) return d * static_cast<float>(static_cast<int8_t>(p[2 + i]));
+        const uint32_t byte = p[kB - 16 + (i & 15)];
+        int c = static_cast<int>(i < 16 ? byte & 15u : byte >> 4);
+        if constexpr (T == KVM_TYPE_Q5_0) c |= static_cast<int>((p[2 + i / 8] >> (i & 7)) & 1u) << 4;
+        return d * static_cast<float>(c - Slice<T, 64>::kOffset);
+    }
+}
+
+template <int D, int KT, int VT, int NT>
+__global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_split_kernel(const __grid_constant__ AttendArgs a) {
+    using G = SplitGeom<D, KT, VT>;
+    using SK = Slice<KT, D>;
+    using SV = Slice<VT, D>;
+    constexpr int NB = D / 32, W = G::kWarps, kThreads = G::kThreads, NS = G::kStages, R = 8 * NT;
+    constexpr bool kCodesK = KT != KVM_TYPE_F16, kCodesV = VT != KVM_TYPE_F16;
+    constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 14.0f;
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kMerge = attend_merge_bytes<D, NT>(W), kBig = G::kRing > kMerge ? G::kRing : kMerge;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    uint8_t *ring = smem + warp * NS * G::kStage;
+    uint8_t *scales = smem + kBig + warp * G::kScaleBytes;
+    __half *k16 = reinterpret_cast<__half *>(scales);              // [16 keys][8 blocks]
+    float *k32 = reinterpret_cast<float *>(scales + 256);          // [16][8]
+    __half *v16 = reinterpret_cast<__half *>(scales + 768);        // [8 blocks][16 keys, a lane's four together]
+    uint32_t *valid = reinterpret_cast<uint32_t *>(smem + kBig + W * G::kScaleBytes) + warp * NS;
+    __shared__ unsigned long long s_scan[W], s_total;
+    __shared__ unsigned long long s_off;
+    __shared__ uint32_t s_seq;
+
+    // ---- this CTA's share of the line of steps
+    auto units = [&](uint32_t s) -> unsigned long long {
+        const AttendSeq q = attend_seq(a, s);
+        const uint64_t rows = static_cast<uint64_t>(q.n_new) * a.group;
+        if (q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) return 0ull;
+        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kAttendStep - 1u) / kAttendStep);
+        return ((rows + R - 1) / R) * a.n_head_kv * steps;
+    };
+    if (tid == 0) s_total = 0;
+    unsigned long long mine = 0;
+    for (uint32_t s = tid; s < a.n_seq; s += kThreads) mine += units(s);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    __syncthreads();
+    if (lane == 0) atomicAdd(&s_total, mine);
+    __syncthreads();
+    const unsigned long long total = s_total;
+    unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
+    if (share < static_cast<unsigned long long>(W)) share = W;
+    const unsigned long long u0 = share * blockIdx.x;
+    const unsigned long long u1 = min(u0 + share, total);
+    AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
+    if (u0 >= total) {
+        if (tid == 0) desc->parts = 0;
+        return;
+    }
+    unsigned long long carry = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += kThreads) {
+        const uint32_t s = base + tid;
+        const unsigned long long n = s < a.n_seq ? units(s) : 0ull;
+        unsigned long long x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        unsigned long long before = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) before += s_scan[w];
+            all += s_scan[w];
+        }
+        x += before;
+        if (n != 0 && x - n <= u0 && u0 < x) {
+            s_seq = s;
+            s_off = u0 - (x - n);
+        }
+        carry += all;
+        __syncthreads();
+        if (carry > u0) break;
+    }
+    uint32_t seq = s_seq;
+    unsigned long long off = s_off;
+    bool described = false;
+
+    for (unsigned long long pos = u0; pos < u1;) {
+        // ---- the segment at `pos`
+        AttendSeq q = attend_seq(a, seq);
+        {
+            const unsigned long long n = units(seq);
+            if (off >= n) {
+                off = 0;
+                ++seq;
+                continue;
+            }
+        }
+        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kAttendStep - 1u) / kAttendStep);
+        const uint32_t seg = static_cast<uint32_t>(off / steps);
+        const uint32_t in0 = static_cast<uint32_t>(off - static_cast<unsigned long long>(seg) * steps);
+        const uint32_t left = steps - in0;
+        const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(left), u1 - pos));
+        const uint32_t head = seg % a.n_head_kv;
+        const uint32_t first = seg / a.n_head_kv * R;
+        const uint32_t all_rows = static_cast<uint32_t>(q.n_new) * a.group;
+        const uint32_t rows = min(static_cast<uint32_t>(R), all_rows - first);
+        const int32_t kend = attend_limit(a, q, (first + rows - 1) / a.group);
+        const int32_t kfull = attend_limit(a, q, first / a.group);      // every row sees the keys below
+
+        // ---- q of this lane's columns: row first + nt*8 + g
+        uint32_t qf[NT][NB][4];
+        uint32_t qc[NT][2];
+        float fac[NT][2];
+        int32_t lim[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t r = first + nt * 8 + g;
+            const bool in = r < first + rows;
+            const uint32_t tok = r / a.group;
+            const uint8_t *qp = a.q.p + (static_cast<uint64_t>(q.row0) + (in ? tok : 0)) * a.q.nb_tok +
+                                (static_cast<uint64_t>(head) * a.group + (in ? r % a.group : 0)) * a.q.nb_head;
+            float x[NB][4][2], top = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[b][k][i] = in ? load16(qp + (32 * b + k_elem<KT>(t, k, i)) * a.q.nb_dim, a.q.bf16) : 0.0f;
+                        top = fmaxf(top, fabsf(x[b][k][i]));
+                    }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // largest element to [2^(9-o), 2^(10-o)), o = log2(offset): the sums of 32
+            // elements times the offset stay in F16
+            const int want = kCodesK ? 9 - SK::kOffsetLog : 9;
+            const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
+            // two steps: a factor of 2^(want - e) alone may be out of F32's range
+            const int up = (top > 0.0f && e < 128) ? max(-126, min(126, want - e)) : 0;
+            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+            uint32_t hi[NB / 2 ? NB / 2 : 1], lo[NB / 2 ? NB / 2 : 1];
+            float sums[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float part = (SK::kNibble && k >= 2) ? 0.0625f : 1.0f;
+                    const uint32_t h = pack_half2(x[b][k][0] * mul * part, x[b][k][1] * mul * part);
+                    qf[nt][b][k] = h;
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+                    sum += (back.x + back.y) / part;
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sums[b] = -static_cast<float>(SK::kOffset) * sum;
+            }
+            qc[nt][0] = qc[nt][1] = 0;
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                hi[b / 2] = pack_half2(sums[b], sums[b + 1]);
+                const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi[b / 2]));
+                lo[b / 2] = pack_half2(sums[b] - back.x, sums[b + 1] - back.y);
+                if (t == b / 2) {
+                    qc[nt][0] = hi[b / 2];
+                    qc[nt][1] = lo[b / 2];
+                }
+            }
+            // columns 2t, 2t+1 of the accumulators: their factor and limit
+            const float f = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            const int32_t l = in ? attend_limit(a, q, static_cast<int32_t>(tok)) : kend;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fac[nt][i] = __shfl_sync(0xffffffffu, f, (2 * t + i) * 4);
+                lim[nt][i] = __shfl_sync(0xffffffffu, l, (2 * t + i) * 4);
+            }
+        }
+
+        float o[NT][NB][2][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = kNegInf;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][b][0][i] = o[nt][b][1][i] = 0.0f;
+        }
+        int vexp = 15;                        // o holds the output times 2^(vexp - 24)
+
+        // ---- the warp's steps: in0 + warp, + W, ...
+        const uint32_t kstart = in0 * kAttendStep;
+        const uint32_t in1 = min(in0 + take, (static_cast<uint32_t>(kend) + kAttendStep - 1u) / kAttendStep);
+        const int n_steps = in1 > in0 + warp ? static_cast<int>((in1 - in0 - warp + W - 1) / W) : 0;
+        const int32_t *trow = a.table + seq * a.table_stride;
+        const uint8_t *kbase = a.k + static_cast<uint64_t>(head) * SK::kBytes;
+        const uint8_t *vbase = a.v + static_cast<uint64_t>(head) * SV::kBytes;
+
+        auto load = [&](int i) {
+            uint8_t *st = ring + (i % NS) * G::kStage;
+            const uint32_t key = kstart + (warp + i * W) * kAttendStep + (lane & 15);
+            int32_t cell = -1;
+            if (key < static_cast<uint32_t>(kend)) {
+                const uint32_t blk = key / a.block_tokens;
+                const int32_t slot = trow[blk];
+                if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
+                    cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
+            }
+            const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
+            if (lane == 0) valid[i % NS] = ok;
+            auto copy = [&](auto slice, uint8_t *dst, const uint8_t *base, uint64_t row_bytes) {
+                using S = decltype(slice);
+                auto pieces = [&](auto width) {
+                    constexpr int V = decltype(width)::value, C = S::kBytes / V;
+#pragma unroll 9
+                    for (int y = 0; y < (kAttendStep * C + 31) / 32; ++y) {
+                        const int x = lane + 32 * y, r = min(x / C, kAttendStep - 1), c = x - r * C;
+                        const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
+                        const uint8_t *src = base + (cr >= 0 ? cr * row_bytes + c * V : 0ull);
+                        const uint32_t d = smem_u32(dst + r * S::kStride + c * V);
+                        if (x < kAttendStep * C) {
+                            if constexpr (V == 16) cp_async16(d, src, cr >= 0 ? 16u : 0u);
+                            else cp_async4(d, src, cr >= 0 ? 4u : 0u);
+                        }
+                    }
+                };
+                if constexpr (S::kBytes % 16 == 0) {
+                    if (a.align16) {
+                        pieces(std::integral_constant<int, 16>{});
+                        return;
+                    }
+                }
+                pieces(std::integral_constant<int, 4>{});
+            };
+            copy(SK{}, st, kbase, a.row_k);
+            copy(SV{}, st + kAttendStep * SK::kStride, vbase, a.row_v);
+        };
+
+#pragma unroll 1
+        for (int i = 0; i < NS - 1; ++i) {
+            if (i < n_steps) load(i);
+            cp_async_commit();
+        }
+#pragma unroll 1
+        for (int i = 0; i < n_steps; ++i) {
+            cp_async_wait<NS - 2>();
+            __syncwarp();
+            if (i + NS - 1 < n_steps) load(i + NS - 1);
+            cp_async_commit();
+            const uint8_t *kr = ring + (i % NS) * G::kStage;
+            const uint8_t *vr = kr + kAttendStep * SK::kStride;
+            const int32_t key0 = static_cast<int32_t>(kstart + (warp + i * W) * kAttendStep);
+            const uint32_t ok = valid[i % NS];
+
+            // ---- the step's scales, laid out for the products
+            bool odd_values = false;          // an infinite or NaN V value
+            if constexpr (kCodesK) {
+#pragma unroll
+                for (int x = lane; x < 16 * NB; x += 32) {
+                    const int key = x & 15, b = x >> 4;
+                    const __half d = *reinterpret_cast<const __half *>(kr + key * SK::kStride + b * SK::kBlock);
+                    k16[key * 8 + b] = d;
+                    k32[key * 8 + b] = __half2float(d);
+                }
+            }
+            if constexpr (kCodesV) {
+                uint32_t d[NB / 2], top = 0;
+#pragma unroll
+                for (int y = 0; y < NB / 2; ++y) {
+                    const int x = lane + 32 * y;
+                    d[y] = lds16(vr + (x & 15) * SV::kStride + (x >> 4) * SV::kBlock);
+                    top = max(top, d[y] & 0x7fffu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                odd_values = top >= 0x7c00u;
+                const int need = min(15, 15 - static_cast<int>(min(top, 0x7bffu) >> 10));
+                if (need < vexp) {            // the largest scale so far to [1, 2)
+                    const float f = __uint_as_float(static_cast<uint32_t>(need - vexp + 127) << 23);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                o[nt][b][0][j] *= f;
+                                o[nt][b][1][j] *= f;
+                            }
+                    vexp = need;
+                }
+                const __half mul = vexp >= -14 ? __ushort_as_half(static_cast<uint16_t>((vexp + 15) << 10))
+                                               : __ushort_as_half(static_cast<uint16_t>(0x0200u));   // 2^-15
+#pragma unroll
+                for (int y = 0; y < NB / 2; ++y) {
+                    const int x = lane + 32 * y, key = x & 15;
+                    const int at = (key & 6) * 2 + (key & 1) + (key >> 3) * 2;
+                    v16[(x >> 4) * 16 + at] = __hmul(__ushort_as_half(static_cast<uint16_t>(d[y])), mul);
+                }
+            }
+            __syncwarp();
+
+            // ---- S^T = K Q^T
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const uint8_t *row0 = kr + g * SK::kStride, *row1 = row0 + 8 * SK::kStride;
+#pragma unroll
+            for (int p = 0; p < NB / 2; ++p) {
+                uint32_t c0[2][2][2], c1[2][2][2];
+                k_codes<KT>(row0 + p * 2 * SK::kBlock, t, c0);
+                k_codes<KT>(row1 + p * 2 * SK::kBlock, t, c1);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t a0[4] = {c0[b][0][0], c1[b][0][0], c0[b][0][1], c1[b][0][1]};
+                    const uint32_t a1[4] = {c0[b][1][0], c1[b][1][0], c0[b][1][1], c1[b][1][1]};
+                    float d0 = 1.0f, d1 = 1.0f;
+                    if constexpr (kCodesK) {
+                        d0 = k32[g * 8 + 2 * p + b];
+                        d1 = k32[(g + 8) * 8 + 2 * p + b];
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t *qq = qf[nt][2 * p + b];
+                        if constexpr (kCodesK) {
+                            float part[4];
+                            mma_f16(part, a0, qq[0], qq[1], zero);
+                            mma_f16(part, a1, qq[2], qq[3], part);
+                            s[nt][0] = fmaf(d0, part[0], s[nt][0]);
+                            s[nt][1] = fmaf(d0, part[1], s[nt][1]);
+                            s[nt][2] = fmaf(d1, part[2], s[nt][2]);
+                            s[nt][3] = fmaf(d1, part[3], s[nt][3]);
+                        } else {
+                            mma_f16(s[nt], a0, qq[0], qq[1], s[nt]);
+                            mma_f16(s[nt], a1, qq[2], qq[3], s[nt]);
+                        }
+                    }
+                }
+            }
+            if constexpr (kCodesK) {
+                const bool has = 2 * t < NB;
+                const uint32_t w0 = has ? *reinterpret_cast<const uint32_t *>(k16 + g * 8 + 2 * t) : 0u;
+                const uint32_t w1 = has ? *reinterpret_cast<const uint32_t *>(k16 + (g + 8) * 8 + 2 * t) : 0u;
+                const uint32_t aw[4] = {w0, w1, w0, w1};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float c[4];
+                    mma_f16(c, aw, qc[nt][0], qc[nt][1], zero);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[nt][j] = fmaf(s[nt][j], 16777216.0f, c[j]);
+                }
+            }
+
+            // ---- softmax step
+            const bool mixed = key0 + kAttendStep > kfull || ok != 0xffffu;
+            uint32_t pb[NT][2];
+            float pr[NT][4];
+            bool grew = false;
+            float mn[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[nt][j] *= fac[nt][j & 1];
+                    if (mixed) {
+                        const int kk = g + (j >> 1) * 8;
+                        if (key0 + kk >= lim[nt][j & 1] || !((ok >> kk) & 1u)) s[nt][j] = kNegInf;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float x = fmaxf(s[nt][i], s[nt][i + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    mn[nt][i] = fmaxf(m[nt][i], x);
+                    grew = grew || mn[nt][i] > m[nt][i];
+                }
+            }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float f[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        f[i] = mn[nt][i] > m[nt][i] ? exp2_approx(m[nt][i] - mn[nt][i]) : 1.0f;
+                        l[nt][i] *= f[i];
+                        m[nt][i] = mn[nt][i];
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[nt][b][0][j] *= f[j & 1];
+                            o[nt][b][1][j] *= f[j & 1];
+                        }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float mm = m[nt][j & 1] == kNegInf ? 0.0f : m[nt][j & 1] - kWeightLog;
+                    pr[nt][j] = exp2_approx(s[nt][j] - mm);
+                    l[nt][j & 1] += pr[nt][j];
+                }
+                pb[nt][0] = transpose8(pack_half2(pr[nt][0], pr[nt][1]));
+                pb[nt][1] = transpose8(pack_half2(pr[nt][2], pr[nt][3]));
+            }
+
+            if constexpr (!kCodesV) {
+                if (mixed) {                  // a hidden key's infinity must not meet p = 0 in a product
+                    for (int x = lane; x < 16 * (D / 2); x += 32) {
+                        const uint32_t u = lds32(vr + (x & 15) * SV::kStride + (x >> 4) * 4);
+                        odd_values = odd_values || (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
+                    }
+                    odd_values = __any_sync(0xffffffffu, odd_values);
+                }
+            }
+
+            // ---- O^T += V^T P^T
+            if (!odd_values) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t x[2][2], y[2][2];
+                    v_codes<VT>(vr + 2 * t * SV::kStride, vr + (2 * t + 1) * SV::kStride, b, g, x);
+                    v_codes<VT>(vr + (2 * t + 8) * SV::kStride, vr + (2 * t + 9) * SV::kStride, b, g, y);
+                    uint2 ds = make_uint2(0u, 0u);
+                    if constexpr (kCodesV) ds = *reinterpret_cast<const uint2 *>(v16 + b * 16 + 4 * t);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t b0 = pb[nt][0], b1 = pb[nt][1];
+                        if constexpr (kCodesV) {
+                            b0 = mul_half2(b0, ds.x);
+                            b1 = mul_half2(b1, ds.y);
+                        }
+#pragma unroll
+                        for (int tile = 0; tile < 2; ++tile) {
+                            const uint32_t av[4] = {x[tile][0], x[tile][1], y[tile][0], y[tile][1]};
+                            mma_f16(o[nt][b][tile], av, b0, b1, o[nt][b][tile]);
+                            if constexpr (kCodesV) {
+                                // the constant -offset (times 16 in the high-nibble tile) * 2^-24
+                                constexpr uint32_t c0 = 0x8000u | SV::kOffset;
+                                constexpr uint32_t c1 = 0x8000u | (SV::kNibble ? 16 * SV::kOffset : SV::kOffset);
+                                const uint32_t cc = tile ? c1 * 0x10001u : c0 * 0x10001u;
+                                const uint32_t ac[4] = {cc, cc, cc, cc};
+                                mma_f16(o[nt][b][tile], ac, b0, b1, o[nt][b][tile]);
+                            }
+                        }
+                    }
+                }
+            } else {
+                // values that are not finite: by the definition, p = 0 leaves them out
+                const float unit = kCodesV ? __uint_as_float(static_cast<uint32_t>(vexp - 24 + 127) << 23) : 1.0f;
+#pragma unroll 1
+                for (int k = 0; k < 16; ++k) {
+                    const uint8_t *row = vr + k * SV::kStride;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const int from = (k & 7) * 4 + t;
+                        const float p0 = __shfl_sync(0xffffffffu, k < 8 ? pr[nt][0] : pr[nt][2], from);
+                        const float p1 = __shfl_sync(0xffffffffu, k < 8 ? pr[nt][1] : pr[nt][3], from);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const float up = SV::kNibble && tile ? 16.0f : 1.0f;
+                                    const float v = row_value<VT>(row, v_dim<VT>(b, tile, h, g)) * unit * up;
+                                    if (p0 != 0.0f) o[nt][b][tile][2 * h] += p0 * v;
+                                    if (p1 != 0.0f) o[nt][b][tile][2 * h + 1] += p1 * v;
+                                }
+                    }
+                }
+            }
+        }
+
+        // ---- the warps' results together
+        cp_async_wait<0>();
+        __syncthreads();
+        float *sm_m = reinterpret_cast<float *>(smem), *sm_l = sm_m + W * R, *sm_o = sm_l + W * R;
+        constexpr int OS = D + 4;
+        const float unit = kCodesV ? __uint_as_float(static_cast<uint32_t>(24 - vexp + 127) << 23) : 1.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x = l[nt][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int col = nt * 8 + 2 * t + i;
+                if (g == 0) {
+                    sm_m[warp * R + col] = m[nt][i];
+                    sm_l[warp * R + col] = x;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float up = SV::kNibble && tile ? 0.0625f : 1.0f;
+                        sm_o[(warp * R + nt * 8 + 2 * t + (j & 1)) * OS + v_dim<VT>(b, tile, j >> 1, g)] =
+                            o[nt][b][tile][j] * unit * up;
+                    }
+        }
+        __syncthreads();
+        const bool starts = in0 == 0, ends = take == left;
+        float *part = nullptr;
+        if (!starts || !ends) part = attend_part<D, NT>(a.work, 2u * blockIdx.x + (starts ? 1u : 0u));
+        for (int x = tid; x < static_cast<int>(rows) * D; x += kThreads) {
+            const int r = x / D, d = x - r * D;
+            float top = kNegInf;
+#pragma unroll
+            for (int w = 0; w < W; ++w) top = fmaxf(top, sm_m[w * R + r]);
+            const float ref = top == kNegInf ? 0.0f : top;
+            float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float f = exp2_approx(sm_m[w * R + r] - ref);
+                sum += f * sm_l[w * R + r];
+                acc += f * sm_o[(w * R + r) * OS + d];
+            }
+            if (part) {
+                if (d == 0) {
+                    part[r] = top;
+                    part[R + r] = sum;
+                }
+                part[2 * R + r * D + d] = acc;
+            } else {
+                const uint32_t rr = first + r, tok = rr / a.group;
+                store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(q.row0) + tok) * a.out.nb_tok +
+                            (static_cast<uint64_t>(head) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
+                        sum == 0.0f ? 0.0f : acc / sum, a.out.bf16);
+            }
+        }
+        if (starts && !ends && tid == 0) {
+            desc->row0 = q.row0;
+            desc->head = head;
+            desc->first = first;
+            desc->rows = rows;
+            desc->parts = 1u + static_cast<uint32_t>((pos + left - u1 + share - 1) / share);
+        }
+        described = described || (starts && !ends);
+        __syncthreads();
+        pos += take;
+        off += take;
+    }
+    if (!described && tid == 0) desc->parts = 0;
+    pdl_launch_dependents();
+}
+
+// One (split segment, row) a CTA, one dim a thread: the parts of a segment that
+// starts in CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...
+template <int D, int NT>
+__global__ void __launch_bounds__(D) attend_join_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int R = 8 * NT;
+    pdl_wait();
+    const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + blockIdx.x;
+    const uint32_t parts = desc->parts, r = blockIdx.y;
+    if (parts == 0 || r >= desc->rows) return;
+    const int d = threadIdx.x;
+    float top = -__builtin_huge_valf();
+    for (uint32_t i = 0; i < parts; ++i)
+        top = fmaxf(top, attend_part<D, NT>(a.work, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u)[r]);
+    const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
+    float sum = 0.0f, acc = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < parts; ++i) {
+        const float *p = attend_part<D, NT>(a.work, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u);
+        const float f = exp2_approx(p[r] - ref);
+        sum += f * p[R + r];
+        acc += f * p[2 * R + r * D + d];
+    }
+    const uint32_t rr = desc->first + r, tok = rr / a.group;
+    store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
+                (static_cast<uint64_t>(desc->head) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
+            sum == 0.0f ? 0.0f : acc / sum, a.out.bf16);
+}
+
+}  // namespace kvm

@@ -1,0 +1,220 @@
+// kvm_rows.cu -- kvm_write_rows and kvm_read_rows: rows of values into and out
+// of the cells of a cache, as ggml blocks.
+//
+// Write: the quantizers' definition in 32 bits with IEEE operations and no
+// contraction (kvm_quant.cuh has the formulas), so the bytes are those of
+// ggml's quantize_row_*_ref and of the stage-in.  Read: code * scale, exact in
+// F32, rounded once to the output's type.
+//
+// Both are HBM- or latency-bound streams over 32-value blocks.
+#include <cuda_bf16.h>
+
+#include "kvm_layer.cuh"
+
+namespace kvm {
+namespace {
+
+constexpr int kRowsThreads = 256;
+
+struct RowsSide {
+    uint8_t *cache;
+    uint8_t *act;                  // source rows (write) or destination rows (read)
+    uint64_t nb_dim, nb_head, nb_tok;
+    uint64_t row_bytes;
+    int32_t cache_type;
+    uint32_t on;
+};
+
+struct RowsArgs {
+    RowsSide side[2];
+    const int64_t *cells;
+    int64_t n_cells;
+    uint32_t n, blocks, head_dim;  // blocks of 32 a row
+};
+
+template <int TYPE>
+__device__ __forceinline__ float act_load(const uint8_t *p) {
+    if constexpr (TYPE == KVM_TYPE_F32) return *reinterpret_cast<const float *>(p);
+    else if constexpr (TYPE == KVM_TYPE_F16) return __half2float(*reinterpret_cast<const __half *>(p));
+    else return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(p)) << 16);
+}
+
+template <int TYPE>
+__device__ __forceinline__ void act_store(uint8_t *p, float x) {
+    if constexpr (TYPE == KVM_TYPE_F32) *reinterpret_cast<float *>(p) = x;
+    else if constexpr (TYPE == KVM_TYPE_F16) *reinterpret_cast<__half *>(p) = __float2half_rn(x);
+    else *reinterpret_cast<__nv_bfloat16 *>(p) = __float2bfloat16_rn(x);
+}
+
+// Byte offset of block b's first value in a row of heads.
+__device__ __forceinline__ uint64_t block_offset(const RowsSide &s, uint32_t head_dim, uint32_t b) {
+    const uint32_t e = b * 32u, h = e / head_dim;
+    return h * s.nb_head + (e - h * head_dim) * s.nb_dim;
+}
+
+// One block of 32 values to ggml bytes, in order.
+__device__ __forceinline__ void write_block(const float (&x)[32], int32_t type, uint8_t *dst) {
+    if (type == KVM_TYPE_F16) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) st_u16(dst + 2 * i, f16_bits(x[i]));
+        return;
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    if (type == KVM_TYPE_Q8_0) {
+        const float d = div127(amax), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+        st_u16(dst, f16_bits(d));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t lo = static_cast<uint32_t>(round_half_away(__fmul_rn(x[2 * i], id))) & 255u;
+            const uint32_t hi = static_cast<uint32_t>(round_half_away(__fmul_rn(x[2 * i + 1], id))) & 255u;
+            st_u16(dst + 2 + 2 * i, lo | hi << 8);
+        }
+        return;
+    }
+    float vmax = 0.0f;                       // the first value of the largest magnitude
+#pragma unroll
+    for (int i = 31; i >= 0; --i) vmax = fabsf(x[i]) == amax ? x[i] : vmax;
+    const bool q5 = type == KVM_TYPE_Q5_0;
+    const float d = __fmul_rn(vmax, q5 ? -0.0625f : -0.125f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+    const float off = q5 ? 16.5f : 8.5f;
+    const int top = q5 ? 31 : 15;
+    st_u16(dst, f16_bits(d));
+    uint32_t fifth = 0;
+    uint8_t *qs = dst + (q5 ? 6 : 2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t c[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {        // values 2i, 2i+1, and their partners 16 further on
+            const int e = 2 * i + (k & 1) + (k >> 1) * 16;
+            c[k] = static_cast<uint32_t>(min(top, __float2int_rz(__fadd_rn(__fmul_rn(x[e], id), off))));
+            fifth |= ((c[k] >> 4) & 1u) << e;
+        }
+        st_u16(qs + 2 * i, (c[0] & 15u) | (c[2] & 15u) << 4 | (c[1] & 15u) << 8 | (c[3] & 15u) << 12);
+    }
+    if (q5) {
+        st_u16(dst + 2, fifth & 0xffffu);
+        st_u16(dst + 4, fifth >> 16);
+    }
+}
+
+// A thread a block; blocks of a row are neighbours.
+template <int TYPE>
+__global__ void __launch_bounds__(kRowsThreads) write_rows_kernel(const __grid_constant__ RowsArgs a) {
+    const RowsSide &s = a.side[blockIdx.y];
+    if (!s.on) return;
+    const uint64_t all = static_cast<uint64_t>(a.n) * a.blocks;
+    for (uint64_t i = blockIdx.x * static_cast<uint64_t>(kRowsThreads) + threadIdx.x; i < all;
+         i += static_cast<uint64_t>(gridDim.x) * kRowsThreads) {
+        const uint32_t row = static_cast<uint32_t>(i / a.blocks), b = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * a.blocks);
+        const int64_t cell = a.cells[row];
+        if (cell < 0 || cell >= a.n_cells) continue;
+        const uint8_t *src = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b);
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = act_load<TYPE>(src + e * s.nb_dim);
+        const int bb = block_bytes(s.cache_type);
+        write_block(x, s.cache_type, s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb);
+    }
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const __grid_constant__ RowsArgs a) {
+    const RowsSide &s = a.side[blockIdx.y];
+    if (!s.on) return;
+    const uint64_t all = static_cast<uint64_t>(a.n) * a.blocks;
+    for (uint64_t i = blockIdx.x * static_cast<uint64_t>(kRowsThreads) + threadIdx.x; i < all;
+         i += static_cast<uint64_t>(gridDim.x) * kRowsThreads) {
+        const uint32_t row = static_cast<uint32_t>(i / a.blocks), b = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * a.blocks);
+        const int64_t cell = a.cells[row];
+        uint8_t *dst = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b);
+        if (cell < 0 || cell >= a.n_cells) {
+            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, 0.0f);
+            continue;
+        }
+        const int bb = block_bytes(s.cache_type);
+        const uint8_t *p = s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb;
+        auto half_at = [](const uint8_t *q) { return __half2float(*reinterpret_cast<const __half *>(q)); };
+        if (s.cache_type == KVM_TYPE_F16) {
+            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, half_at(p + 2 * e));
+            continue;
+        }
+        const float d = half_at(p);
+        if (s.cache_type == KVM_TYPE_Q8_0) {
+            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, d * static_cast<float>(static_cast<int8_t>(p[2 + e])));
+            continue;
+        }
+        const bool q5 = s.cache_type == KVM_TYPE_Q5_0;
+        for (int e = 0; e < 32; ++e) {
+            int c = (p[bb - 16 + (e & 15)] >> (e < 16 ? 0 : 4)) & 15;
+            if (q5) c |= ((p[2 + e / 8] >> (e & 7)) & 1) << 4;
+            act_store<TYPE>(dst + e * s.nb_dim, d * static_cast<float>(c - (q5 ? 16 : 8)));
+        }
+    }
+}
+
+kvm_status rows_call(const char *me, bool write, kvm_stream stream, const kvm_cache *c, uint32_t n,
+                     const int64_t *d_cells, const kvm_rows *k, const kvm_rows *v) {
+    kvm_status r = cache_check(c, me);
+    if (r != KVM_OK) return r;
+    if (!k && !v) return layer_fail(KVM_EINVAL, "%s: neither k nor v", me);
+    if (n > 0x7fffffffu) return layer_fail(KVM_EINVAL, "%s: too many rows", me);
+    if (n == 0) return KVM_OK;
+    if (k && (r = rows_check(k, c->n_head_kv, c->head_dim, me)) != KVM_OK) return r;
+    if (v && (r = rows_check(v, c->n_head_kv, c->head_dim, me)) != KVM_OK) return r;
+    if (k && v && k->type != v->type) return layer_fail(KVM_EINVAL, "%s: k and v must have one type", me);
+    if (!d_cells || (reinterpret_cast<uintptr_t>(d_cells) & 7u))
+        return layer_fail(KVM_EINVAL, "%s: cells must be an 8-byte aligned array", me);
+    PointerDevice dev(c->d_k, me);
+    if (dev.status() != KVM_OK) return dev.status();
+    RowsArgs a{};
+    const uint32_t width = c->n_head_kv * c->head_dim;
+    a.cells = d_cells;
+    a.n_cells = static_cast<int64_t>(c->block_tokens) * c->n_slots;
+    a.n = n;
+    a.blocks = width / 32u;
+    a.head_dim = c->head_dim;
+    for (int i = 0; i < 2; ++i) {
+        const kvm_rows *x = i ? v : k;
+        RowsSide &s = a.side[i];
+        s.on = x != nullptr;
+        if (!x) continue;
+        s.cache = static_cast<uint8_t *>(i ? c->d_v : c->d_k);
+        s.cache_type = i ? c->type_v : c->type_k;
+        s.row_bytes = kvm_row_bytes(s.cache_type, width);
+        s.act = static_cast<uint8_t *>(const_cast<void *>(x->data));
+        s.nb_dim = x->nb_dim;
+        s.nb_head = x->nb_head;
+        s.nb_tok = x->nb_tok;
+    }
+    const uint64_t want = (static_cast<uint64_t>(n) * a.blocks + kRowsThreads - 1) / kRowsThreads;
+    const uint64_t most = 8ull * num_sms();
+    const dim3 grid(static_cast<uint32_t>(want < most ? want : most), 2);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int32_t type = (k ? k : v)->type;
+    auto go = [&](auto write_kernel, auto read_kernel) {
+        if (write) write_kernel<<<grid, kRowsThreads, 0, st>>>(a);
+        else read_kernel<<<grid, kRowsThreads, 0, st>>>(a);
+    };
+    if (type == KVM_TYPE_F32) go(write_rows_kernel<KVM_TYPE_F32>, read_rows_kernel<KVM_TYPE_F32>);
+    else if (type == KVM_TYPE_F16) go(write_rows_kernel<KVM_TYPE_F16>, read_rows_kernel<KVM_TYPE_F16>);
+    else go(write_rows_kernel<KVM_TYPE_BF16>, read_rows_kernel<KVM_TYPE_BF16>);
+    return layer_cuda(cudaGetLastError(), me);
+}
+
+}  // namespace
+}  // namespace kvm
+
+using namespace kvm;
+
+extern "C" kvm_status kvm_write_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n, const int64_t *d_cells,
+                                     const kvm_rows *k, const kvm_rows *v) {
+    return rows_call("kvm_write_rows", true, stream, cache, n, d_cells, k, v);
+}
+
+extern "C" kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n, const int64_t *d_cells,
+                                    const kvm_rows *k_out, const kvm_rows *v_out) {
+    return rows_call("kvm_read_rows", false, stream, cache, n, d_cells, k_out, v_out);
+}

@@ -1,7 +1,8 @@
 """ctypes binding of libkvm (include/kvm.h) for tests, the bench and Python callers.
 
 libkvm is the B200-native (sm_100a) KV reselection library: score -> select ->
-diff -> gather+quantize stage-in.  This module only marshals arguments; all
+diff -> gather+quantize stage-in, and the attention layer around the window:
+map_batch, qk_norm_rope, write_rows / read_rows, attend.  This module only marshals arguments; all
 work runs in the CUDA library.  Importing it when ``libkvm.so`` is missing
 raises -- there is no CPU fallback.
 
@@ -42,8 +43,12 @@ ABI_SYMBOLS = (
     "kvm_quantize_rows_noalloc", "kvm_write_mean_k", "kvm_meank_add", "kvm_meank_flush",
     "kvm_meank_zero", "kvm_query_reset", "kvm_query_add", "kvm_set_transform",
     "kvm_attn_rot_nrot", "kvm_stageout", "kvm_stageout_item_bytes", "kvm_select_groups",
-    "kvm_stagein_packed", "kvm_test_inject",
+    "kvm_stagein_packed", "kvm_test_inject", "kvm_map_batch", "kvm_qk_norm_rope",
+    "kvm_write_rows", "kvm_read_rows", "kvm_attend",
 )
+
+ATTEND_CAUSAL = 1                 # kvm_attend_batch flag
+ATTEND_WORK_BYTES = 32 << 20      # KVM_ATTEND_WORK_BYTES
 
 
 class KvmError(RuntimeError):
@@ -119,6 +124,31 @@ class PackedSource(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_layer_stride", C.c_uint64),
                 ("k_block_stride", C.c_uint64), ("v_layer_stride", C.c_uint64),
                 ("v_block_stride", C.c_uint64), ("location", C.c_int32), ("reserved0", C.c_int32)]
+
+
+class _Cache(C.Structure):
+    """kvm_cache"""
+    _fields_ = [("d_k", C.c_void_p), ("d_v", C.c_void_p), ("type_k", C.c_int32),
+                ("type_v", C.c_int32), ("n_head_kv", C.c_uint32), ("head_dim", C.c_uint32),
+                ("block_tokens", C.c_uint32), ("n_slots", C.c_uint32)]
+
+
+class _BatchMap(C.Structure):
+    """kvm_batch_map"""
+    _fields_ = [("d_past", C.c_void_p), ("d_new", C.c_void_p), ("d_free", C.c_void_p),
+                ("d_table", C.c_void_p), ("table_stride", C.c_uint64), ("table_cols", C.c_uint32),
+                ("n_seq", C.c_uint32), ("n_free", C.c_uint32), ("block_tokens", C.c_uint32),
+                ("n_rows", C.c_uint32), ("reserved0", C.c_uint32), ("d_q_start", C.c_void_p),
+                ("d_kv_len", C.c_void_p), ("d_cells", C.c_void_p), ("d_pos", C.c_void_p),
+                ("d_seq", C.c_void_p), ("d_info", C.c_void_p)]
+
+
+class _AttendBatch(C.Structure):
+    """kvm_attend_batch"""
+    _fields_ = [("d_table", C.c_void_p), ("table_stride", C.c_uint64), ("table_cols", C.c_uint32),
+                ("n_seq", C.c_uint32), ("d_q_start", C.c_void_p), ("d_kv_len", C.c_void_p),
+                ("n_rows", C.c_uint32), ("max_new", C.c_uint32), ("flags", C.c_uint32),
+                ("scale", C.c_float)]
 
 
 class Window(C.Structure):
@@ -205,6 +235,13 @@ def lib():
             "kvm_stageout_item_bytes": (u64, [vp]),
             "kvm_select_groups": (C.c_int, [vp, vp, vp, vp, u32, vp, u32]),
             "kvm_stagein_packed": (C.c_int, [vp, vp, C.POINTER(PackedSource), C.POINTER(Window)]),
+            "kvm_map_batch": (C.c_int, [vp, C.POINTER(_BatchMap)]),
+            "kvm_qk_norm_rope": (C.c_int, [vp, u32, C.POINTER(Rows), C.POINTER(Rows), vp, vp, C.c_float,
+                                           vp, u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
+            "kvm_write_rows": (C.c_int, [vp, C.POINTER(_Cache), u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
+            "kvm_read_rows": (C.c_int, [vp, C.POINTER(_Cache), u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
+            "kvm_attend": (C.c_int, [vp, C.POINTER(_Cache), C.POINTER(_AttendBatch), C.POINTER(Rows),
+                                     C.POINTER(Rows), vp, u64]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -262,6 +299,182 @@ def quantize_rows(type_: int, src, n_rows: int, n_embd: int, dst, stream=None) -
 
 def make_source(k, v, layer_stride, block_stride, row_stride, location=LOC_DEVICE) -> Source:
     return Source(_ptr(k), _ptr(v), layer_stride, block_stride, row_stride, location, 0)
+
+
+# ------------------------------------- the attention layer around a window
+#
+# Device tensors in, device tensors out: buffers are the caller's, the work is
+# ordered on `stream` (default: the current stream of the tensors' device).
+
+def _bad(what):
+    raise KvmError(KVM_EINVAL, what)
+
+
+def _layer_check(st):
+    if st != KVM_OK:
+        raise KvmError(st, lib().kvm_last_error(None).decode())
+
+
+class _Torch:
+    """torch's dtypes and stream lookup, fetched at the first call."""
+    ready = False
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.i32, cls.i64, cls.f32 = torch.int32, torch.int64, torch.float32
+        cls.rows = {torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2), torch.bfloat16: (TYPE_BF16, 2)}
+        cls.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        cls.ready = True
+        return cls
+
+
+def _device(t, what):
+    """CUDA device index of the call's first tensor; loads torch's names."""
+    if not _Torch.ready:
+        _Torch.load()
+    dev = t.get_device()
+    if dev < 0:
+        _bad(f"{what}: a CUDA tensor")
+    return dev
+
+
+def _layer_stream(stream, dev):
+    if stream is None:
+        return _Torch.raw_stream(dev)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _act(t, what, dev):
+    """kvm_rows of [rows, heads, head_dim], any strides."""
+    ty = _Torch.rows.get(t.dtype)
+    if ty is None or t.dim() != 3 or t.get_device() != dev:
+        _bad(f"{what}: float32, float16 or bfloat16 [rows, heads, head_dim] on cuda:{dev}, "
+             f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    es = ty[1]
+    _, heads, dim = t.shape
+    st, sh, sd = t.stride()
+    return Rows(t.data_ptr(), ty[0], heads, dim, 0, sd * es, sh * es, st * es)
+
+
+def _index(t, dtype, n, what, dev):
+    """Address of a contiguous vector of at least n entries."""
+    if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev or t.shape[0] < n:
+        _bad(f"{what}: a contiguous {dtype} vector of at least {n} on cuda:{dev}, "
+             f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _table(t, n_seq, dev):
+    """(address, row stride, columns) of a block table."""
+    if t.dtype is not _Torch.i32 or t.dim() != 2 or t.get_device() != dev:
+        _bad(f"table: int32 [{n_seq}, blocks] on cuda:{dev}")
+    rows, cols = t.shape
+    stride, step = t.stride()
+    if rows != n_seq or (cols > 1 and step != 1) or (rows > 1 and stride < cols):
+        _bad(f"table: [{n_seq}, blocks] with neighbouring columns, not {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), max(stride, cols), cols
+
+
+_BLOCK_BYTES = {TYPE_F16: 64, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34}
+
+
+class Cache(_Cache):
+    """One layer's cache (kvm_cache): n_slots blocks of block_tokens ggml rows in
+    the contiguous tensors k and v."""
+
+    def __init__(self, k, v, type_k, type_v, n_head_kv, head_dim, block_tokens, n_slots):
+        self.device = _device(k, "cache k")
+        cells, width = block_tokens * n_slots, n_head_kv * head_dim
+        for t, ty, what in ((k, type_k, "k"), (v, type_v, "v")):
+            if ty not in _BLOCK_BYTES or width <= 0 or width % 32 or cells <= 0:
+                _bad(f"cache {what}: F16, Q8_0, Q5_0 or Q4_0 rows of blocks of 32, at least one cell")
+            want = cells * (width // 32 * _BLOCK_BYTES[ty])
+            if not t.is_contiguous() or t.get_device() != self.device or t.numel() * t.element_size() < want:
+                _bad(f"cache {what}: a contiguous tensor of at least {want} bytes on cuda:{self.device}")
+        super().__init__(k.data_ptr(), v.data_ptr(), type_k, type_v, n_head_kv, head_dim, block_tokens, n_slots)
+        self.tensors = (k, v)
+
+
+def map_batch(past, new, free_slots, block_tokens, table, q_start, kv_len, cells, pos, seq, info, stream=None):
+    """kvm_map_batch: block tables and the cell map of a step from the requests'
+    lengths.  past, new: int32 [n]; free_slots: int32; table: int32 [n, blocks],
+    updated; out: q_start int32 [n+1], kv_len int32 [n], cells int64 [rows], pos
+    and seq int32 [rows], info int32 [4]."""
+    dev = _device(past, "past")
+    i32, n, rows = _Torch.i32, past.shape[0], cells.shape[0]
+    tab, stride, cols = _table(table, n, dev)
+    m = _BatchMap(_index(past, i32, n, "past", dev), _index(new, i32, n, "new", dev),
+                  _index(free_slots, i32, 0, "free_slots", dev), tab, stride, cols, n, free_slots.shape[0], block_tokens,
+                  rows, 0, _index(q_start, i32, n + 1, "q_start", dev), _index(kv_len, i32, n, "kv_len", dev),
+                  _index(cells, _Torch.i64, rows, "cells", dev), _index(pos, i32, rows, "pos", dev),
+                  _index(seq, i32, rows, "seq", dev), _index(info, i32, 4, "info", dev))
+    _layer_check(lib().kvm_map_batch(_layer_stream(stream, dev), C.byref(m)))
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, eps, freqs, pos, q_out, k_out, stream=None):
+    """kvm_qk_norm_rope: RMS norm of every head and the NeoX rotation of its first
+    2 * len(freqs) dims at pos[row].  q, k: [rows, heads, head_dim]; weights
+    float32 [head_dim] or None; freqs float32 [n_rot / 2] or None; k and k_out
+    may be None."""
+    dev = _device(q, "q")
+    n, _, d = q.shape
+    a, ao = _act(q, "q", dev), _act(q_out, "q_out", dev)
+    if q_out.shape != q.shape:
+        _bad("q_out: shape of q")
+    b = bo = None
+    if k is not None or k_out is not None:
+        if k is None or k_out is None or k_out.shape != k.shape or k.shape[0] != n:
+            _bad("k and k_out: [rows of q, heads, head_dim]")
+        b, bo = C.byref(_act(k, "k", dev)), C.byref(_act(k_out, "k_out", dev))
+    f32, half = _Torch.f32, 0 if freqs is None else freqs.shape[0]
+    _layer_check(lib().kvm_qk_norm_rope(
+        _layer_stream(stream, dev), n, C.byref(a), b,
+        None if q_weight is None else _index(q_weight, f32, d, "q_weight", dev),
+        None if k_weight is None else _index(k_weight, f32, d, "k_weight", dev), eps,
+        None if freqs is None else _index(freqs, f32, half, "freqs", dev), 2 * half,
+        None if pos is None else _index(pos, _Torch.i32, n, "pos", dev), C.byref(ao), bo))
+
+
+def _rows_call(fn, cache, cells, k, v, stream):
+    dev, n = cache.device, cells.shape[0]
+    if (k is not None and k.shape[0] != n) or (v is not None and v.shape[0] != n):
+        _bad("k and v: one row a cell")
+    _layer_check(fn(_layer_stream(stream, dev), C.byref(cache), n, _index(cells, _Torch.i64, n, "cells", dev),
+                    None if k is None else C.byref(_act(k, "k", dev)),
+                    None if v is None else C.byref(_act(v, "v", dev))))
+
+
+def write_rows(cache, cells, k, v, stream=None):
+    """kvm_write_rows: quantize k[i] and v[i] ([rows, n_head_kv, head_dim]; either
+    may be None) into cell cells[i] (int64; negative = skip)."""
+    _rows_call(lib().kvm_write_rows, cache, cells, k, v, stream)
+
+
+def read_rows(cache, cells, k_out, v_out, stream=None):
+    """kvm_read_rows: the values of cell cells[i] into k_out[i] and v_out[i]
+    (either may be None)."""
+    _rows_call(lib().kvm_read_rows, cache, cells, k_out, v_out, stream)
+
+
+def attend(cache, q, q_start, kv_len, table, out, work, scale, causal=True, max_new=1, stream=None):
+    """kvm_attend: attention of q [rows, heads, head_dim] over the cache into out.
+    q_start int32 [n+1], kv_len int32 [n], table int32 [n, blocks]; work: a
+    tensor of ATTEND_WORK_BYTES for this call alone while it runs; max_new: the
+    most rows of a request, as far as the caller knows."""
+    dev, n = cache.device, kv_len.shape[0]
+    a, b = _act(q, "q", dev), _act(out, "out", dev)
+    if out.shape != q.shape:
+        _bad("out: shape of q")
+    if work.get_device() != dev or not work.is_contiguous():
+        _bad(f"work: a contiguous tensor on cuda:{dev}")
+    tab, stride, cols = _table(table, n, dev)
+    i32 = _Torch.i32
+    batch = _AttendBatch(tab, stride, cols, n, _index(q_start, i32, n + 1, "q_start", dev),
+                         _index(kv_len, i32, n, "kv_len", dev), q.shape[0], max_new, ATTEND_CAUSAL if causal else 0, scale)
+    _layer_check(lib().kvm_attend(_layer_stream(stream, dev), C.byref(cache), C.byref(batch), C.byref(a), C.byref(b),
+                                  work.data_ptr(), work.numel() * work.element_size()))
 
 
 class Session:
