@@ -1,4 +1,5 @@
 // kvm_attend.cu -- kvm_attend: argument checks and the choice of kernel.
+#include <algorithm>
 #include <cmath>
 
 #include "kvm_attend.cuh"
@@ -8,6 +9,29 @@ namespace kvm {
 
 template <int D, int KT>
 cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st);
+
+bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return reinterpret_cast<Encode>(fn);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {row_bytes / 4u, static_cast<uint64_t>(a.n_slots) * a.block_tokens};
+    const cuuint64_t strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {box_bytes / 4u, kAttendStep}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 namespace {
 
@@ -85,6 +109,9 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     a.out = rows_of(out);
     a.work = static_cast<uint8_t *>(d_work);
     a.align16 = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.row_k | a.row_v) & 15u) == 0;
+    a.tma = a.align16 && c->block_tokens % kAttendStep == 0;
+    a.q_vec = rows_vec16(q);
+    a.heads_cta = c->n_head_kv % 4u == 0 ? 4 : c->n_head_kv % 2u == 0 ? 2 : 1;
     a.min_rows = 1;
     a.max_rows = 0xffffffffu;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -95,7 +122,7 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     const uint64_t steps = (static_cast<uint64_t>(b->table_cols) * c->block_tokens + kAttendStep - 1) / kAttendStep + 1;
     const uint64_t most = static_cast<uint64_t>(num_sms());
     uint64_t grid = most;
-    if (tiles * c->n_head_kv <= 8u * most) grid = std::min<uint64_t>(most, (tiles * c->n_head_kv * std::min<uint64_t>(steps, 1u << 24) + 7) / 8);
+    if (tiles * c->n_head_kv <= 8u * most) grid = std::min<uint64_t>(most, (tiles * c->n_head_kv * std::min<uint64_t>(steps, 1u << 24) + 3) / 4);
     grid = std::max<uint64_t>(1, std::min<uint64_t>(grid, kAttendMaxCtas));
     cudaError_t e;
     if (D == 64u) e = split_d<64>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);

@@ -8,6 +8,7 @@
 // small integers and the scales are applied outside the products.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,7 +38,11 @@ struct AttendArgs {
     AttendRows q, out;
     uint8_t *work;             // split descriptors, then partial results
     uint32_t align16;          // cache bases and row bytes are multiples of 16
+    uint32_t tma;              // the cache's rows come through map_k, map_v (steps lie in one block)
+    uint32_t q_vec;            // q: contiguous heads, 16-byte aligned
+    uint32_t heads_cta;        // KV heads that a CTA takes together: 1, 2 or 4
     uint32_t min_rows, max_rows;   // query rows (tokens * group) a sequence needs to be taken by this launch
+    CUtensorMap map_k, map_v;      // [cells][row bytes / 4] of 32-bit words
 };
 
 // A sequence as the kernels see it; nothing read from device memory is trusted
@@ -83,7 +88,7 @@ __device__ __forceinline__ void store16(uint8_t *p, float x, int32_t bf16) {
 // D += A B on f16 operands with F32 accumulation, A 16x16, B 16x8.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                         const float (&c)[4]) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
@@ -135,13 +140,23 @@ struct AttendDesc {                           // segment that starts in CTA c an
 };
 static_assert(sizeof(AttendDesc) == kAttendDescBytes, "AttendDesc");
 
+// Partial results of one slot: for every head of the CTA its R maxima, R sums
+// and R rows of D.
 template <int D, int NT>
-constexpr uint32_t attend_part_floats() { return 8u * NT * (D + 2u); }
+__host__ __device__ constexpr uint32_t attend_part_floats() { return 8u * NT * (D + 2u); }
 
 template <int D, int NT>
-__device__ __forceinline__ float *attend_part(uint8_t *work, uint32_t slot) {
-    return reinterpret_cast<float *>(work + kAttendMaxCtas * kAttendDescBytes) +
-           static_cast<uint64_t>(slot) * attend_part_floats<D, NT>();
+__device__ __forceinline__ float *attend_part(const AttendArgs &a, uint32_t slot, uint32_t head) {
+    return reinterpret_cast<float *>(a.work + kAttendMaxCtas * kAttendDescBytes) +
+           (static_cast<uint64_t>(slot) * a.heads_cta + head) * attend_part_floats<D, NT>();
+}
+
+// Box of `map` at (x words, y row) to shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int32_t x, int32_t y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
 }
 
 // ------------------------------------------------------------ block codes --
@@ -150,10 +165,12 @@ template <int T, int D>
 struct Slice {
     static constexpr int kBlock = T == KVM_TYPE_F16 ? 64 : block_bytes(T);
     static constexpr int kBytes = D / 32 * kBlock;
-    // shared-memory stride: an odd multiple of 16 bytes, so that eight rows'
-    // words fall into different banks
-    static constexpr int kUp = (kBytes + 15) / 16;
-    static constexpr int kStride = (kUp | 1) * 16;
+    // a head's slice starts at a multiple of kBytes: up to this many bytes behind
+    // the last 16-byte boundary
+    static constexpr int kLead = kBytes % 16 == 0 ? 0 : kBytes % 8 == 0 ? 8 : 12;
+    // shared-memory stride: the slice with its lead, as an odd multiple of 16
+    // bytes, so that eight rows' words fall into different banks
+    static constexpr int kStride = ((kBytes + kLead + 15) / 16 | 1) * 16;
     static constexpr bool kNibble = T == KVM_TYPE_Q4_0 || T == KVM_TYPE_Q5_0;
     // codes are stored unsigned; the value is (code - kOffset) * d
     static constexpr int kOffset = T == KVM_TYPE_Q4_0 ? 8 : T == KVM_TYPE_Q5_0 ? 16 : T == KVM_TYPE_Q8_0 ? 128 : 0;

@@ -1,21 +1,33 @@
 // kvm_attend_split.cu -- the instances of attend_split_kernel for one head size
 // and K type (compiled once for each pair of KVM_ATTEND_D, KVM_ATTEND_KT).
+#include <algorithm>
+
 #include "kvm_attend_split.cuh"
 
 namespace kvm {
+
+// Tensor map of one side of the cache: rows of 32-bit words, boxes of a step's
+// 16 rows by box_bytes.  False when the driver cannot make it.
+bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes);
+
 namespace {
 
 template <int D, int KT, int VT, int NT>
-cudaError_t launch(const AttendArgs &a, uint32_t grid, cudaStream_t st) {
+cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
     static std::atomic<uint64_t> attr{0};
-    constexpr int smem = attend_split_smem<D, KT, VT, NT>();
+    using G = SplitGeom<D, KT, VT, NT>;
+    constexpr int smem = G::kSmem;
     static_assert(smem <= 227 * 1024, "shared memory");
     if (!attr_once(attr, reinterpret_cast<const void *>(attend_split_kernel<D, KT, VT, NT>), smem))
         return cudaErrorInvalidValue;
-    attend_split_kernel<D, KT, VT, NT><<<grid, SplitGeom<D, KT, VT>::kThreads, smem, st>>>(a);
+    if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride)))
+        a.tma = 0;
+    const uint64_t slot = static_cast<uint64_t>(a.heads_cta) * attend_part_floats<D, NT>() * 4u;
+    grid = static_cast<uint32_t>(std::min<uint64_t>(grid, (KVM_ATTEND_WORK_BYTES - kAttendMaxCtas * kAttendDescBytes) / (2 * slot)));
+    attend_split_kernel<D, KT, VT, NT><<<grid, G::kThreads, smem, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_after_prev(attend_join_kernel<D, NT>, dim3(grid, 8 * NT), dim3(D), 0, st, a);
+    return launch_after_prev(attend_join_kernel<D, NT>, dim3(grid, 8 * NT * a.heads_cta), dim3(kJoinThreads), 0, st, a);
 }
 
 template <int D, int KT, int VT>

@@ -26,38 +26,37 @@
 // straight from the rows' bytes, and P^T goes from the accumulators to the B
 // operand by one 8x8 transpose a half.  Which 16 elements of a block form one
 // K = 16 product is free as long as q agrees, so every lane takes the bytes of
-// one word.  A warp streams its own keys (16 a step) through its own
-// cp.async ring and keeps its own running maximum, sum and output; the warps
-// of a CTA meet once a segment.
+// one word.  A warp streams its own keys (16 a step) of one KV head through its
+// own ring in shared memory and keeps its own running maximum, sum and output;
+// the warps of a CTA meet once a segment.  A CTA takes up to four KV heads of the
+// same keys: their slices share 32-byte sectors, and read by different CTAs at
+// different times they cost 1.7 times the window's bytes (961 of 569 MB over 32
+// windows).  The slices come by TMA, one 2D box a step, where a step lies in one
+// block and rows are multiples of 16 bytes, else by cp.async.
 #pragma once
 
 #include "kvm_attend.cuh"
 
 namespace kvm {
 
-template <int D, int KT, int VT>
+template <int D, int KT, int VT, int NT>
 struct SplitGeom {
     using K = Slice<KT, D>;
     using V = Slice<VT, D>;
     static constexpr int kStage = kAttendStep * (K::kStride + V::kStride);
-    // eight warps unless two stages of each no longer fit
-    static constexpr int kWarps = 16 * kStage <= 210 * 1024 ? 8 : 4;
+    static constexpr int kRoom = 200 * 1024;
+    // twelve warps where the registers (D / 4 a row tile for the output) and two
+    // stages of each warp allow it
+    static constexpr int kWarps = (D * NT <= 256 && 24 * kStage <= kRoom) ? 12 : 16 * kStage <= kRoom ? 8 : 4;
     static constexpr int kThreads = kWarps * 32;
-    static constexpr int kBudget = 196 * 1024 / (kWarps * kStage);
+    static constexpr int kBudget = kRoom / (kWarps * kStage);
     static constexpr int kStages = kBudget > 6 ? 6 : kBudget < 2 ? 2 : kBudget;
     static constexpr int kScaleBytes = 1024;      // per warp: K f16, K f32, V f16
     static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kMerge = kWarps * 8 * NT * (D + 4 + 2) * 4;
+    static constexpr int kBig = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
+    static constexpr int kSmem = kBig + kWarps * (kScaleBytes + kStages * 16);
 };
-
-template <int D, int NT>
-constexpr int attend_merge_bytes(int warps) { return warps * 8 * NT * (D + 4 + 2) * 4; }
-
-template <int D, int KT, int VT, int NT>
-constexpr int attend_split_smem() {
-    using G = SplitGeom<D, KT, VT>;
-    const int merge = attend_merge_bytes<D, NT>(G::kWarps), big = G::kRing > merge ? G::kRing : merge;
-    return big + G::kWarps * (G::kScaleBytes + G::kStages * 4) + 64;
-}
 
 __device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ uint32_t lds16(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
@@ -118,13 +117,6 @@ __device__ __forceinline__ void k_codes(const uint8_t *pair, int t, uint32_t (&w
             w[b][0][0] = x.x; w[b][0][1] = x.y; w[b][1][0] = x.z; w[b][1][1] = x.w;
         }
     }
-}
-
-// Element of a 32-block that register r (0..3: product r >> 1, register r & 1)
-// holds in half i, for lane t of a K row.
-template <int KT>
-__device__ __forceinline__ constexpr int k_elem(int t, int r, int i) {
-    return Slice<KT, 64>::kNibble ? 4 * t + 2 * i + (r & 1) + 16 * (r >> 1) : 8 * t + 2 * r + i;
 }
 
 // V: lane (g, t) supplies dims of rows g and g + 8 of two M = 16 tiles of block
@@ -190,25 +182,29 @@ __device__ __forceinline__ float row_value(const uint8_t *row, int e) {
 }
 
 template <int D, int KT, int VT, int NT>
-__global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_split_kernel(const __grid_constant__ AttendArgs a) {
-    using G = SplitGeom<D, KT, VT>;
+__global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) attend_split_kernel(const __grid_constant__ AttendArgs a) {
+    using G = SplitGeom<D, KT, VT, NT>;
     using SK = Slice<KT, D>;
     using SV = Slice<VT, D>;
     constexpr int NB = D / 32, W = G::kWarps, kThreads = G::kThreads, NS = G::kStages, R = 8 * NT;
     constexpr bool kCodesK = KT != KVM_TYPE_F16, kCodesV = VT != KVM_TYPE_F16;
     constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 14.0f;
-    extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int kMerge = attend_merge_bytes<D, NT>(W), kBig = G::kRing > kMerge ? G::kRing : kMerge;
+    extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int hg = static_cast<int>(a.heads_cta), hsub = warp % hg, sub = warp / hg, nsub = W / hg;
     uint8_t *ring = smem + warp * NS * G::kStage;
-    uint8_t *scales = smem + kBig + warp * G::kScaleBytes;
+    uint8_t *scales = smem + G::kBig + warp * G::kScaleBytes;
     __half *k16 = reinterpret_cast<__half *>(scales);              // [16 keys][8 blocks]
     float *k32 = reinterpret_cast<float *>(scales + 256);          // [16][8]
     __half *v16 = reinterpret_cast<__half *>(scales + 768);        // [8 blocks][16 keys, a lane's four together]
-    uint32_t *valid = reinterpret_cast<uint32_t *>(smem + kBig + W * G::kScaleBytes) + warp * NS;
-    __shared__ unsigned long long s_scan[W], s_total;
-    __shared__ unsigned long long s_off;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBig + W * G::kScaleBytes) + warp * NS;
+    uint32_t *valid = reinterpret_cast<uint32_t *>(smem + G::kBig + W * (G::kScaleBytes + NS * 8)) + warp * NS;
+    __shared__ unsigned long long s_scan[W], s_off;
     __shared__ uint32_t s_seq;
+
+    if (lane == 0)
+        for (int i = 0; i < NS; ++i) mbar_init(&bars[i], 1);
+    fence_mbar_init();
 
     // ---- this CTA's share of the line of steps
     auto units = [&](uint32_t s) -> unsigned long long {
@@ -216,19 +212,34 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         const uint64_t rows = static_cast<uint64_t>(q.n_new) * a.group;
         if (q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) return 0ull;
         const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kAttendStep - 1u) / kAttendStep);
-        return ((rows + R - 1) / R) * a.n_head_kv * steps;
+        return ((rows + R - 1) / R) * (a.n_head_kv / hg) * steps;
     };
-    if (tid == 0) s_total = 0;
-    unsigned long long mine = 0;
-    for (uint32_t s = tid; s < a.n_seq; s += kThreads) mine += units(s);
+    // inclusive sum of n over the CTA's threads; *all gets the total
+    auto scan = [&](unsigned long long n, unsigned long long *all) -> unsigned long long {
+        unsigned long long x = n;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    __syncthreads();
-    if (lane == 0) atomicAdd(&s_total, mine);
-    __syncthreads();
-    const unsigned long long total = s_total;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        unsigned long long before = 0, sum = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) before += s_scan[w];
+            sum += s_scan[w];
+        }
+        *all = sum;
+        __syncthreads();
+        return x + before;
+    };
+    const bool once = a.n_seq <= kThreads;
+    unsigned long long mine = 0, total = 0;
+    for (uint32_t s = tid; s < a.n_seq; s += kThreads) mine += units(s);
+    const unsigned long long upto = scan(mine, &total);
     unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < static_cast<unsigned long long>(W)) share = W;
+    if (share < static_cast<unsigned long long>(nsub)) share = nsub;
     const unsigned long long u0 = share * blockIdx.x;
     const unsigned long long u1 = min(u0 + share, total);
     AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
@@ -239,33 +250,24 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
     unsigned long long carry = 0;
     for (uint32_t base = 0; base < a.n_seq; base += kThreads) {
         const uint32_t s = base + tid;
-        const unsigned long long n = s < a.n_seq ? units(s) : 0ull;
-        unsigned long long x = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+        unsigned long long n = mine, x = upto, all = total;
+        if (!once) {
+            n = s < a.n_seq ? units(s) : 0ull;
+            x = carry + scan(n, &all);
         }
-        if (lane == 31) s_scan[warp] = x;
-        __syncthreads();
-        unsigned long long before = carry, all = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) before += s_scan[w];
-            all += s_scan[w];
-        }
-        x += before;
         if (n != 0 && x - n <= u0 && u0 < x) {
             s_seq = s;
             s_off = u0 - (x - n);
         }
         carry += all;
-        __syncthreads();
         if (carry > u0) break;
     }
+    __syncthreads();
     uint32_t seq = s_seq;
     unsigned long long off = s_off;
     bool described = false;
+    uint32_t issued = 0;                      // ring position of the warp's next load
+    bool lost = false;                        // a bounded wait ran out
 
     for (unsigned long long pos = u0; pos < u1;) {
         // ---- the segment at `pos`
@@ -283,8 +285,8 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         const uint32_t in0 = static_cast<uint32_t>(off - static_cast<unsigned long long>(seg) * steps);
         const uint32_t left = steps - in0;
         const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(left), u1 - pos));
-        const uint32_t head = seg % a.n_head_kv;
-        const uint32_t first = seg / a.n_head_kv * R;
+        const uint32_t head0 = seg % (a.n_head_kv / hg) * hg, head = head0 + hsub;
+        const uint32_t first = seg / (a.n_head_kv / hg) * R;
         const uint32_t all_rows = static_cast<uint32_t>(q.n_new) * a.group;
         const uint32_t rows = min(static_cast<uint32_t>(R), all_rows - first);
         const int32_t kend = attend_limit(a, q, (first + rows - 1) / a.group);
@@ -302,14 +304,41 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
             const uint32_t tok = r / a.group;
             const uint8_t *qp = a.q.p + (static_cast<uint64_t>(q.row0) + (in ? tok : 0)) * a.q.nb_tok +
                                 (static_cast<uint64_t>(head) * a.group + (in ? r % a.group : 0)) * a.q.nb_head;
-            float x[NB][4][2], top = 0.0f;
+            uint32_t raw[NB][4];              // the lane's 8 values a block, in order
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (a.q_vec) {
+                    if constexpr (SK::kNibble) {
+                        const uint2 u = *reinterpret_cast<const uint2 *>(qp + 64 * b + 8 * t);
+                        const uint2 v = *reinterpret_cast<const uint2 *>(qp + 64 * b + 32 + 8 * t);
+                        raw[b][0] = u.x; raw[b][1] = u.y; raw[b][2] = v.x; raw[b][3] = v.y;
+                    } else {
+                        const uint4 u = *reinterpret_cast<const uint4 *>(qp + 64 * b + 16 * t);
+                        raw[b][0] = u.x; raw[b][1] = u.y; raw[b][2] = u.z; raw[b][3] = u.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int e = 32 * b + (SK::kNibble ? 4 * t + 2 * (k & 1) + 16 * (k >> 1) : 8 * t + 2 * k);
+                        raw[b][k] = *reinterpret_cast<const uint16_t *>(qp + e * a.q.nb_dim) |
+                                    static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(qp + (e + 1) * a.q.nb_dim)) << 16;
+                    }
+                }
+            }
+            auto value = [&](int b, int k, int i) {       // value i of pair k
+                const uint32_t u = i ? raw[b][k] >> 16 : raw[b][k] & 0xffffu;
+                const float v = a.q.bf16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u)));
+                return in ? v : 0.0f;
+            };
+            float x[NB][4][2], top = 0.0f;    // by operand register, as k_codes lays them out
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        x[b][k][i] = in ? load16(qp + (32 * b + k_elem<KT>(t, k, i)) * a.q.nb_dim, a.q.bf16) : 0.0f;
+                        // nibbles: register k pairs values (k & 1) and (k & 1) + 2 of half k >> 1
+                        x[b][k][i] = SK::kNibble ? value(b, (k & 2) + i, k & 1) : value(b, k, i);
                         top = fmaxf(top, fabsf(x[b][k][i]));
                     }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -371,17 +400,42 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         }
         int vexp = 15;                        // o holds the output times 2^(vexp - 24)
 
-        // ---- the warp's steps: in0 + warp, + W, ...
+        // ---- the warp's steps: in0 + sub, + nsub, ...
         const uint32_t kstart = in0 * kAttendStep;
         const uint32_t in1 = min(in0 + take, (static_cast<uint32_t>(kend) + kAttendStep - 1u) / kAttendStep);
-        const int n_steps = in1 > in0 + warp ? static_cast<int>((in1 - in0 - warp + W - 1) / W) : 0;
+        const int n_steps = in1 > in0 + sub ? static_cast<int>((in1 - in0 - sub + nsub - 1) / nsub) : 0;
         const int32_t *trow = a.table + seq * a.table_stride;
         const uint8_t *kbase = a.k + static_cast<uint64_t>(head) * SK::kBytes;
         const uint8_t *vbase = a.v + static_cast<uint64_t>(head) * SV::kBytes;
 
+        // bytes between the slice and the 16-byte boundary its box starts at
+        const int lead_k = a.tma ? static_cast<int>(head * SK::kBytes & 15u) : 0;
+        const int lead_v = a.tma ? static_cast<int>(head * SV::kBytes & 15u) : 0;
+
         auto load = [&](int i) {
-            uint8_t *st = ring + (i % NS) * G::kStage;
-            const uint32_t key = kstart + (warp + i * W) * kAttendStep + (lane & 15);
+            const uint32_t slot_at = (issued + i) % NS;
+            uint8_t *st = ring + slot_at * G::kStage;
+            const uint32_t key0 = kstart + (sub + i * nsub) * kAttendStep;
+            if (a.tma) {                      // all 16 keys lie in one block
+                if (lane == 0) {
+                    const uint32_t blk = key0 / a.block_tokens;
+                    const int32_t slot = trow[blk];
+                    const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots;
+                    const uint32_t left = static_cast<uint32_t>(kend) - key0;
+                    valid[slot_at] = ok ? (left >= 16u ? 0xffffu : (1u << left) - 1u) : 0u;
+                    if (ok) {
+                        const int32_t cell = static_cast<int32_t>(slot * a.block_tokens + (key0 - blk * a.block_tokens));
+                        mbar_arrive_expect_tx(&bars[slot_at], G::kStage);
+                        tma_load_2d(st, &a.map_k, static_cast<int32_t>(head * SK::kBytes / 16u * 4u), cell, &bars[slot_at]);
+                        tma_load_2d(st + kAttendStep * SK::kStride, &a.map_v, static_cast<int32_t>(head * SV::kBytes / 16u * 4u),
+                                    cell, &bars[slot_at]);
+                    } else {
+                        mbar_arrive(&bars[slot_at]);
+                    }
+                }
+                return;
+            }
+            const uint32_t key = key0 + (lane & 15);
             int32_t cell = -1;
             if (key < static_cast<uint32_t>(kend)) {
                 const uint32_t blk = key / a.block_tokens;
@@ -390,12 +444,12 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
                     cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
             }
             const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
-            if (lane == 0) valid[i % NS] = ok;
+            if (lane == 0) valid[slot_at] = ok;
             auto copy = [&](auto slice, uint8_t *dst, const uint8_t *base, uint64_t row_bytes) {
                 using S = decltype(slice);
                 auto pieces = [&](auto width) {
                     constexpr int V = decltype(width)::value, C = S::kBytes / V;
-#pragma unroll 9
+#pragma unroll 4
                     for (int y = 0; y < (kAttendStep * C + 31) / 32; ++y) {
                         const int x = lane + 32 * y, r = min(x / C, kAttendStep - 1), c = x - r * C;
                         const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
@@ -426,14 +480,32 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         }
 #pragma unroll 1
         for (int i = 0; i < n_steps; ++i) {
-            cp_async_wait<NS - 2>();
+            const uint32_t at = (issued + i) % NS;
+            if (a.tma) {
+                if (!lost && !mbar_wait_bounded(&bars[at], ((issued + i) / NS) & 1u)) lost = true;
+            } else {
+                cp_async_wait<NS - 2>();
+            }
             __syncwarp();
+            const uint32_t ok = valid[at];
             if (i + NS - 1 < n_steps) load(i + NS - 1);
             cp_async_commit();
-            const uint8_t *kr = ring + (i % NS) * G::kStage;
-            const uint8_t *vr = kr + kAttendStep * SK::kStride;
-            const int32_t key0 = static_cast<int32_t>(kstart + (warp + i * W) * kAttendStep);
-            const uint32_t ok = valid[i % NS];
+            if (ok == 0) continue;
+            const uint8_t *kr = ring + at * G::kStage + lead_k;
+            const uint8_t *vr = ring + at * G::kStage + kAttendStep * SK::kStride + lead_v;
+            const int32_t key0 = static_cast<int32_t>(kstart + (sub + i * nsub) * kAttendStep);
+            if (a.tma && ok != 0xffffu) {     // a box brings the bytes of hidden rows too: drop them
+                for (int x = lane; x < 16 * (SK::kBytes / 4 + SV::kBytes / 4); x += 32) {
+                    const int r = x & 15, w = x >> 4;
+                    if ((ok >> r) & 1u) continue;
+                    uint8_t *p = ring + at * G::kStage;
+                    p += w < SK::kBytes / 4 ? lead_k + r * SK::kStride + 4 * w
+                                            : kAttendStep * SK::kStride + lead_v + r * SV::kStride + 4 * (w - SK::kBytes / 4);
+                    *reinterpret_cast<uint32_t *>(p) = 0u;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
 
             // ---- the step's scales, laid out for the products
             bool odd_values = false;          // an infinite or NaN V value
@@ -452,11 +524,13 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
                 for (int y = 0; y < NB / 2; ++y) {
                     const int x = lane + 32 * y;
                     d[y] = lds16(vr + (x & 15) * SV::kStride + (x >> 4) * SV::kBlock);
-                    top = max(top, d[y] & 0x7fffu);
+                    const uint32_t size = d[y] & 0x7fffu;
+                    odd_values = odd_values || size >= 0x7c00u;
+                    top = max(top, size >= 0x7c00u ? 0u : size);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
-                odd_values = top >= 0x7c00u;
-                const int need = min(15, 15 - static_cast<int>(min(top, 0x7bffu) >> 10));
+                odd_values = __any_sync(0xffffffffu, odd_values);
+                const int need = min(15, 15 - static_cast<int>(top >> 10));
                 if (need < vexp) {            // the largest scale so far to [1, 2)
                     const float f = __uint_as_float(static_cast<uint32_t>(need - vexp + 127) << 23);
 #pragma unroll
@@ -489,6 +563,14 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
                 for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
             const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const uint8_t *row0 = kr + g * SK::kStride, *row1 = row0 + 8 * SK::kStride;
+            float dk[2][NB < 4 ? 4 : NB];     // scales of keys g, g + 8
+            if constexpr (kCodesK) {
+#pragma unroll
+                for (int b = 0; b < NB; b += 4) {
+                    *reinterpret_cast<float4 *>(&dk[0][b]) = *reinterpret_cast<const float4 *>(k32 + g * 8 + b);
+                    *reinterpret_cast<float4 *>(&dk[1][b]) = *reinterpret_cast<const float4 *>(k32 + (g + 8) * 8 + b);
+                }
+            }
 #pragma unroll
             for (int p = 0; p < NB / 2; ++p) {
                 uint32_t c0[2][2][2], c1[2][2][2];
@@ -498,11 +580,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
                 for (int b = 0; b < 2; ++b) {
                     const uint32_t a0[4] = {c0[b][0][0], c1[b][0][0], c0[b][0][1], c1[b][0][1]};
                     const uint32_t a1[4] = {c0[b][1][0], c1[b][1][0], c0[b][1][1], c1[b][1][1]};
-                    float d0 = 1.0f, d1 = 1.0f;
-                    if constexpr (kCodesK) {
-                        d0 = k32[g * 8 + 2 * p + b];
-                        d1 = k32[(g + 8) * 8 + 2 * p + b];
-                    }
+                    const float d0 = dk[0][2 * p + b], d1 = dk[1][2 * p + b];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint32_t *qq = qf[nt][2 * p + b];
@@ -661,6 +739,8 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         }
 
         // ---- the warps' results together
+        issued += n_steps;
+        if (lost) l[0][0] = __int_as_float(0x7fc00000);       // no result rather than a wrong one
         cp_async_wait<0>();
         __syncthreads();
         float *sm_m = reinterpret_cast<float *>(smem), *sm_l = sm_m + W * R, *sm_o = sm_l + W * R;
@@ -693,22 +773,20 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
         }
         __syncthreads();
         const bool starts = in0 == 0, ends = take == left;
-        float *part = nullptr;
-        if (!starts || !ends) part = attend_part<D, NT>(a.work, 2u * blockIdx.x + (starts ? 1u : 0u));
-        for (int x = tid; x < static_cast<int>(rows) * D; x += kThreads) {
-            const int r = x / D, d = x - r * D;
+        const bool whole = starts && ends;
+        for (int x = tid; x < hg * static_cast<int>(rows) * D; x += kThreads) {
+            const int hr = x / D, d = x - hr * D, hs = hr / static_cast<int>(rows), r = hr - hs * static_cast<int>(rows);
             float top = kNegInf;
-#pragma unroll
-            for (int w = 0; w < W; ++w) top = fmaxf(top, sm_m[w * R + r]);
+            for (int w = hs; w < W; w += hg) top = fmaxf(top, sm_m[w * R + r]);
             const float ref = top == kNegInf ? 0.0f : top;
             float sum = 0.0f, acc = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
+            for (int w = hs; w < W; w += hg) {
                 const float f = exp2_approx(sm_m[w * R + r] - ref);
                 sum += f * sm_l[w * R + r];
                 acc += f * sm_o[(w * R + r) * OS + d];
             }
-            if (part) {
+            if (!whole) {
+                float *part = attend_part<D, NT>(a, 2u * blockIdx.x + (starts ? 1u : 0u), hs);
                 if (d == 0) {
                     part[r] = top;
                     part[R + r] = sum;
@@ -717,18 +795,19 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
             } else {
                 const uint32_t rr = first + r, tok = rr / a.group;
                 store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(q.row0) + tok) * a.out.nb_tok +
-                            (static_cast<uint64_t>(head) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
+                            (static_cast<uint64_t>(head0 + hs) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
                         sum == 0.0f ? 0.0f : acc / sum, a.out.bf16);
             }
         }
         if (starts && !ends && tid == 0) {
             desc->row0 = q.row0;
-            desc->head = head;
+            desc->head = head0;
             desc->first = first;
             desc->rows = rows;
             desc->parts = 1u + static_cast<uint32_t>((pos + left - u1 + share - 1) / share);
         }
         described = described || (starts && !ends);
+        fence_proxy_async_smem();             // the ring's next loads come after these reads and writes
         __syncthreads();
         pos += take;
         off += take;
@@ -737,32 +816,64 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT>::kThreads), 1) attend_sp
     pdl_launch_dependents();
 }
 
-// One (split segment, row) a CTA, one dim a thread: the parts of a segment that
-// starts in CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...
+// One (split segment, head, row) a CTA: the parts of a segment that starts in
+// CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...  The parts are spread
+// over groups of D / 4 threads, four dims a thread, and added in a fixed order.
+constexpr int kJoinThreads = 512;
 template <int D, int NT>
-__global__ void __launch_bounds__(D) attend_join_kernel(const __grid_constant__ AttendArgs a) {
-    constexpr int R = 8 * NT;
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int R = 8 * NT, G = kJoinThreads / (D / 4);
+    __shared__ float weight[kAttendMaxCtas], s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
+    __shared__ float4 s_acc[G][D / 4];
     pdl_wait();
     const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + blockIdx.x;
-    const uint32_t parts = desc->parts, r = blockIdx.y;
+    const uint32_t parts = min(desc->parts, kAttendMaxCtas), hs = blockIdx.y / R, r = blockIdx.y % R;
     if (parts == 0 || r >= desc->rows) return;
-    const int d = threadIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto part = [&](uint32_t i) { return attend_part<D, NT>(a, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u, hs); };
     float top = -__builtin_huge_valf();
-    for (uint32_t i = 0; i < parts; ++i)
-        top = fmaxf(top, attend_part<D, NT>(a.work, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u)[r]);
+    for (uint32_t i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, weight[i] = part(i)[r]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
     const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-    float sum = 0.0f, acc = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = 0; i < parts; ++i) {
-        const float *p = attend_part<D, NT>(a.work, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u);
-        const float f = exp2_approx(p[r] - ref);
-        sum += f * p[R + r];
-        acc += f * p[2 * R + r * D + d];
+    float sum = 0.0f;
+    for (uint32_t i = tid; i < parts; i += kJoinThreads) {
+        const float f = exp2_approx(weight[i] - ref);
+        weight[i] = f;
+        sum += f * part(i)[R + r];
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    const int grp = tid / (D / 4), d = tid % (D / 4);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (uint32_t i = grp; i < parts; i += G) {
+        const float f = weight[i];
+        // rows start at 2 R floats behind a multiple of 16 bytes, D floats apart
+        const float4 x = *reinterpret_cast<const float4 *>(part(i) + 2 * R + r * D + 4 * d);
+        acc.x += f * x.x;
+        acc.y += f * x.y;
+        acc.z += f * x.z;
+        acc.w += f * x.w;
+    }
+    s_acc[grp][d] = acc;
+    __syncthreads();
+    if (tid >= D) return;
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) o += reinterpret_cast<const float *>(s_acc[k])[tid];
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) l += s_sum[w];
     const uint32_t rr = desc->first + r, tok = rr / a.group;
     store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
-                (static_cast<uint64_t>(desc->head) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
-            sum == 0.0f ? 0.0f : acc / sum, a.out.bf16);
+                (static_cast<uint64_t>(desc->head + hs) * a.group + rr % a.group) * a.out.nb_head + tid * a.out.nb_dim,
+            l == 0.0f ? 0.0f : o / l, a.out.bf16);
 }
 
 }  // namespace kvm

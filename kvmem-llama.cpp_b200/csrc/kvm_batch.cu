@@ -12,6 +12,8 @@
 //
 // Bound by latency at every size met: a decode step of 64 requests is one CTA's
 // two dependent loads, two scans and one store.
+#include <algorithm>
+
 #include "kvm_layer.cuh"
 
 namespace kvm {
@@ -164,8 +166,8 @@ extern "C" kvm_status kvm_map_batch(kvm_stream stream, const kvm_batch_map *m) {
         return layer_fail(KVM_EINVAL, "%s: buffers must be aligned to their elements", me);
     PointerDevice dev(m->d_past, me);
     if (dev.status() != KVM_OK) return dev.status();
-    const uint64_t work = m->n_rows / 4u + static_cast<uint64_t>(m->n_seq) * 4u;
-    const uint64_t want = (work + kMapThreads - 1) / kMapThreads, most = 2ull * num_sms();
+    const uint64_t work = std::max<uint64_t>(m->n_rows, static_cast<uint64_t>(m->n_seq) * 4u);
+    const uint64_t want = (work + kMapThreads - 1) / kMapThreads, most = 4ull * num_sms();
     map_batch_kernel<<<static_cast<uint32_t>(want < most ? (want ? want : 1) : most), kMapThreads, 0,
                        reinterpret_cast<cudaStream_t>(stream)>>>(*m);
     return layer_cuda(cudaGetLastError(), me);

@@ -5,16 +5,20 @@
 //
 // h = n_rot / 2, (c, s) = cos, sin of pos * freq_i.  The angle is a product of
 // an integer and an F32 value, exact in F64 up to 2^29 and within 2^-53 beyond;
-// it is reduced by multiples of 2 pi in F64 (a far position would lose every
-// digit in F32) and only the remainder goes to F32.  Norm, rotation and sums
+// it is reduced by whole turns in F64 (a far position would lose every digit in
+// F32) and only the remainder goes to F32.  Norm, rotation and sums
 // are F32 and each value is rounded once, at the store.
 //
-// Bound by HBM: every value is read and written once.  One CTA a token: its
-// cos / sin are formed once in shared memory for all heads, while the CTA's
-// first loads are in flight.  A thread owns the chunk pair that a rotation mixes (8
-// values and their partners n_rot/2 further on), so the rotation needs no
-// exchange and the norm only a reduction over the head's head_dim/16 threads.
+// Bound by HBM: every value is read and written once.  A thread owns the chunk
+// pair that a rotation mixes (8 values and their partners n_rot/2 further on) of
+// several heads of one token: its 8 cos / sin pairs and 16 weights stay in
+// registers for all of them, the rotation needs no exchange, and the norm only a
+// reduction over the head's head_dim/16 neighbouring threads.  No shared memory
+// and no barrier.  A token's heads are split over more threads while the tokens
+// alone do not fill the GPU (launch below).
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "kvm_layer.cuh"
 
@@ -38,6 +42,7 @@ struct RopeArgs {
     const int32_t *pos;
     float eps;
     uint32_t head_dim, n_rot, lanes;   // lanes: threads a head, a power of two >= head_dim / 16
+    uint32_t n, splits, per_split;     // a token's heads in `splits` ranges of per_split
 };
 
 template <int TYPE, bool VEC>
@@ -100,79 +105,107 @@ __device__ __forceinline__ void store8(uint8_t *p, uint64_t nb_dim, const float 
     }
 }
 
+template <bool VEC>
+__device__ __forceinline__ void load_weights(const float *w, uint32_t e, float (&x)[8]) {
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 1.0f;
+    } else if constexpr (VEC) {
+        const float4 a = *reinterpret_cast<const float4 *>(w + e), b = *reinterpret_cast<const float4 *>(w + e + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = w[e + i];
+    }
+}
+
 template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
-    __shared__ float2 turn[kRopeMaxDim / 2];
-    const uint32_t tok = blockIdx.x;
-    const uint32_t half = a.n_rot / 2, pairs = a.n_rot / 16;
-    const uint32_t p = threadIdx.x & (a.lanes - 1), per_pass = kRopeThreads / a.lanes;
     const uint32_t heads = a.q.heads + a.k.heads;
-    const bool in = p < a.head_dim / 16;
+    const uint64_t unit = (static_cast<uint64_t>(blockIdx.x) * kRopeThreads + threadIdx.x) / a.lanes;   // (token, head range)
+    const uint32_t p = threadIdx.x & (a.lanes - 1);
+    const uint32_t tok = static_cast<uint32_t>(unit / a.splits), part = static_cast<uint32_t>(unit - static_cast<uint64_t>(tok) * a.splits);
+    const uint32_t h0 = part * a.per_split, h1 = min(heads, h0 + a.per_split);
+    const bool in = p < a.head_dim / 16 && tok < a.n && h0 < h1;
+    const uint32_t half = a.n_rot / 2, pairs = a.n_rot / 16;
     const bool rot = p < pairs;
     // the two chunks of 8 of this thread
     const uint32_t e0 = rot ? 8 * p : a.n_rot + 16 * (p - pairs), e1 = rot ? e0 + half : e0 + 8;
-    uint32_t h = threadIdx.x / a.lanes;
-    float x0[8], x1[8];
-    auto fetch = [&](uint32_t hh) {
-        const bool key = hh >= a.q.heads;
-        const RopeTensor &t = key ? a.k : a.q;
-        const uint8_t *src = t.src + tok * t.s_tok + static_cast<uint64_t>(key ? hh - a.q.heads : hh) * t.s_head;
-        load8<TYPE, VEC>(src + e0 * t.s_dim, t.s_dim, x0);
-        load8<TYPE, VEC>(src + e1 * t.s_dim, t.s_dim, x1);
-    };
-    if (in && h < heads) fetch(h);
-    if (half) {
-        const double pos = static_cast<double>(a.pos[tok]);
-        for (uint32_t i = threadIdx.x; i < half; i += kRopeThreads) {
-            const double ang = pos * static_cast<double>(a.freqs[i]);
-            // 2 pi to 106 bits: its F64 value and the remainder
-            const double k = rint(ang * 0.15915494309189533577);
-            const double r = fma(-k, 2.4492935982947064e-16, fma(-k, 6.2831853071795864769, ang));
-            float sn, cs;
-            sincosf(static_cast<float>(r), &sn, &cs);
-            turn[i] = make_float2(cs, sn);
-        }
-        __syncthreads();
-    }
-    for (; h < heads; h += per_pass) {
+    auto address = [&](uint32_t h, bool out) -> uint64_t {
         const bool key = h >= a.q.heads;
         const RopeTensor &t = key ? a.k : a.q;
-        float ss = 0.0f;
-        if (in) {
+        const uint64_t hh = key ? h - a.q.heads : h;
+        return out ? reinterpret_cast<uint64_t>(t.dst) + tok * t.d_tok + hh * t.d_head
+                   : reinterpret_cast<uint64_t>(t.src) + tok * t.s_tok + hh * t.s_head;
+    };
+    auto fetch = [&](uint32_t h, float (&x0)[8], float (&x1)[8]) {
+        const uint64_t dim = h >= a.q.heads ? a.k.s_dim : a.q.s_dim;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(address(h, false));
+        load8<TYPE, VEC>(src + e0 * dim, dim, x0);
+        load8<TYPE, VEC>(src + e1 * dim, dim, x1);
+    };
+    float x0[8], x1[8], n0[8], n1[8], w0[8], w1[8], cs[8], sn[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
-        }
-        // the threads of a head are neighbours in a warp and leave the loop together
-        for (uint32_t o = a.lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(__activemask(), ss, o);
-        const float rs = rsqrtf(ss / static_cast<float>(a.head_dim) + a.eps);
-        if (in) {
-            float y0[8], y1[8];
+    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+    if (in) {
+        fetch(h0, x0, x1);
+        load_weights<VEC>(h0 < a.q.heads ? a.q.weight : a.k.weight, e0, w0);
+        load_weights<VEC>(h0 < a.q.heads ? a.q.weight : a.k.weight, e1, w1);
+        if (rot) {
+            const double pos = static_cast<double>(a.pos[tok]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                y0[i] = x0[i] * rs * (t.weight ? t.weight[e0 + i] : 1.0f);
-                y1[i] = x1[i] * rs * (t.weight ? t.weight[e1 + i] : 1.0f);
+                const double ang = pos * static_cast<double>(a.freqs[e0 + i]);
+                // in half turns: 1 / pi to 106 bits, its F64 value and the remainder
+                const double turn = ang * 0.31830988618379067154;
+                const double rest = fma(ang, 0.31830988618379067154, -turn) + ang * -1.9678676675182486e-17;
+                const double near = turn - 2.0 * rint(0.5 * turn);
+                sincospif(static_cast<float>(near + rest), &sn[i], &cs[i]);
             }
-            if (rot) {
+        }
+    }
+    // every thread of the warp takes the same number of turns (per_split), so the
+    // head's threads can reduce with full-warp shuffles
+    for (uint32_t j = 0; j < a.per_split; ++j) {
+        const uint32_t h = h0 + j;
+        const bool on = in && h < h1;
+        if (in && h + 1 < h1) fetch(h + 1, n0, n1);
+        if (on && h == a.q.heads && j) {
+            load_weights<VEC>(a.k.weight, e0, w0);
+            load_weights<VEC>(a.k.weight, e1, w1);
+        }
+        float ss = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 cs = turn[e0 + i];
-                    const float u = y0[i] * cs.x - y1[i] * cs.y;
-                    y1[i] = y1[i] * cs.x + y0[i] * cs.y;
-                    y0[i] = u;
-                }
+        for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+        for (uint32_t o = a.lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (on) {
+            const float rs = rsqrtf(ss / static_cast<float>(a.head_dim) + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y0 = x0[i] * rs * w0[i], y1 = x1[i] * rs * w1[i];
+                x0[i] = rot ? y0 * cs[i] - y1 * sn[i] : y0;
+                x1[i] = rot ? y1 * cs[i] + y0 * sn[i] : y1;
             }
-            uint8_t *dst = t.dst + tok * t.d_tok + static_cast<uint64_t>(key ? h - a.q.heads : h) * t.d_head;
-            if (h + per_pass < heads) fetch(h + per_pass);
-            store8<TYPE, VEC>(dst + e0 * t.d_dim, t.d_dim, y0);
-            store8<TYPE, VEC>(dst + e1 * t.d_dim, t.d_dim, y1);
+            const uint64_t dim = h >= a.q.heads ? a.k.d_dim : a.q.d_dim;
+            uint8_t *dst = reinterpret_cast<uint8_t *>(address(h, true));
+            store8<TYPE, VEC>(dst + e0 * dim, dim, x0);
+            store8<TYPE, VEC>(dst + e1 * dim, dim, x1);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x0[i] = n0[i];
+            x1[i] = n1[i];
         }
     }
 }
 
 template <int TYPE>
 void launch(const RopeArgs &a, uint32_t n, bool vec, cudaStream_t st) {
-    if (vec) qk_norm_rope_kernel<TYPE, true><<<n, kRopeThreads, 0, st>>>(a);
-    else qk_norm_rope_kernel<TYPE, false><<<n, kRopeThreads, 0, st>>>(a);
+    const uint64_t threads = static_cast<uint64_t>(n) * a.splits * a.lanes;
+    const uint32_t grid = static_cast<uint32_t>((threads + kRopeThreads - 1) / kRopeThreads);
+    if (vec) qk_norm_rope_kernel<TYPE, true><<<grid, kRopeThreads, 0, st>>>(a);
+    else qk_norm_rope_kernel<TYPE, false><<<grid, kRopeThreads, 0, st>>>(a);
 }
 
 RopeTensor tensor(const kvm_rows *in, const kvm_rows *out, const float *w) {
@@ -230,7 +263,14 @@ extern "C" kvm_status kvm_qk_norm_rope(kvm_stream stream, uint32_t n, const kvm_
     a.n_rot = n_rot;
     a.lanes = 1;
     while (a.lanes < D / 16u) a.lanes *= 2;
-    const bool vec = rows_vec16(q) && rows_vec16(q_out) && (!k || (rows_vec16(k) && rows_vec16(k_out)));
+    const uint32_t heads = a.q.heads + a.k.heads;
+    const uint64_t fill = 1024ull * num_sms(), have = static_cast<uint64_t>(n) * a.lanes;
+    a.n = n;
+    a.per_split = heads;
+    if (have < fill) a.per_split = static_cast<uint32_t>(std::max<uint64_t>(1, heads * have / fill));
+    a.splits = (heads + a.per_split - 1) / a.per_split;
+    if (static_cast<uint64_t>(n) * a.splits * a.lanes / kRopeThreads > 0x7ffffff0ull) return layer_fail(KVM_EINVAL, "%s: too many rows", me);
+    const bool vec = ((reinterpret_cast<uintptr_t>(d_q_weight) | reinterpret_cast<uintptr_t>(d_k_weight)) & 15u) == 0 && rows_vec16(q) && rows_vec16(q_out) && (!k || (rows_vec16(k) && rows_vec16(k_out)));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (q->type == KVM_TYPE_F32) launch<KVM_TYPE_F32>(a, n, vec, st);
     else if (q->type == KVM_TYPE_F16) launch<KVM_TYPE_F16>(a, n, vec, st);

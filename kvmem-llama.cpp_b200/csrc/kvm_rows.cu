@@ -6,7 +6,11 @@
 // ggml's quantize_row_*_ref and of the stage-in.  Read: code * scale, exact in
 // F32, rounded once to the output's type.
 //
-// Both are HBM- or latency-bound streams over 32-value blocks.
+// Both are HBM- or latency-bound streams over 32-value blocks.  Write: a thread a
+// block -- the block's maximum and its codes need no exchange -- with the values
+// loaded as 16-byte vectors; the 18- to 34-byte blocks of a warp are collected in
+// shared memory and leave as words, two blocks (always a whole number of words)
+// at a time.  Read: a thread eight consecutive values, one 16-byte store.
 #include <cuda_bf16.h>
 
 #include "kvm_layer.cuh"
@@ -44,6 +48,17 @@ __device__ __forceinline__ void act_store(uint8_t *p, float x) {
     if constexpr (TYPE == KVM_TYPE_F32) *reinterpret_cast<float *>(p) = x;
     else if constexpr (TYPE == KVM_TYPE_F16) *reinterpret_cast<__half *>(p) = __float2half_rn(x);
     else *reinterpret_cast<__nv_bfloat16 *>(p) = __float2bfloat16_rn(x);
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t act_pack(float x, float y) {
+    if constexpr (TYPE == KVM_TYPE_F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
 }
 
 // Byte offset of block b's first value in a row of heads.
@@ -101,56 +116,113 @@ __device__ __forceinline__ void write_block(const float (&x)[32], int32_t type, 
 }
 
 // A thread a block; blocks of a row are neighbours.
-template <int TYPE>
+template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) write_rows_kernel(const __grid_constant__ RowsArgs a) {
+    __shared__ __align__(16) uint8_t stage[kRowsThreads * kBlockBytesQ8];
     const RowsSide &s = a.side[blockIdx.y];
     if (!s.on) return;
+    const int lane = threadIdx.x & 31, bb = block_bytes(s.cache_type);
+    uint8_t *mine = stage + (threadIdx.x & ~31) * kBlockBytesQ8;
+    // pairs of blocks lie in one row and start at a word: the word path
+    const bool words = s.cache_type != KVM_TYPE_F16 && a.blocks % 2u == 0;
     const uint64_t all = static_cast<uint64_t>(a.n) * a.blocks;
-    for (uint64_t i = blockIdx.x * static_cast<uint64_t>(kRowsThreads) + threadIdx.x; i < all;
-         i += static_cast<uint64_t>(gridDim.x) * kRowsThreads) {
+    for (uint64_t i0 = blockIdx.x * static_cast<uint64_t>(kRowsThreads) + (threadIdx.x & ~31); i0 < all;
+         i0 += static_cast<uint64_t>(gridDim.x) * kRowsThreads) {
+        const uint64_t i = i0 + lane;
         const uint32_t row = static_cast<uint32_t>(i / a.blocks), b = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * a.blocks);
-        const int64_t cell = a.cells[row];
-        if (cell < 0 || cell >= a.n_cells) continue;
-        const uint8_t *src = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b);
-        float x[32];
+        const int64_t cell = i < all ? a.cells[row] : -1;
+        const bool on = cell >= 0 && cell < a.n_cells;
+        uint8_t *dst = on ? s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb : nullptr;
+        if (on) {
+            const uint8_t *src = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b);
+            float x[32];
+            if constexpr (VEC) {
+                uint4 raw[TYPE == KVM_TYPE_F32 ? 8 : 4];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = act_load<TYPE>(src + e * s.nb_dim);
-        const int bb = block_bytes(s.cache_type);
-        write_block(x, s.cache_type, s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb);
+                for (int k = 0; k < (TYPE == KVM_TYPE_F32 ? 8 : 4); ++k) raw[k] = reinterpret_cast<const uint4 *>(src)[k];
+                const uint8_t *p = reinterpret_cast<const uint8_t *>(raw);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = act_load<TYPE>(p + e * (TYPE == KVM_TYPE_F32 ? 4 : 2));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = act_load<TYPE>(src + e * s.nb_dim);
+            }
+            write_block(x, s.cache_type, words ? mine + lane * bb : dst);
+        }
+        if (words) {
+            __syncwarp();
+            const int per = bb / 2;                      // words of a pair
+            const uint32_t ok = __ballot_sync(0xffffffffu, on);
+            const uint64_t base = reinterpret_cast<uint64_t>(dst);
+            for (int w = lane; w < 16 * per + 31 - (16 * per + 31) % 32; w += 32) {
+                const int pair = min(w / per, 15), at = w - pair * per;
+                uint8_t *to = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, base, 2 * pair));
+                if (w < 16 * per && ((ok >> (2 * pair)) & 1u))
+                    reinterpret_cast<uint32_t *>(to)[at] = *reinterpret_cast<const uint32_t *>(mine + w * 4);
+            }
+            __syncwarp();
+        }
     }
 }
 
-template <int TYPE>
+// A thread eight consecutive values: quarter `c` of a block.
+template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const __grid_constant__ RowsArgs a) {
     const RowsSide &s = a.side[blockIdx.y];
     if (!s.on) return;
-    const uint64_t all = static_cast<uint64_t>(a.n) * a.blocks;
+    const int bb = block_bytes(s.cache_type);
+    const uint32_t per_row = a.blocks * 4u;
+    const uint64_t all = static_cast<uint64_t>(a.n) * per_row;
+    auto u16 = [](const uint8_t *q) { return static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(q)); };
     for (uint64_t i = blockIdx.x * static_cast<uint64_t>(kRowsThreads) + threadIdx.x; i < all;
          i += static_cast<uint64_t>(gridDim.x) * kRowsThreads) {
-        const uint32_t row = static_cast<uint32_t>(i / a.blocks), b = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * a.blocks);
+        const uint32_t row = static_cast<uint32_t>(i / per_row), in_row = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * per_row);
+        const uint32_t b = in_row >> 2, c = in_row & 3u;
         const int64_t cell = a.cells[row];
-        uint8_t *dst = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b);
+        float x[8];
         if (cell < 0 || cell >= a.n_cells) {
-            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, 0.0f);
-            continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        } else {
+            const uint8_t *p = s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb;
+            if (s.cache_type == KVM_TYPE_F16) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __half2float(__ushort_as_half(static_cast<uint16_t>(u16(p + 16 * c + 2 * e))));
+            } else {
+                const float d = __half2float(__ushort_as_half(static_cast<uint16_t>(u16(p))));
+                if (s.cache_type == KVM_TYPE_Q8_0) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = u16(p + 2 + 8 * c + 2 * e);
+                        x[2 * e] = d * static_cast<float>(static_cast<int8_t>(w & 255u));
+                        x[2 * e + 1] = d * static_cast<float>(static_cast<int8_t>(w >> 8));
+                    }
+                } else {
+                    const bool q5 = s.cache_type == KVM_TYPE_Q5_0;
+                    const uint32_t fifth = q5 ? u16(p + 2 + 2 * (c >> 1)) >> (8 * (c & 1u)) : 0u;
+                    const uint32_t shift = c < 2 ? 0u : 4u;
+                    const int mid = q5 ? 16 : 8;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = u16(p + bb - 16 + 8 * (c & 1u) + 2 * e) >> shift;
+                        const int c0 = static_cast<int>((w & 15u) | ((fifth >> (2 * e)) & 1u) << 4);
+                        const int c1 = static_cast<int>(((w >> 8) & 15u) | ((fifth >> (2 * e + 1)) & 1u) << 4);
+                        x[2 * e] = d * static_cast<float>(c0 - mid);
+                        x[2 * e + 1] = d * static_cast<float>(c1 - mid);
+                    }
+                }
+            }
         }
-        const int bb = block_bytes(s.cache_type);
-        const uint8_t *p = s.cache + static_cast<uint64_t>(cell) * s.row_bytes + static_cast<uint64_t>(b) * bb;
-        auto half_at = [](const uint8_t *q) { return __half2float(*reinterpret_cast<const __half *>(q)); };
-        if (s.cache_type == KVM_TYPE_F16) {
-            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, half_at(p + 2 * e));
-            continue;
-        }
-        const float d = half_at(p);
-        if (s.cache_type == KVM_TYPE_Q8_0) {
-            for (int e = 0; e < 32; ++e) act_store<TYPE>(dst + e * s.nb_dim, d * static_cast<float>(static_cast<int8_t>(p[2 + e])));
-            continue;
-        }
-        const bool q5 = s.cache_type == KVM_TYPE_Q5_0;
-        for (int e = 0; e < 32; ++e) {
-            int c = (p[bb - 16 + (e & 15)] >> (e < 16 ? 0 : 4)) & 15;
-            if (q5) c |= ((p[2 + e / 8] >> (e & 7)) & 1) << 4;
-            act_store<TYPE>(dst + e * s.nb_dim, d * static_cast<float>(c - (q5 ? 16 : 8)));
+        uint8_t *dst = s.act + row * s.nb_tok + block_offset(s, a.head_dim, b) + 8 * c * s.nb_dim;
+        if constexpr (VEC && TYPE == KVM_TYPE_F32) {
+            reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else if constexpr (VEC) {
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(act_pack<TYPE>(x[0], x[1]), act_pack<TYPE>(x[2], x[3]),
+                                                         act_pack<TYPE>(x[4], x[5]), act_pack<TYPE>(x[6], x[7]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) act_store<TYPE>(dst + e * s.nb_dim, x[e]);
         }
     }
 }
@@ -189,18 +261,22 @@ kvm_status rows_call(const char *me, bool write, kvm_stream stream, const kvm_ca
         s.nb_head = x->nb_head;
         s.nb_tok = x->nb_tok;
     }
-    const uint64_t want = (static_cast<uint64_t>(n) * a.blocks + kRowsThreads - 1) / kRowsThreads;
-    const uint64_t most = 8ull * num_sms();
+    const uint64_t want = (static_cast<uint64_t>(n) * a.blocks * (write ? 1u : 4u) + kRowsThreads - 1) / kRowsThreads;
+    const uint64_t most = 32ull * num_sms();
     const dim3 grid(static_cast<uint32_t>(want < most ? want : most), 2);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int32_t type = (k ? k : v)->type;
-    auto go = [&](auto write_kernel, auto read_kernel) {
-        if (write) write_kernel<<<grid, kRowsThreads, 0, st>>>(a);
-        else read_kernel<<<grid, kRowsThreads, 0, st>>>(a);
+    const bool vec = (!k || rows_vec16(k)) && (!v || rows_vec16(v));
+    auto go = [&](auto ty) {
+        constexpr int T = decltype(ty)::value;
+        if (write && vec) write_rows_kernel<T, true><<<grid, kRowsThreads, 0, st>>>(a);
+        else if (write) write_rows_kernel<T, false><<<grid, kRowsThreads, 0, st>>>(a);
+        else if (vec) read_rows_kernel<T, true><<<grid, kRowsThreads, 0, st>>>(a);
+        else read_rows_kernel<T, false><<<grid, kRowsThreads, 0, st>>>(a);
     };
-    if (type == KVM_TYPE_F32) go(write_rows_kernel<KVM_TYPE_F32>, read_rows_kernel<KVM_TYPE_F32>);
-    else if (type == KVM_TYPE_F16) go(write_rows_kernel<KVM_TYPE_F16>, read_rows_kernel<KVM_TYPE_F16>);
-    else go(write_rows_kernel<KVM_TYPE_BF16>, read_rows_kernel<KVM_TYPE_BF16>);
+    if (type == KVM_TYPE_F32) go(std::integral_constant<int, KVM_TYPE_F32>{});
+    else if (type == KVM_TYPE_F16) go(std::integral_constant<int, KVM_TYPE_F16>{});
+    else go(std::integral_constant<int, KVM_TYPE_BF16>{});
     return layer_cuda(cudaGetLastError(), me);
 }
 
