@@ -9,6 +9,8 @@ namespace kvm {
 
 template <int D, int KT>
 cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st);
+template <int D, int KT>
+cudaError_t launch_attend_tile(const AttendArgs &a, int vt, uint32_t grid, cudaStream_t st);
 
 bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -35,13 +37,19 @@ bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const At
 
 namespace {
 
+// One of the two kernels: split with row tiles of 8 * nt rows, or (nt = 0) tile.
+template <int D, int KT>
+cudaError_t launch_kt(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st) {
+    return nt ? launch_attend_split<D, KT>(a, vt, nt, grid, st) : launch_attend_tile<D, KT>(a, vt, grid, st);
+}
+
 template <int D>
-cudaError_t split_d(const AttendArgs &a, int kt, int vt, int nt, uint32_t grid, cudaStream_t st) {
+cudaError_t launch_d(const AttendArgs &a, int kt, int vt, int nt, uint32_t grid, cudaStream_t st) {
     switch (kt) {
-        case KVM_TYPE_Q4_0: return launch_attend_split<D, KVM_TYPE_Q4_0>(a, vt, nt, grid, st);
-        case KVM_TYPE_Q5_0: return launch_attend_split<D, KVM_TYPE_Q5_0>(a, vt, nt, grid, st);
-        case KVM_TYPE_Q8_0: return launch_attend_split<D, KVM_TYPE_Q8_0>(a, vt, nt, grid, st);
-        default: return launch_attend_split<D, KVM_TYPE_F16>(a, vt, nt, grid, st);
+        case KVM_TYPE_Q4_0: return launch_kt<D, KVM_TYPE_Q4_0>(a, vt, nt, grid, st);
+        case KVM_TYPE_Q5_0: return launch_kt<D, KVM_TYPE_Q5_0>(a, vt, nt, grid, st);
+        case KVM_TYPE_Q8_0: return launch_kt<D, KVM_TYPE_Q8_0>(a, vt, nt, grid, st);
+        default: return launch_kt<D, KVM_TYPE_F16>(a, vt, nt, grid, st);
     }
 }
 
@@ -111,22 +119,39 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     a.align16 = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.row_k | a.row_v) & 15u) == 0;
     a.tma = a.align16 && c->block_tokens % kAttendStep == 0;
     a.q_vec = rows_vec16(q);
+    a.out_vec = rows_vec16(out);
     a.heads_cta = c->n_head_kv % 4u == 0 ? 4 : c->n_head_kv % 2u == 0 ? 2 : 1;
-    a.min_rows = 1;
-    a.max_rows = 0xffffffffu;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    // row tiles of 8 when every request fits one, else of 16
-    const int nt = static_cast<uint64_t>(b->max_new) * a.group <= 8u ? 1 : 2;
-    // no more CTAs than a warp's step each can fill
-    const uint64_t tiles = static_cast<uint64_t>(b->n_rows) * a.group / (8u * nt) + b->n_seq;
-    const uint64_t steps = (static_cast<uint64_t>(b->table_cols) * c->block_tokens + kAttendStep - 1) / kAttendStep + 1;
-    const uint64_t most = static_cast<uint64_t>(num_sms());
-    uint64_t grid = most;
-    if (tiles * c->n_head_kv <= 8u * most) grid = std::min<uint64_t>(most, (tiles * c->n_head_kv * std::min<uint64_t>(steps, 1u << 24) + 3) / 4);
-    grid = std::max<uint64_t>(1, std::min<uint64_t>(grid, kAttendMaxCtas));
+    const uint64_t sms = static_cast<uint64_t>(num_sms());
+    // no more CTAs than the call can have work for: row tiles of r rows, steps of k keys
+    auto ctas = [&](uint32_t r, uint32_t k, uint32_t heads) -> uint32_t {
+        const uint64_t tiles = static_cast<uint64_t>(b->n_rows) * a.group / r + b->n_seq;
+        const uint64_t steps = (static_cast<uint64_t>(b->table_cols) * c->block_tokens + k - 1) / k + 1;
+        const uint64_t items = tiles * (c->n_head_kv / heads);
+        uint64_t n = std::min<uint64_t>(sms, kAttendMaxCtas);
+        if (items < n && steps < n) n = std::min(n, items * steps);
+        return static_cast<uint32_t>(std::max<uint64_t>(n, 1));
+    };
+    auto launch = [&](int nt, uint32_t min_rows, uint32_t max_rows) {
+        a.min_rows = min_rows;
+        a.max_rows = max_rows;
+        const uint32_t grid = nt ? ctas(8u * nt, kAttendStep, a.heads_cta) : ctas(128, 64, 1);
+        if (D == 64u) return launch_d<64>(a, c->type_k, c->type_v, nt, grid, st);
+        if (D == 128u) return launch_d<128>(a, c->type_k, c->type_v, nt, grid, st);
+        return launch_d<256>(a, c->type_k, c->type_v, nt, grid, st);
+    };
+    // Requests of up to 16 query rows go to the split kernel, longer ones to the tile
+    // kernel; the device sorts them, so a wrong max_new only costs time.  One
+    // request that should be long needs no second launch.
+    const uint64_t most = static_cast<uint64_t>(b->max_new) * a.group;
     cudaError_t e;
-    if (D == 64u) e = split_d<64>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
-    else if (D == 128u) e = split_d<128>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
-    else e = split_d<256>(a, c->type_k, c->type_v, nt, static_cast<uint32_t>(grid), st);
+    if (most <= 16u) {
+        e = launch(most <= 8u ? 1 : 2, 1, 0xffffffffu);
+    } else if (b->n_seq == 1) {
+        e = launch(0, 1, 0xffffffffu);
+    } else {
+        e = launch(2, 1, 16);
+        if (e == cudaSuccess) e = launch(0, 17, 0xffffffffu);
+    }
     return layer_cuda(e, me);
 }

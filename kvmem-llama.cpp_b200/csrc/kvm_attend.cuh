@@ -39,11 +39,15 @@ struct AttendArgs {
     uint8_t *work;             // split descriptors, then partial results
     uint32_t align16;          // cache bases and row bytes are multiples of 16
     uint32_t tma;              // the cache's rows come through map_k, map_v (steps lie in one block)
-    uint32_t q_vec;            // q: contiguous heads, 16-byte aligned
+    uint32_t q_vec, out_vec;   // contiguous heads, 16-byte aligned
     uint32_t heads_cta;        // KV heads that a CTA takes together: 1, 2 or 4
     uint32_t min_rows, max_rows;   // query rows (tokens * group) a sequence needs to be taken by this launch
     CUtensorMap map_k, map_v;      // [cells][row bytes / 4] of 32-bit words
 };
+
+// Tensor map of one side of the cache: rows of 32-bit words, boxes of a step's
+// 16 rows by box_bytes.  False when the driver cannot make it.
+bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes);
 
 // A sequence as the kernels see it; nothing read from device memory is trusted
 // to stay inside the tables.
@@ -54,7 +58,7 @@ struct AttendSeq {
     int32_t keys;              // keys held by the table
 };
 
-__device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, uint32_t s) {
+__host__ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, uint32_t s) {
     AttendSeq q;
     const int64_t lo = a.q_start[s], hi = a.q_start[s + 1];
     const int64_t kv = max(a.kv_len[s], 0);
@@ -69,7 +73,7 @@ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, uint32_t s)
 }
 
 // Keys that row token i of the sequence sees.
-__device__ __forceinline__ int32_t attend_limit(const AttendArgs &a, const AttendSeq &q, int32_t i) {
+__host__ __device__ __forceinline__ int32_t attend_limit(const AttendArgs &a, const AttendSeq &q, int32_t i) {
     if (!a.causal) return q.keys;
     return max(0, min(q.keys, static_cast<int32_t>(min(static_cast<int64_t>(q.shift) + i + 1,
                                                        static_cast<int64_t>(0x7fffff00)))));

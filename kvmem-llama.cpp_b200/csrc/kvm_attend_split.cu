@@ -6,10 +6,6 @@
 
 namespace kvm {
 
-// Tensor map of one side of the cache: rows of 32-bit words, boxes of a step's
-// 16 rows by box_bytes.  False when the driver cannot make it.
-bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes);
-
 namespace {
 
 template <int D, int KT, int VT, int NT>

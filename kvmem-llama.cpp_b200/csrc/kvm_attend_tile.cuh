@@ -1,0 +1,875 @@
+// kvm_attend_tile.cuh -- attend_tile_kernel: attention for many query rows a
+// sequence (prompt chunks, drafts), bound by the tensor cores.
+//
+// A work item is 128 rows (token, query head of one KV head) against the keys
+// they see, 64 keys at a time:
+//     S = Q K^T  (128 x 64, tcgen05, Q from TMEM, K from shared memory)
+//     P = exp2(S * f - m)             -> F16 in TMEM, over S
+//     O += P V   (128 x D, tcgen05, P from TMEM, V from shared memory)
+// K and V enter as F16 values code * d, rounded once: unlike the few-row kernel
+// this one is not bound by the window's bytes, and dequantizing once for 128
+// rows leaves the tensor cores plain F16 operands.  Q is scaled a row by a power
+// of two (exact for 16-bit inputs but for elements 2^24 below the row's
+// largest), P is F16, all sums and statistics are F32.  The running maximum is
+// raised only when it would grow by more than 2^8, so O in TMEM is rescaled
+// rarely; P carries a factor 2^7 that cancels in the quotient, which keeps it
+// below F16's top and its bits down to 2^-31 of the row's largest weight.
+//
+// Roles (13 warps, one CTA an SM): warps 0-3 own the 128 rows (Q into TMEM,
+// softmax, epilogue), warps 4-7 turn raw K rows into an operand tile, warps 8-11
+// raw V rows, warp 12 issues the products.  Everything is double-buffered on
+// mbarriers: QK of tile j + 1 is issued before PV of tile j, so that the softmax
+// of one tile runs under the products of the other.  With D = 256: S 2 x 64,
+// O 256 and Q 128 columns are all of TMEM; Q there rather than in shared memory
+// halves what QK reads from shared memory, which would otherwise bound it at
+// N = 64 (A 4 KB + B 2 KB an instruction of 32 cycles, at 128 bytes a cycle).
+//
+// Operand tiles: rows of 64 keys by 128-byte chunks of 64 dims with the 128-byte
+// swizzle; K is read K-major, V from the same layout MN-major.  Which dim a
+// position stands for is free as long as Q (for K) and the epilogue (for V)
+// agree: q4_0 and q5_0 keep the order their nibbles fall out in (position i of
+// eight holds value 0 2 1 3 4 6 5 7).
+//
+// The (item, key tile) pairs of the call form one line, shared evenly by the
+// CTAs; an item that several CTAs share leaves its pieces' maxima, sums and
+// normalised F16 outputs (one rounding as large as the output's own) for
+// attend_tile_join_kernel.
+#pragma once
+
+#include "kvm_attend_split.cuh"
+
+namespace kvm {
+
+constexpr int kTileRows = 128, kTileKeys = 64, kTileThreads = 13 * 32;
+
+template <int D, int KT, int VT>
+struct TileGeom {
+    using K = Slice<KT, D>;
+    using V = Slice<VT, D>;
+    static constexpr int kOperand = kTileKeys * D * 2;             // one K or V tile
+    static constexpr int kRawK = kAttendStep * K::kStride, kRawV = kAttendStep * V::kStride;   // a warp's 16 keys
+    static constexpr int kRoom = 220 * 1024 - 4 * kOperand;
+    static constexpr int kFit = kRoom / (4 * (kRawK + kRawV));
+    static constexpr int kStages = kFit > 6 ? 6 : kFit < 1 ? 1 : kFit;
+    static constexpr int kRaw = 4 * kOperand;                      // offset of the raw rings
+    static constexpr int kBars = kRaw + 4 * kStages * (kRawK + kRawV);
+    static constexpr int kSmem = kBars + 1024 + 1024;              // barriers; alignment of the operand tiles
+};
+
+// ------------------------------------------------------------- tcgen05 PTX --
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem], F16 operands, F32 accumulator.
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld32(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptor: 128-byte swizzle, byte strides.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | static_cast<uint64_t>((lbo >> 4) & 0x3fffu) << 16 |
+           static_cast<uint64_t>((sbo >> 4) & 0x3fffu) << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: F16 x F16 -> F32, M = 128.
+constexpr uint32_t tc_idesc(int n, bool b_mn_major) {
+    return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | static_cast<uint32_t>(n / 8) << 17 | (128u / 16) << 24;
+}
+
+// ------------------------------------------------------------- work line --
+// sum_{i < n} floor((a i + b) / m), all arguments non-negative, m > 0.
+__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+    int64_t sum = 0;
+    for (;;) {
+        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const int64_t top = a * n + b;
+        if (top < m) return sum;
+        n = top / m;
+        b = top % m;
+        const int64_t x = m;
+        m = a;
+        a = x;
+    }
+}
+
+struct TileSeq {
+    AttendSeq q;
+    int64_t tiles;       // row tiles, 0 = not taken by this kernel
+    int64_t cap;         // keys its last row sees
+};
+
+__host__ __device__ __forceinline__ TileSeq tile_seq(const AttendArgs &a, uint32_t s) {
+    TileSeq t;
+    t.q = attend_seq(a, s);
+    const int64_t rows = static_cast<int64_t>(t.q.n_new) * a.group;
+    t.tiles = (t.q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) ? 0 : (rows + kTileRows - 1) / kTileRows;
+    t.cap = t.q.n_new > 0 ? attend_limit(a, t.q, t.q.n_new - 1) : 0;
+    return t;
+}
+
+// Key tiles of row tile i: those its last row sees, at least one.
+__host__ __device__ __forceinline__ int64_t tile_steps(const AttendArgs &a, const TileSeq &t, int64_t i) {
+    const int64_t last = min(((i + 1) * kTileRows - 1) / static_cast<int64_t>(a.group), static_cast<int64_t>(t.q.n_new) - 1);
+    const int64_t keys = attend_limit(a, t.q, static_cast<int32_t>(last));
+    return max(static_cast<int64_t>(1), (keys + kTileKeys - 1) / kTileKeys);
+}
+
+// Key tiles of the first n row tiles.  Row tile i's last token is
+// floor((128 i + 127) / group) (the sequence's last for the last tile), so its
+// count is floor((group (shift + 64) + 128 i + 127) / (64 group)) between the
+// tiles that need one key tile and those that see `cap` keys.
+__host__ __device__ inline int64_t tile_prefix(const AttendArgs &a, const TileSeq &t, int64_t n) {
+    const int64_t most = max(static_cast<int64_t>(1), (t.cap + kTileKeys - 1) / kTileKeys);
+    if (!a.causal) return n * most;
+    const int64_t g = a.group, shift = t.q.shift;
+    auto first_with = [&](int64_t keys) -> int64_t {      // first tile whose last row sees at least `keys`, unclamped
+        const int64_t need = g * (keys - shift - 1) - (kTileRows - 1);    // 128 i >= need
+        const int64_t i = need <= 0 ? 0 : (need + kTileRows - 1) / kTileRows;
+        return i < n ? i : n;
+    };
+    const int64_t ones = first_with(kTileKeys + 1), full = max(ones, first_with(t.cap));
+    int64_t sum = ones + (n - full) * most;
+    if (full > ones)
+        sum += floor_sum(full - ones, kTileKeys * g, kTileRows, g * (shift + kTileKeys) + kTileRows * ones + kTileRows - 1);
+    return sum;
+}
+
+// One CTA's part of one item.
+struct TilePiece {
+    AttendSeq q;
+    uint32_t seq, head, first, rows;     // first: (token, group) row of the tile in the sequence
+    int32_t in0, in1;                    // key tiles
+    int32_t kend, kfull;                 // keys any row / every row sees
+    bool starts, ends;
+    uint32_t more;                       // CTAs behind this one that share the item
+};
+
+// Walks the pieces of a CTA; every thread of the CTA runs it alike.
+struct TileWalk {
+    uint64_t pos, u1, share;
+    uint32_t seq;
+    TileSeq t;
+    int64_t tile, head, in0, steps;      // where in the sequence's items
+
+    // Position `off` of sequence s's items.
+    __host__ __device__ __forceinline__ void seek(const AttendArgs &a, uint32_t s, int64_t off) {
+        seq = s;
+        t = tile_seq(a, s);
+        const int64_t heads = a.n_head_kv;
+        int64_t lo = 0, hi = t.tiles;    // the last tile whose items start at or before off
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (heads * tile_prefix(a, t, mid) <= off) lo = mid;
+            else hi = mid;
+        }
+        tile = lo;
+        steps = tile_steps(a, t, tile);
+        off -= heads * tile_prefix(a, t, lo);
+        head = off / steps;
+        in0 = off - head * steps;
+    }
+
+    __host__ __device__ __forceinline__ bool next(const AttendArgs &a, TilePiece &p) {
+        if (pos >= u1) return false;
+        while (in0 == steps) {           // the next item
+            in0 = 0;
+            if (++head < a.n_head_kv) break;
+            head = 0;
+            if (++tile < t.tiles) {
+                steps = tile_steps(a, t, tile);
+                break;
+            }
+            tile = 0;
+            do t = tile_seq(a, ++seq);
+            while (t.tiles == 0);        // u1 is within the line, so there is one
+            steps = tile_steps(a, t, 0);
+        }
+        const int64_t left = steps - in0;
+        const int64_t take = min(left, static_cast<int64_t>(u1 - pos));
+        p.q = t.q;
+        p.seq = seq;
+        p.head = static_cast<uint32_t>(head);
+        p.first = static_cast<uint32_t>(tile) * kTileRows;
+        p.rows = min(static_cast<uint32_t>(kTileRows), static_cast<uint32_t>(t.q.n_new) * a.group - p.first);
+        p.in0 = static_cast<int32_t>(in0);
+        p.kend = attend_limit(a, t.q, static_cast<int32_t>((p.first + p.rows - 1) / a.group));
+        p.kfull = attend_limit(a, t.q, static_cast<int32_t>(p.first / a.group));
+        p.in1 = min(static_cast<int32_t>(in0 + take), (p.kend + kTileKeys - 1) / kTileKeys);
+        p.starts = in0 == 0;
+        p.ends = take == left;
+        p.more = p.ends ? 0u : static_cast<uint32_t>((pos + left - u1 + share - 1) / share);
+        pos += take;
+        in0 += take;
+        return true;
+    }
+};
+
+// A piece's results in the workspace: maxima, sums, then rows of D halves.
+template <int D>
+__host__ __device__ constexpr uint32_t tile_part_bytes() { return kTileRows * (8u + 2u * D); }
+template <int D>
+__device__ __forceinline__ uint8_t *tile_part(const AttendArgs &a, uint32_t slot) {
+    return a.work + kAttendMaxCtas * kAttendDescBytes + static_cast<uint64_t>(slot) * tile_part_bytes<D>();
+}
+
+// ------------------------------------------------------------ dequantizing --
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b),
+                              *reinterpret_cast<const __half2 *>(&c));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Position i of eight holds value tile_order<T>(i).
+template <int T>
+__host__ __device__ constexpr int tile_order(int i) {
+    return Slice<T, 64>::kNibble ? (i & 4) | (i & 1) << 1 | (i & 2) >> 1 : i;
+}
+
+// Writes 16 keys' slices as F16 values into the operand tile.  `raw` is the
+// warp's 16 rows, `key0` its first row of the tile's 64, `ok` its visible keys
+// (the others become zeros).  V values that are not finite become zeros too and
+// set *odd.  An eighth of a warp takes eight keys' same 16-byte chunk, so reads
+// and swizzled stores are free of bank conflicts.
+template <int T, int D, bool IS_V>
+__device__ __forceinline__ void tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, uint32_t ok, int lane, bool *odd) {
+    using S = Slice<T, D>;
+    const int k8 = lane & 7, quad = lane >> 3;
+    auto put = [&](int key, int dim8, uint4 v) {       // dims 8 dim8 .. 8 dim8 + 7 of a key
+        const int row = key0 + key;
+        *reinterpret_cast<uint4 *>(tile + (dim8 >> 3) * (kTileKeys * 128) + row * 128 + (((dim8 & 7) ^ (row & 7)) << 4)) = v;
+    };
+    auto scale_at = [&](const uint8_t *p, int key) -> uint32_t {
+        uint32_t d = lds16(p);
+        if (IS_V && (d & 0x7c00u) == 0x7c00u && ((ok >> key) & 1u)) *odd = true;
+        if (!((ok >> key) & 1u) || (IS_V && (d & 0x7c00u) == 0x7c00u)) d = 0;
+        return d * 0x10001u;
+    };
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        const int key = 8 * half + k8;
+        const uint8_t *row = raw + key * S::kStride;
+        if constexpr (T == KVM_TYPE_F16) {
+            const bool see = (ok >> key) & 1u;
+#pragma unroll 4
+            for (int c = quad; c < D / 8; c += 4) {
+                uint4 v = *reinterpret_cast<const uint4 *>(row + 16 * c);
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (IS_V) {
+                        const bool lo = (w[i] & 0x7c00u) == 0x7c00u, hi = (w[i] & 0x7c000000u) == 0x7c000000u;
+                        if (see && (lo || hi)) *odd = true;
+                        if (lo) w[i] &= 0xffff0000u;
+                        if (hi) w[i] &= 0x0000ffffu;
+                    }
+                    if (!see) w[i] = 0;
+                }
+                put(key, c, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        } else if constexpr (T == KVM_TYPE_Q8_0) {
+#pragma unroll 4
+            for (int b = 0; b < D / 32; ++b) {
+                const uint8_t *p = row + (b >> 1) * 68;
+                const uint32_t d = scale_at(p + (b & 1) * 34, key);
+                uint32_t x[2];
+                if (b & 1) {
+                    x[0] = lds32(p + 36 + 8 * quad);
+                    x[1] = lds32(p + 40 + 8 * quad);
+                } else {
+                    const uint32_t w0 = lds32(p + 8 * quad), w1 = lds32(p + 8 * quad + 4), w2 = lds32(p + 8 * quad + 8);
+                    x[0] = __byte_perm(w0, w1, 0x5432);
+                    x[1] = __byte_perm(w1, w2, 0x5432);
+                }
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t u = x[i] ^ 0x80808080u;       // 1024 + code + 128, less 1152
+                    o[2 * i] = mul_half2(h2_sub(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u), d);
+                    o[2 * i + 1] = mul_half2(h2_sub(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u), d);
+                }
+                put(key, 4 * b + quad, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+        } else {
+            // quad: block (quad >> 1) of a pair, bytes 8 h .. 8 h + 7 of its nibbles, h = quad & 1
+            const int b = quad >> 1, h = quad & 1;
+            constexpr int kPair = 2 * S::kBlock, kCodes = S::kBlock - 16;
+            const uint32_t align = b ? 0x3210u : 0x5432u;
+#pragma unroll
+            for (int pr = 0; pr < D / 64; ++pr) {
+                const uint8_t *p = row + pr * kPair;
+                const uint32_t d = scale_at(p + b * S::kBlock, key);
+                // q4_0: the codes start at byte 2 or 20, q5_0: 6 or 28
+                const uint8_t *q = p + (b ? S::kBlock + kCodes : kCodes - 2) + 8 * h;
+                const uint32_t w0 = lds32(q), w1 = lds32(q + 4), w2 = lds32(q + 8);
+                const uint32_t x[2] = {__byte_perm(w0, w1, align), __byte_perm(w1, w2, align)};
+                uint32_t lo[4], hi[4];
+                uint32_t fl = 0, fh = 0;
+                if constexpr (T == KVM_TYPE_Q5_0) {
+                    const uint32_t f = lds16(p + b * S::kBlock + 2) >> (8 * h), e = lds16(p + b * S::kBlock + 4) >> (8 * h);
+                    fl = f;
+                    fh = e;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t y = x[i] >> 8;
+                    uint32_t l0 = (x[i] & 0x000f000fu) | 0x64006400u, l1 = (y & 0x000f000fu) | 0x64006400u;
+                    uint32_t h0 = (x[i] & 0x00f000f0u) | 0x64006400u, h1 = (y & 0x00f000f0u) | 0x64006400u;
+                    if constexpr (T == KVM_TYPE_Q5_0) {
+                        const uint32_t a = fl >> (4 * i), c = fh >> (4 * i);
+                        l0 |= ((a & 5u) * 0x00040010u) & 0x00100010u;
+                        l1 |= ((a & 10u) * 0x00020008u) & 0x00100010u;
+                        h0 |= ((c & 5u) * 0x00400100u) & 0x01000100u;
+                        h1 |= ((c & 10u) * 0x00200080u) & 0x01000100u;
+                        // 1024 + n less 1040; (1024 + 16 n) / 16 less 80
+                        lo[2 * i] = mul_half2(h2_sub(l0, 0x64106410u), d);
+                        lo[2 * i + 1] = mul_half2(h2_sub(l1, 0x64106410u), d);
+                        hi[2 * i] = mul_half2(h2_fma(h0, 0x2c002c00u, 0xd500d500u), d);
+                        hi[2 * i + 1] = mul_half2(h2_fma(h1, 0x2c002c00u, 0xd500d500u), d);
+                    } else {
+                        // 1024 + n less 1032; (1024 + 16 n) / 16 less 72
+                        lo[2 * i] = mul_half2(h2_sub(l0, 0x64086408u), d);
+                        lo[2 * i + 1] = mul_half2(h2_sub(l1, 0x64086408u), d);
+                        hi[2 * i] = mul_half2(h2_fma(h0, 0x2c002c00u, 0xd480d480u), d);
+                        hi[2 * i + 1] = mul_half2(h2_fma(h1, 0x2c002c00u, 0xd480d480u), d);
+                    }
+                }
+                put(key, 8 * pr + 4 * b + h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                put(key, 8 * pr + 4 * b + h + 2, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ kernel --
+template <int D, int KT, int VT>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __grid_constant__ AttendArgs a) {
+    using G = TileGeom<D, KT, VT>;
+    constexpr int NS = G::kStages;
+    constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 7.0f, kSlack = 8.0f;
+    constexpr uint32_t kColS = 0, kColO = 2 * kTileKeys, kColQ = kColO + D;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBars);
+    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
+             *q_full = bars + 12, *raw_full = bars + 13;          // raw_full [8 warps][NS]
+    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][4 warps]
+    __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
+    __shared__ uint32_t s_seq, s_tmem, s_odd;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_free[i], 1);
+            mbar_init(&s_full[i], 1);
+        }
+        mbar_init(q_full, 4);
+        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
+        s_odd = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+
+    // ---- this CTA's share of the line of (item, key tile)
+    auto units = [&](uint32_t s) -> unsigned long long {
+        const TileSeq t = tile_seq(a, s);
+        return t.tiles ? static_cast<unsigned long long>(a.n_head_kv * tile_prefix(a, t, t.tiles)) : 0ull;
+    };
+    auto scan = [&](unsigned long long n, unsigned long long *all) -> unsigned long long {
+        unsigned long long x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        unsigned long long before = 0, sum = 0;
+        for (int w = 0; w < kTileThreads / 32; ++w) {
+            if (w < warp) before += s_scan[w];
+            sum += s_scan[w];
+        }
+        *all = sum;
+        __syncthreads();
+        return x + before;
+    };
+    unsigned long long mine = 0, total = 0;
+    for (uint32_t s = tid; s < a.n_seq; s += kTileThreads) mine += units(s);
+    scan(mine, &total);
+    unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
+    if (share == 0) share = 1;
+    const unsigned long long u0 = share * blockIdx.x, u1 = min(u0 + share, total);
+    AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
+    if (u0 >= total) {
+        if (tid == 0) desc->parts = 0;
+        return;
+    }
+    unsigned long long carry = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += kTileThreads) {
+        const uint32_t s = base + tid;
+        unsigned long long all;
+        const unsigned long long n = s < a.n_seq ? units(s) : 0ull, x = carry + scan(n, &all);
+        if (n != 0 && x - n <= u0 && u0 < x) {
+            s_seq = s;
+            s_off = u0 - (x - n);
+        }
+        carry += all;
+        if (carry > u0) break;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    TileWalk walk;
+    walk.pos = u0;
+    walk.u1 = u1;
+    walk.share = share;
+    walk.seek(a, s_seq, static_cast<int64_t>(s_off));
+    TilePiece p;
+    bool lost = false;                         // a bounded wait ran out: go on without waiting
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+        if (!lost && !mbar_wait_bounded(bar, phase & 1u)) lost = true;
+    };
+    uint32_t j = 0;                            // running key tile of the CTA: stage j & 1, phase j >> 1
+
+    // Registers: 13 warps launch with 128 each; the rows' warps take 48 more from
+    // the dequantizing ones (4 * 32 * (176 + 104 + 104) + 32 * 128 = 416 * 128).
+    if (warp < 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        // ======== rows: Q into TMEM, softmax, epilogue
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) * 32u << 16);
+        const int row = tid;
+        bool described = false;
+        while (walk.next(a, p)) {
+            const bool in = static_cast<uint32_t>(row) < p.rows;
+            const uint32_t rr = p.first + (in ? row : 0), tok = rr / a.group;
+            const uint64_t at_tok = static_cast<uint64_t>(p.q.row0) + tok, at_head = static_cast<uint64_t>(p.head) * a.group + rr % a.group;
+            const uint8_t *qp = a.q.p + at_tok * a.q.nb_tok + at_head * a.q.nb_head;
+            const int32_t lim = in ? attend_limit(a, p.q, static_cast<int32_t>(tok)) : p.kend;
+            // the row's largest element to [2^14, 2^15)
+            float top = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+                uint32_t u[4];
+                if (a.q_vec) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * c);
+                    u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        u[i] = *reinterpret_cast<const uint16_t *>(qp + (8 * c + 2 * i) * a.q.nb_dim) |
+                               static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(qp + (8 * c + 2 * i + 1) * a.q.nb_dim)) << 16;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = a.q.bf16 ? __uint_as_float(u[i] << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] & 0xffffu)));
+                    const float y = a.q.bf16 ? __uint_as_float(u[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] >> 16)));
+                    top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                }
+            }
+            const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
+            // the sum of D products must stay in F32: a top of 2^14 leaves 2^98 for K
+            const int up = (top > 0.0f && e < 128) ? max(-126, min(126, 14 - e)) : 0;
+            const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+            const float mul = sign * __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+            const float fac = fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            // a piece without key tiles issues no products and leaves Q alone
+#pragma unroll 1
+            for (int c0 = 0; c0 < (p.in0 < p.in1 ? D / 64 : 0); ++c0) {       // 64 dims = 32 columns at a time
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float x[8];
+                    if (a.q_vec) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * (8 * c0 + c));
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[2 * i] = a.q.bf16 ? __uint_as_float(u[i] << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] & 0xffffu)));
+                            x[2 * i + 1] = a.q.bf16 ? __uint_as_float(u[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] >> 16)));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = load16(qp + (64 * c0 + 8 * c + i) * a.q.nb_dim, a.q.bf16);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[4 * c + i] = in ? pack_half2(x[tile_order<KT>(2 * i)] * mul, x[tile_order<KT>(2 * i + 1)] * mul) : 0u;
+                }
+                tc_st32(lanes + kColQ + 32 * c0, w);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && p.in0 < p.in1) mbar_arrive(q_full);
+
+            float m = kNegInf, l = 0.0f;
+            const uint32_t j0 = j;
+            for (int32_t n = p.in0; n < p.in1; ++n, ++j) {
+                const uint32_t st = j & 1u;
+                wait(&s_full[st], j >> 1);
+                // valid[] of this tile: written before k_full, which the products behind
+                // s_full waited for, and not again before the tile after next's products.
+                // (k_full itself may be a phase ahead here and must not be waited on.)
+                tc_fence_after();
+                uint32_t s0[32], s1[32];
+                tc_ld32(s0, lanes + kColS + st * kTileKeys);
+                tc_ld32(s1, lanes + kColS + st * kTileKeys + 32);
+                tc_wait_ld();
+                const uint4 ok4 = *reinterpret_cast<const uint4 *>(valid + 4 * (j & 3u));
+                const uint32_t ok0 = ok4.x | ok4.y << 16, ok1 = ok4.z | ok4.w << 16;
+                const int32_t key0 = n * kTileKeys;
+                if (key0 + kTileKeys > p.kfull || (ok0 & ok1) != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (key0 + i >= lim || !((ok0 >> i) & 1u)) s0[i] = __float_as_uint(kNegInf);
+                        if (key0 + 32 + i >= lim || !((ok1 >> i) & 1u)) s1[i] = __float_as_uint(kNegInf);
+                    }
+                }
+                float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) t4[i & 3] = fmaxf(t4[i & 3], fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+                const float x = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                const float mt = x == kNegInf ? kNegInf : x * fac;
+                if (__any_sync(0xffffffffu, mt > m + kSlack || (m == kNegInf && mt > m))) {
+                    const float mn = fmaxf(m, mt);
+                    const float f = m == kNegInf ? 0.0f : exp2_approx(m - mn);
+                    if (j != j0) {                     // O holds something: scale it behind the last product
+                        wait(&v_free[(j - 1) & 1u], (j - 1) >> 1);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tc_ld32(o, lanes + kColO + 32 * c);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(m == mn ? __uint_as_float(o[i]) : __uint_as_float(o[i]) * f);
+                            tc_st32(lanes + kColO + 32 * c, o);
+                        }
+                        tc_wait_st();
+                    }
+                    l = m == mn ? l : l * f;
+                    m = mn;
+                }
+                const float ref = m == kNegInf ? 0.0f : kWeightLog - m;
+                uint32_t w[32];
+                float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const uint32_t *s = i < 16 ? s0 + 2 * i : s1 + 2 * (i - 16);
+                    const float p0 = exp2_approx(fmaf(__uint_as_float(s[0]), fac, ref));
+                    const float p1 = exp2_approx(fmaf(__uint_as_float(s[1]), fac, ref));
+                    a0 += p0;
+                    a1 += p1;
+                    w[i] = pack_half2(p0, p1);
+                }
+                l += a0 + a1;
+                tc_st32(lanes + kColS + st * kTileKeys, w);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[st]);
+            }
+            // ---- epilogue
+            const bool any = j != j0;
+            if (any) {
+                wait(&v_free[(j - 1) & 1u], (j - 1) >> 1);
+                tc_fence_after();
+            }
+            if (lost) l = __int_as_float(0x7fc00000);
+            const bool whole = p.starts && p.ends;
+            const bool odd = *reinterpret_cast<volatile uint32_t *>(&s_odd) != 0;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint8_t *part = whole ? nullptr : tile_part<D>(a, 2u * blockIdx.x + (p.starts ? 1u : 0u));
+            uint8_t *op = const_cast<uint8_t *>(a.out.p) + at_tok * a.out.nb_tok + at_head * a.out.nb_head;
+            if (part) {
+                reinterpret_cast<float *>(part)[row] = m;
+                reinterpret_cast<float *>(part)[kTileRows + row] = l;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                if (any) {
+                    tc_ld32(o, lanes + kColO + 32 * c);
+                    tc_wait_ld();
+                }
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[(i & ~7) | tile_order<VT>(i & 7)] = any ? __uint_as_float(o[i]) * inv : 0.0f;
+                if (odd && in) {                       // values the tiles left out: infinities and NaN that this row sees
+                    const int32_t hi = min(lim, p.in1 * kTileKeys);
+                    for (int32_t key = p.in0 * kTileKeys; key < hi; ++key) {
+                        const uint32_t blk = static_cast<uint32_t>(key) / a.block_tokens;
+                        const int32_t slot = a.table[p.seq * a.table_stride + blk];
+                        if (slot < 0 || static_cast<uint32_t>(slot) >= a.n_slots) continue;
+                        const uint64_t cell = static_cast<uint64_t>(slot) * a.block_tokens + (key - blk * a.block_tokens);
+                        const uint8_t *v = a.v + cell * a.row_v + static_cast<uint64_t>(p.head) * G::V::kBytes;
+                        if (VT != KVM_TYPE_F16 && (*reinterpret_cast<const uint16_t *>(v + c * G::V::kBlock) & 0x7c00u) != 0x7c00u) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float x = row_value<VT>(v, 32 * c + i);
+                            if (!isfinite(x)) y[i] += x;
+                        }
+                    }
+                }
+                if (part) {
+                    uint4 *to = reinterpret_cast<uint4 *>(part + 8 * kTileRows + (row * D + 32 * c) * 2);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        to[k] = make_uint4(pack_half2(y[8 * k], y[8 * k + 1]), pack_half2(y[8 * k + 2], y[8 * k + 3]),
+                                           pack_half2(y[8 * k + 4], y[8 * k + 5]), pack_half2(y[8 * k + 6], y[8 * k + 7]));
+                } else if (in) {
+                    if (a.out_vec) {
+                        uint4 *to = reinterpret_cast<uint4 *>(op + 64 * c);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t u[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x0 = y[8 * k + 2 * i], x1 = y[8 * k + 2 * i + 1];
+                                if (a.out.bf16) {
+                                    const __nv_bfloat162 b2 = __floats2bfloat162_rn(x0, x1);
+                                    u[i] = *reinterpret_cast<const uint32_t *>(&b2);
+                                } else {
+                                    u[i] = pack_half2(x0, x1);
+                                }
+                            }
+                            to[k] = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) store16(op + (32 * c + i) * a.out.nb_dim, y[i], a.out.bf16);
+                    }
+                }
+            }
+            tc_fence_before();                         // O and Q are free for the next piece's products
+            if (tid == 0 && p.starts && !p.ends) {
+                desc->row0 = p.q.row0;
+                desc->head = p.head;
+                desc->first = p.first;
+                desc->rows = p.rows;
+                desc->parts = 1u + p.more;
+            }
+            described = described || (p.starts && !p.ends);
+        }
+        if (tid == 0 && !described) desc->parts = 0;
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        // ======== K (warps 4-7) and V (warps 8-11): raw rows to operand tiles
+        const bool is_v = warp >= 8;
+        const int w4 = warp & 3;
+        const int raw_bytes = is_v ? G::kRawV : G::kRawK;
+        uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kRawK : 0) + w4 * NS * raw_bytes;
+        uint64_t *full = raw_full + (warp - 4) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
+        uint32_t *vmask = valid + w4;
+        uint32_t issued = 0;
+        while (walk.next(a, p)) {
+            const int32_t n_tiles = max(0, p.in1 - p.in0);
+            const int32_t *trow = a.table + p.seq * a.table_stride;
+            const uint64_t slice = static_cast<uint64_t>(p.head) * (is_v ? G::V::kBytes : G::K::kBytes);
+            const int lead = a.tma ? static_cast<int>(slice & 15u) : 0;
+            uint32_t ring_ok[NS];                      // visible keys of the loads in flight
+#pragma unroll
+            for (int i = 0; i < NS; ++i) ring_ok[i] = 0;
+            // every lane computes the visible keys of the warp's 16 in tile n
+            auto load = [&](int32_t i) -> uint32_t {
+                uint8_t *st = ring + ((issued + i) % NS) * raw_bytes;
+                uint64_t *bar = &full[(issued + i) % NS];
+                const uint32_t key0 = static_cast<uint32_t>((p.in0 + i) * kTileKeys + w4 * 16);
+                const int32_t left = p.kend - static_cast<int32_t>(key0);
+                if (a.tma) {
+                    uint32_t ok = 0;
+                    if (left > 0) {
+                        const uint32_t blk = key0 / a.block_tokens;
+                        const int32_t slot = trow[blk];
+                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
+                            ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                            if (lane == 0) {
+                                const int32_t cell = static_cast<int32_t>(slot * a.block_tokens + (key0 - blk * a.block_tokens));
+                                mbar_arrive_expect_tx(bar, raw_bytes);
+                                tma_load_2d(st, is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u), cell, bar);
+                            }
+                        }
+                    }
+                    if (ok == 0 && lane == 0) mbar_arrive(bar);
+                    return ok;
+                }
+                const uint32_t key = key0 + (lane & 15);
+                int32_t cell = -1;
+                if (static_cast<int32_t>(key) < p.kend) {
+                    const uint32_t blk = key / a.block_tokens;
+                    const int32_t slot = trow[blk];
+                    if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
+                        cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
+                }
+                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
+                auto copy = [&](auto slice_t, const uint8_t *base, uint64_t row_bytes) {
+                    using S = decltype(slice_t);
+                    constexpr int C = S::kBytes / 4;
+#pragma unroll 4
+                    for (int y = 0; y < (kAttendStep * C + 31) / 32; ++y) {
+                        const int x = lane + 32 * y, r = min(x / C, kAttendStep - 1), c = x - r * C;
+                        const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
+                        if (x < kAttendStep * C)
+                            cp_async4(smem_u32(st + r * S::kStride + c * 4), base + (cr >= 0 ? cr * row_bytes + c * 4 : 0ull), cr >= 0 ? 4u : 0u);
+                    }
+                };
+                if (is_v) copy(typename G::V{}, a.v + slice, a.row_v);
+                else copy(typename G::K{}, a.k + slice, a.row_k);
+                return ok;
+            };
+#pragma unroll
+            for (int i = 0; i < NS - 1; ++i) {
+                if (i < n_tiles) ring_ok[i] = load(i);
+                cp_async_commit();
+            }
+            bool odd = false;
+            for (int32_t i = 0; i < n_tiles; ++i, ++j) {
+                if (NS == 1) ring_ok[0] = load(i);
+                if (a.tma) wait(&full[(issued + i) % NS], (issued + i) / NS);
+                else if (NS == 1) cp_async_commit(), cp_async_wait<0>();
+                else cp_async_wait<(NS > 1 ? NS - 2 : 0)>();
+                __syncwarp();
+                const uint32_t ok = ring_ok[0];
+#pragma unroll
+                for (int k = 0; k + 1 < NS; ++k) ring_ok[k] = ring_ok[k + 1];
+                if (NS > 1) {
+                    if (i + NS - 1 < n_tiles) ring_ok[NS - 2 < 0 ? 0 : NS - 2] = load(i + NS - 1);
+                    cp_async_commit();
+                }
+                if (j >= 2) wait(&tile_free[j & 1u], (j >> 1) - 1u);
+                const uint8_t *raw = ring + ((issued + i) % NS) * raw_bytes + lead;
+                uint8_t *tile = smem + (is_v ? 2 * G::kOperand : 0) + (j & 1u) * G::kOperand;
+                if (is_v) tile_dequant<VT, D, true>(raw, tile, w4 * 16, ok, lane, &odd);
+                else tile_dequant<KT, D, false>(raw, tile, w4 * 16, ok, lane, &odd);
+                if (is_v && odd) *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
+                if (!is_v && lane == 0) vmask[4 * (j & 3u)] = ok;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tile_full[j & 1u]);
+            }
+            issued += n_tiles;
+            cp_async_wait<0>();
+            __syncwarp();
+        }
+    } else {
+        // ======== products, issued by one thread
+        constexpr uint32_t kIdS = tc_idesc(kTileKeys, false), kIdO = tc_idesc(D, true);
+        const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + 2 * G::kOperand;
+        uint32_t piece = 0;
+        while (walk.next(a, p)) {
+            const int32_t n_tiles = max(0, p.in1 - p.in0);
+            if (n_tiles == 0) continue;
+            wait(q_full, piece++);
+            tc_fence_after();
+            const uint32_t j0 = j;
+            auto qk = [&](uint32_t t) {
+                wait(&k_full[t & 1u], t >> 1);
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+                        tc_mma(tmem + kColS + (t & 1u) * kTileKeys, tmem + kColQ + 8 * s,
+                               tc_desc(k_tile + (t & 1u) * G::kOperand + (s >> 2) * (kTileKeys * 128) + (s & 3) * 32, 16, 1024), kIdS, s != 0);
+                    tc_commit(&s_full[t & 1u]);
+                    tc_commit(&k_free[t & 1u]);
+                }
+                __syncwarp();
+            };
+            qk(j0);
+            for (int32_t i = 0; i < n_tiles; ++i, ++j) {
+                if (i + 1 < n_tiles) qk(j + 1);
+                wait(&p_full[j & 1u], j >> 1);
+                wait(&v_full[j & 1u], j >> 1);
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int s = 0; s < kTileKeys / 16; ++s)
+                        tc_mma(tmem + kColO, tmem + kColS + (j & 1u) * kTileKeys + 8 * s,
+                               tc_desc(v_tile + (j & 1u) * G::kOperand + s * 2048, kTileKeys * 128, 1024), kIdO, i != 0 || s != 0);
+                    tc_commit(&v_free[j & 1u]);
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    pdl_launch_dependents();
+}
+
+// One (split item, row) a CTA, a pair of dims a thread: out = sum w_i o_i / sum w_i,
+// w_i = l_i 2^(m_i - max).
+template <int D>
+__global__ void __launch_bounds__(D / 2) attend_tile_join_kernel(const __grid_constant__ AttendArgs a) {
+    pdl_wait();
+    const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + blockIdx.x;
+    const uint32_t parts = min(desc->parts, kAttendMaxCtas), r = blockIdx.y;
+    if (parts == 0 || r >= desc->rows) return;
+    auto part = [&](uint32_t i) { return tile_part<D>(a, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u); };
+    float top = -__builtin_huge_valf();
+    for (uint32_t i = 0; i < parts; ++i) top = fmaxf(top, reinterpret_cast<const float *>(part(i))[r]);
+    const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
+    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < parts; ++i) {
+        const float *f = reinterpret_cast<const float *>(part(i));
+        const float w = f[kTileRows + r] * exp2_approx(f[r] - ref);
+        const float2 x = __half22float2(reinterpret_cast<const __half2 *>(part(i) + 8 * kTileRows)[(r * D) / 2 + threadIdx.x]);
+        sum += w;
+        if (w != 0.0f) {
+            o0 += w * x.x;
+            o1 += w * x.y;
+        }
+    }
+    const uint32_t rr = desc->first + r, tok = rr / a.group;
+    uint8_t *op = const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
+                  (static_cast<uint64_t>(desc->head) * a.group + rr % a.group) * a.out.nb_head;
+    store16(op + 2 * threadIdx.x * a.out.nb_dim, sum == 0.0f ? 0.0f : o0 / sum, a.out.bf16);
+    store16(op + (2 * threadIdx.x + 1) * a.out.nb_dim, sum == 0.0f ? 0.0f : o1 / sum, a.out.bf16);
+}
+
+}  // namespace kvm

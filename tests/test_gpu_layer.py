@@ -343,6 +343,26 @@ def test_attend_prompt_types(kvm_lib, kinds, D):
     w.check(q, [0, 200, 270], True, max_new=200)
 
 
+@pytest.mark.parametrize("D, group, news, lens", [(64, 8, [500, 410, 300], [700, 410, 900]), (256, 6, [260, 17], [5000, 3001])])
+def test_attend_prompt_items_of_every_cut(kvm_lib, D, group, news, lens):
+    """Several items a CTA, and items that several CTAs share."""
+    import torch
+    w = Window(kvm_lib, torch, D, ("q4_0", "q4_0"), 4, D, 32, lens)
+    start = np.concatenate([[0], np.cumsum(news)])
+    q = queries(torch, w.rng, int(start[-1]), 4 * group, D, "bf16")
+    got = w.run(q, start, True, max_new=max(news))
+    rows = np.unique(np.concatenate([[0, 1, start[1] - 1, start[1], start[-1] - 1], w.rng.integers(0, start[-1], 40)]))
+    for r in rows:                        # each row as a request of its own that sees what it saw
+        s = int(np.searchsorted(start, r, side="right")) - 1
+        seen = lens[s] - news[s] + int(r - start[s]) + 1
+        want, spread, peak = ref.attend(q[r:r + 1].float().cpu().numpy(), w.raw[0], w.raw[1], w.kinds, 4, 32, w.slots,
+                                        w.table[s:s + 1], [0, 1], [seen], D ** -0.5, True, np.zeros((1, 4 * group, D)))
+        check_attend(got[r:r + 1].float().cpu().numpy(), want, spread, peak, q[r:r + 1].float().cpu().numpy(),
+                     ref.row_values(w.raw[0], "q4_0"), D ** -0.5, seen, True)
+    for _ in range(3):
+        assert torch.equal(w.run(q, start, True, max_new=max(news)), got)
+
+
 def test_attend_long_window(kvm_lib):
     """Many splits of one window, and the same bits on every run."""
     import torch
