@@ -111,6 +111,9 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     a.group = q->n_head / c->n_head_kv;
     a.block_tokens = c->block_tokens;
     a.n_slots = c->n_slots;
+    a.block_shift = 32;
+    for (uint32_t s = 0; s < 32; ++s)
+        if (c->block_tokens == 1u << s) a.block_shift = s;
     a.scale_log2 = b->scale * 1.4426950408889634f;
     a.causal = (b->flags & KVM_ATTEND_CAUSAL) ? 1u : 0u;
     a.q = rows_of(q);

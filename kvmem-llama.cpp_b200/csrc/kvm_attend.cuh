@@ -33,6 +33,7 @@ struct AttendArgs {
     const int32_t *q_start;    // [n_seq + 1]
     const int32_t *kv_len;     // [n_seq]
     uint32_t n_seq, n_rows, n_head_kv, group, block_tokens, n_slots;
+    uint32_t block_shift;      // log2(block_tokens), 32 when that is no power of two
     float scale_log2;          // scale * log2(e)
     uint32_t causal;
     AttendRows q, out;
@@ -79,6 +80,11 @@ __host__ __device__ __forceinline__ int32_t attend_limit(const AttendArgs &a, co
                                                        static_cast<int64_t>(0x7fffff00)))));
 }
 
+// Block of a key.
+__device__ __forceinline__ uint32_t attend_block(const AttendArgs &a, uint32_t key) {
+    return a.block_shift < 32u ? key >> a.block_shift : key / a.block_tokens;
+}
+
 __device__ __forceinline__ float load16(const uint8_t *p, int32_t bf16) {
     const uint16_t u = *reinterpret_cast<const uint16_t *>(p);
     return bf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(__ushort_as_half(u));
@@ -122,6 +128,20 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Bounded wait on an mbarrier phase for the short waits of a pipeline: polls
+// without a suspend hint, and looks at the clock only once in a while.
+__device__ __forceinline__ bool mbar_wait_near(uint64_t *bar, uint32_t parity) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023u) == 1023u) {
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > kWaitLimitNs) return false;
+        }
+    }
 }
 
 // ------------------------------------------------------- split bookkeeping --

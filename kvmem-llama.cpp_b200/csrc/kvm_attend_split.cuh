@@ -418,7 +418,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             const uint32_t key0 = kstart + (sub + i * nsub) * kAttendStep;
             if (a.tma) {                      // all 16 keys lie in one block
                 if (lane == 0) {
-                    const uint32_t blk = key0 / a.block_tokens;
+                    const uint32_t blk = attend_block(a, key0);
                     const int32_t slot = trow[blk];
                     const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots;
                     const uint32_t left = static_cast<uint32_t>(kend) - key0;
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             const uint32_t key = key0 + (lane & 15);
             int32_t cell = -1;
             if (key < static_cast<uint32_t>(kend)) {
-                const uint32_t blk = key / a.block_tokens;
+                const uint32_t blk = attend_block(a, key);
                 const int32_t slot = trow[blk];
                 if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
                     cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         for (int i = 0; i < n_steps; ++i) {
             const uint32_t at = (issued + i) % NS;
             if (a.tma) {
-                if (!lost && !mbar_wait_bounded(&bars[at], ((issued + i) / NS) & 1u)) lost = true;
+                if (!lost && !mbar_wait_near(&bars[at], ((issued + i) / NS) & 1u)) lost = true;
             } else {
                 cp_async_wait<NS - 2>();
             }
@@ -816,64 +816,115 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
     pdl_launch_dependents();
 }
 
-// One (split segment, head, row) a CTA: the parts of a segment that starts in
-// CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...  The parts are spread
-// over groups of D / 4 threads, four dims a thread, and added in a fixed order.
+// The rows of the split segments, listed by every CTA of a join: the first row
+// of each segment in the order of the CTAs they start in.
 constexpr int kJoinThreads = 512;
+struct JoinList {
+    uint32_t upto[kAttendMaxCtas];       // rows up to and with CTA c's segment
+    uint32_t sums[kJoinThreads / 32], total;
+};
+
+__device__ __forceinline__ void join_list(const AttendArgs &a, uint32_t ctas, uint32_t heads, JoinList &list) {
+    const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < ctas; base += kJoinThreads) {
+        const uint32_t c = base + threadIdx.x;
+        uint32_t x = c < ctas && desc[c].parts ? desc[c].rows * heads : 0u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) list.sums[warp] = x;
+        __syncthreads();
+        uint32_t all = 0;
+        for (int w = 0; w < kJoinThreads / 32; ++w) {
+            if (w < warp) x += list.sums[w];
+            all += list.sums[w];
+        }
+        if (c < ctas) list.upto[c] = before + x;
+        before += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) list.total = before;
+    __syncthreads();
+}
+
+// CTA whose segment holds row x of the list, and the row in it.
+__device__ __forceinline__ uint32_t join_find(const JoinList &list, uint32_t ctas, uint32_t x, uint32_t *row) {
+    uint32_t c = 0;
+    for (uint32_t step = 512; step; step >>= 1)
+        if (c + step <= ctas && list.upto[c + step - 1] <= x) c += step;
+    *row = x - (c ? list.upto[c - 1] : 0u);
+    return c;
+}
+
+// One (head, row) of a split segment at a time: the parts of a segment that
+// starts in CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...  They are
+// spread over groups of D / 4 threads, four dims a thread, and added in a fixed
+// order.
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a, uint32_t ctas) {
     constexpr int R = 8 * NT, G = kJoinThreads / (D / 4);
     __shared__ float weight[kAttendMaxCtas], s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
     __shared__ float4 s_acc[G][D / 4];
-    pdl_wait();
-    const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + blockIdx.x;
-    const uint32_t parts = min(desc->parts, kAttendMaxCtas), hs = blockIdx.y / R, r = blockIdx.y % R;
-    if (parts == 0 || r >= desc->rows) return;
+    __shared__ JoinList list;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    auto part = [&](uint32_t i) { return attend_part<D, NT>(a, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u, hs); };
-    float top = -__builtin_huge_valf();
-    for (uint32_t i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, weight[i] = part(i)[r]);
+    pdl_wait();
+    join_list(a, ctas, a.heads_cta, list);
+    for (uint32_t at = blockIdx.x; at < list.total; at += gridDim.x) {
+        uint32_t hr;
+        const uint32_t c = join_find(list, ctas, at, &hr);
+        const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + c;
+        const uint32_t parts = min(desc->parts, ctas), hs = hr / desc->rows, r = hr - hs * desc->rows;
+        auto part = [&](uint32_t i) { return attend_part<D, NT>(a, i ? 2u * (c + i) : 2u * c + 1u, hs); };
+        float top = -__builtin_huge_valf();
+        for (uint32_t i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, weight[i] = part(i)[r]);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
-    const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-    float sum = 0.0f;
-    for (uint32_t i = tid; i < parts; i += kJoinThreads) {
-        const float f = exp2_approx(weight[i] - ref);
-        weight[i] = f;
-        sum += f * part(i)[R + r];
-    }
+        for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
+        const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
+        float sum = 0.0f;
+        for (uint32_t i = tid; i < parts; i += kJoinThreads) {
+            const float f = exp2_approx(weight[i] - ref);
+            weight[i] = f;
+            sum += f * part(i)[R + r];
+        }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    const int grp = tid / (D / 4), d = tid % (D / 4);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        const int grp = tid / (D / 4), d = tid % (D / 4);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (uint32_t i = grp; i < parts; i += G) {
-        const float f = weight[i];
-        // rows start at 2 R floats behind a multiple of 16 bytes, D floats apart
-        const float4 x = *reinterpret_cast<const float4 *>(part(i) + 2 * R + r * D + 4 * d);
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
+        for (uint32_t i = grp; i < parts; i += G) {
+            const float f = weight[i];
+            // rows start at 2 R floats behind a multiple of 16 bytes, D floats apart
+            const float4 x = *reinterpret_cast<const float4 *>(part(i) + 2 * R + r * D + 4 * d);
+            acc.x += f * x.x;
+            acc.y += f * x.y;
+            acc.z += f * x.z;
+            acc.w += f * x.w;
+        }
+        s_acc[grp][d] = acc;
+        __syncthreads();
+        if (tid < D) {
+            float o = 0.0f, l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < G; ++k) o += reinterpret_cast<const float *>(s_acc[k])[tid];
+#pragma unroll
+            for (int w = 0; w < kJoinThreads / 32; ++w) l += s_sum[w];
+            const uint32_t rr = desc->first + r, tok = rr / a.group;
+            store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
+                        (static_cast<uint64_t>(desc->head + hs) * a.group + rr % a.group) * a.out.nb_head + tid * a.out.nb_dim,
+                    l == 0.0f ? 0.0f : o / l, a.out.bf16);
+        }
+        __syncthreads();
     }
-    s_acc[grp][d] = acc;
-    __syncthreads();
-    if (tid >= D) return;
-    float o = 0.0f, l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < G; ++k) o += reinterpret_cast<const float *>(s_acc[k])[tid];
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) l += s_sum[w];
-    const uint32_t rr = desc->first + r, tok = rr / a.group;
-    store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
-                (static_cast<uint64_t>(desc->head + hs) * a.group + rr % a.group) * a.out.nb_head + tid * a.out.nb_dim,
-            l == 0.0f ? 0.0f : o / l, a.out.bf16);
 }
 
 }  // namespace kvm

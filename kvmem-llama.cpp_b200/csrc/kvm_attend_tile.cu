@@ -19,7 +19,7 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
     attend_tile_kernel<D, KT, VT><<<grid, kTileThreads, G::kSmem, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_after_prev(attend_tile_join_kernel<D>, dim3(grid, kTileRows), dim3(D / 2), 0, st, a);
+    return launch_after_prev(attend_tile_join_kernel<D>, dim3(std::min<uint32_t>(2u * num_sms(), grid * kTileRows)), dim3(kJoinThreads), 0, st, a, grid);
 }
 
 }  // namespace

@@ -15,9 +15,11 @@
 // rarely; P carries a factor 2^7 that cancels in the quotient, which keeps it
 // below F16's top and its bits down to 2^-31 of the row's largest weight.
 //
-// Roles (13 warps, one CTA an SM): warps 0-3 own the 128 rows (Q into TMEM,
-// softmax, epilogue), warps 4-7 turn raw K rows into an operand tile, warps 8-11
-// raw V rows, warp 12 issues the products.  Everything is double-buffered on
+// Roles (17 warps, one CTA an SM): warps 0-7 own the 128 rows (Q into TMEM,
+// softmax, epilogue), two threads a row with half the columns each; warps 8-11
+// turn raw K rows into an operand tile, warps 12-15 raw V rows, warp 16 issues
+// the products.  (One thread a row left a single softmax warp on each scheduler,
+// whose latencies alone took 2250 cycles a tile.)  Everything is double-buffered on
 // mbarriers: QK of tile j + 1 is issued before PV of tile j, so that the softmax
 // of one tile runs under the products of the other.  With D = 256: S 2 x 64,
 // O 256 and Q 128 columns are all of TMEM; Q there rather than in shared memory
@@ -40,7 +42,7 @@
 
 namespace kvm {
 
-constexpr int kTileRows = 128, kTileKeys = 64, kTileThreads = 13 * 32;
+constexpr int kTileRows = 128, kTileKeys = 64, kTileThreads = 17 * 32;
 
 template <int D, int KT, int VT>
 struct TileGeom {
@@ -48,7 +50,7 @@ struct TileGeom {
     using V = Slice<VT, D>;
     static constexpr int kOperand = kTileKeys * D * 2;             // one K or V tile
     static constexpr int kRawK = kAttendStep * K::kStride, kRawV = kAttendStep * V::kStride;   // a warp's 16 keys
-    static constexpr int kRoom = 220 * 1024 - 4 * kOperand;
+    static constexpr int kRoom = 218 * 1024 - 4 * kOperand;
     static constexpr int kFit = kRoom / (4 * (kRawK + kRawV));
     static constexpr int kStages = kFit > 6 ? 6 : kFit < 1 ? 1 : kFit;
     static constexpr int kRaw = 4 * kOperand;                      // offset of the raw rings
@@ -80,15 +82,19 @@ __device__ __forceinline__ void tc_ld32(uint32_t (&r)[32], uint32_t addr) {
           "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
         ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -233,6 +239,14 @@ struct TileWalk {
     }
 };
 
+// A warp's walk in shared memory: its state is needed once a piece and would
+// otherwise hold forty registers through the inner loops.
+struct WarpWalk {
+    TileWalk walk;
+    TilePiece piece;
+    uint32_t more;
+};
+
 // A piece's results in the workspace: maxima, sums, then rows of D halves.
 template <int D>
 __host__ __device__ constexpr uint32_t tile_part_bytes() { return kTileRows * (8u + 2u * D); }
@@ -258,52 +272,63 @@ __host__ __device__ constexpr int tile_order(int i) {
     return Slice<T, 64>::kNibble ? (i & 4) | (i & 1) << 1 | (i & 2) >> 1 : i;
 }
 
-// Writes 16 keys' slices as F16 values into the operand tile.  `raw` is the
-// warp's 16 rows, `key0` its first row of the tile's 64, `ok` its visible keys
-// (the others become zeros).  V values that are not finite become zeros too and
-// set *odd.  An eighth of a warp takes eight keys' same 16-byte chunk, so reads
-// and swizzled stores are free of bank conflicts.
+// Drops from a warp's 16 raw rows what must not reach a product: hidden keys (not
+// in `ok`) become zeros, and with IS_V blocks or values that are not finite.
 template <int T, int D, bool IS_V>
-__device__ __forceinline__ void tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, uint32_t ok, int lane, bool *odd) {
+__device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
+    using S = Slice<T, D>;
+    {
+        for (int x = lane; x < 16 * (S::kBytes / 4); x += 32)
+            if (!((ok >> (x & 15)) & 1u)) *reinterpret_cast<uint32_t *>(raw + (x & 15) * S::kStride + (x >> 4) * 4) = 0u;
+    }
+    __syncwarp();
+    if constexpr (IS_V) {
+        constexpr int kStep = T == KVM_TYPE_F16 ? 2 : S::kBlock;      // halves to look at: every value, or the scales
+        for (int x = lane; x < 16 * (S::kBytes / kStep); x += 32) {
+            uint16_t *p = reinterpret_cast<uint16_t *>(raw + (x & 15) * S::kStride + (x >> 4) * kStep);
+            if ((*p & 0x7c00u) == 0x7c00u) *p = 0;
+        }
+        __syncwarp();
+    }
+    fence_proxy_async_smem();       // before the ring's next load lands here
+}
+
+// Writes 16 keys' slices as F16 values into the operand tile; `raw` is the warp's
+// 16 rows, `key0` its first row of the tile's 64.  An eighth of a warp takes eight
+// keys' same 16-byte chunk, so reads and swizzled stores are free of bank
+// conflicts.  Returns whether a scale (F16: a value) of this lane is not finite.
+template <int T, int D>
+__device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
+    uint32_t top = 0;              // largest magnitude bits of the scales
     using S = Slice<T, D>;
     const int k8 = lane & 7, quad = lane >> 3;
     auto put = [&](int key, int dim8, uint4 v) {       // dims 8 dim8 .. 8 dim8 + 7 of a key
         const int row = key0 + key;
         *reinterpret_cast<uint4 *>(tile + (dim8 >> 3) * (kTileKeys * 128) + row * 128 + (((dim8 & 7) ^ (row & 7)) << 4)) = v;
     };
-    auto scale_at = [&](const uint8_t *p, int key) -> uint32_t {
-        uint32_t d = lds16(p);
-        if (IS_V && (d & 0x7c00u) == 0x7c00u && ((ok >> key) & 1u)) *odd = true;
-        if (!((ok >> key) & 1u) || (IS_V && (d & 0x7c00u) == 0x7c00u)) d = 0;
-        return d * 0x10001u;
+    auto scale_at = [&](const uint8_t *p) -> uint32_t {
+        const uint32_t d = lds16(p);
+        top = max(top, d & 0x7fffu);
+        return __byte_perm(d, 0u, 0x1010);
     };
-#pragma unroll 1
+#pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int key = 8 * half + k8;
         const uint8_t *row = raw + key * S::kStride;
         if constexpr (T == KVM_TYPE_F16) {
-            const bool see = (ok >> key) & 1u;
 #pragma unroll 4
             for (int c = quad; c < D / 8; c += 4) {
-                uint4 v = *reinterpret_cast<const uint4 *>(row + 16 * c);
-                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const uint4 v = *reinterpret_cast<const uint4 *>(row + 16 * c);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (IS_V) {
-                        const bool lo = (w[i] & 0x7c00u) == 0x7c00u, hi = (w[i] & 0x7c000000u) == 0x7c000000u;
-                        if (see && (lo || hi)) *odd = true;
-                        if (lo) w[i] &= 0xffff0000u;
-                        if (hi) w[i] &= 0x0000ffffu;
-                    }
-                    if (!see) w[i] = 0;
-                }
-                put(key, c, make_uint4(w[0], w[1], w[2], w[3]));
+                for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                put(key, c, v);
             }
         } else if constexpr (T == KVM_TYPE_Q8_0) {
 #pragma unroll 4
             for (int b = 0; b < D / 32; ++b) {
                 const uint8_t *p = row + (b >> 1) * 68;
-                const uint32_t d = scale_at(p + (b & 1) * 34, key);
+                const uint32_t d = scale_at(p + (b & 1) * 34);
                 uint32_t x[2];
                 if (b & 1) {
                     x[0] = lds32(p + 36 + 8 * quad);
@@ -327,28 +352,35 @@ __device__ __forceinline__ void tile_dequant(const uint8_t *raw, uint8_t *tile, 
             const int b = quad >> 1, h = quad & 1;
             constexpr int kPair = 2 * S::kBlock, kCodes = S::kBlock - 16;
             const uint32_t align = b ? 0x3210u : 0x5432u;
+            // all reads first: nothing tells the compiler that the stores below do not
+            // change them
+            uint32_t w[D / 64][3], scale[D / 64], five[D / 64][2];
 #pragma unroll
             for (int pr = 0; pr < D / 64; ++pr) {
                 const uint8_t *p = row + pr * kPair;
-                const uint32_t d = scale_at(p + b * S::kBlock, key);
                 // q4_0: the codes start at byte 2 or 20, q5_0: 6 or 28
                 const uint8_t *q = p + (b ? S::kBlock + kCodes : kCodes - 2) + 8 * h;
-                const uint32_t w0 = lds32(q), w1 = lds32(q + 4), w2 = lds32(q + 8);
-                const uint32_t x[2] = {__byte_perm(w0, w1, align), __byte_perm(w1, w2, align)};
-                uint32_t lo[4], hi[4];
-                uint32_t fl = 0, fh = 0;
+                scale[pr] = scale_at(p + b * S::kBlock);
+                w[pr][0] = lds32(q);
+                w[pr][1] = lds32(q + 4);
+                w[pr][2] = lds32(q + 8);
                 if constexpr (T == KVM_TYPE_Q5_0) {
-                    const uint32_t f = lds16(p + b * S::kBlock + 2) >> (8 * h), e = lds16(p + b * S::kBlock + 4) >> (8 * h);
-                    fl = f;
-                    fh = e;
+                    five[pr][0] = lds16(p + b * S::kBlock + 2) >> (8 * h);
+                    five[pr][1] = lds16(p + b * S::kBlock + 4) >> (8 * h);
                 }
+            }
+#pragma unroll
+            for (int pr = 0; pr < D / 64; ++pr) {
+                const uint32_t d = scale[pr];
+                const uint32_t x[2] = {__byte_perm(w[pr][0], w[pr][1], align), __byte_perm(w[pr][1], w[pr][2], align)};
+                uint32_t lo[4], hi[4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t y = x[i] >> 8;
                     uint32_t l0 = (x[i] & 0x000f000fu) | 0x64006400u, l1 = (y & 0x000f000fu) | 0x64006400u;
                     uint32_t h0 = (x[i] & 0x00f000f0u) | 0x64006400u, h1 = (y & 0x00f000f0u) | 0x64006400u;
                     if constexpr (T == KVM_TYPE_Q5_0) {
-                        const uint32_t a = fl >> (4 * i), c = fh >> (4 * i);
+                        const uint32_t a = five[pr][0] >> (4 * i), c = five[pr][1] >> (4 * i);
                         l0 |= ((a & 5u) * 0x00040010u) & 0x00100010u;
                         l1 |= ((a & 10u) * 0x00020008u) & 0x00100010u;
                         h0 |= ((c & 5u) * 0x00400100u) & 0x01000100u;
@@ -371,6 +403,7 @@ __device__ __forceinline__ void tile_dequant(const uint8_t *raw, uint8_t *tile, 
             }
         }
     }
+    return top >= 0x7c00u;
 }
 
 // ------------------------------------------------------------------ kernel --
@@ -389,17 +422,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
     uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][4 warps]
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
     __shared__ uint32_t s_seq, s_tmem, s_odd;
+    __shared__ float s_swap[2][2 * kTileRows];
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 4);
             mbar_init(&v_full[i], 4);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 8);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
         }
-        mbar_init(q_full, 4);
+        mbar_init(q_full, 8);
         for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
         s_odd = 0;
         fence_mbar_init();
@@ -452,7 +486,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         carry += all;
         if (carry > u0) break;
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -460,27 +494,42 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    TileWalk walk;
-    walk.pos = u0;
-    walk.u1 = u1;
-    walk.share = share;
-    walk.seek(a, s_seq, static_cast<int64_t>(s_off));
-    TilePiece p;
+    __shared__ WarpWalk s_walk[kTileThreads / 32];
+    WarpWalk &mywalk = s_walk[warp];
+    const TilePiece &p = mywalk.piece;
+    if (lane == 0) {
+        mywalk.walk.pos = u0;
+        mywalk.walk.u1 = u1;
+        mywalk.walk.share = share;
+        mywalk.walk.seek(a, s_seq, static_cast<int64_t>(s_off));
+    }
+    auto next_piece = [&]() -> bool {
+        __syncwarp();                          // every lane is done with the last piece
+        if (lane == 0) mywalk.more = mywalk.walk.next(a, mywalk.piece) ? 1u : 0u;
+        __syncwarp();
+        return mywalk.more != 0u;
+    };
     bool lost = false;                         // a bounded wait ran out: go on without waiting
     auto wait = [&](uint64_t *bar, uint32_t phase) {
-        if (!lost && !mbar_wait_bounded(bar, phase & 1u)) lost = true;
+        if (!lost && !mbar_wait_near(bar, phase & 1u)) lost = true;
     };
     uint32_t j = 0;                            // running key tile of the CTA: stage j & 1, phase j >> 1
 
-    // Registers: 13 warps launch with 128 each; the rows' warps take 48 more from
-    // the dequantizing ones (4 * 32 * (176 + 104 + 104) + 32 * 128 = 416 * 128).
-    if (warp < 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-        // ======== rows: Q into TMEM, softmax, epilogue
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) * 32u << 16);
-        const int row = tid;
+    if (warp < 8) {
+        // ======== rows: Q into TMEM, softmax, epilogue; thread (row, wg) has columns 32 wg .. of S
+        // and dims D / 2 wg .. of Q and O
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) * 32u << 16);
+        const int row = tid & 127, wg = tid >> 7;
+        uint32_t swaps = 0;
+        // the other thread's value of the row's pair
+        auto swap = [&](float x) -> float {
+            float *at = s_swap[swaps++ & 1u];
+            at[wg * kTileRows + row] = x;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+            return at[(wg ^ 1) * kTileRows + row];
+        };
         bool described = false;
-        while (walk.next(a, p)) {
+        while (next_piece()) {
             const bool in = static_cast<uint32_t>(row) < p.rows;
             const uint32_t rr = p.first + (in ? row : 0), tok = rr / a.group;
             const uint64_t at_tok = static_cast<uint64_t>(p.q.row0) + tok, at_head = static_cast<uint64_t>(p.head) * a.group + rr % a.group;
@@ -489,7 +538,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             // the row's largest element to [2^14, 2^15)
             float top = 0.0f;
 #pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
+            for (int c = wg * (D / 16); c < (wg + 1) * (D / 16); ++c) {
                 uint32_t u[4];
                 if (a.q_vec) {
                     const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * c);
@@ -507,21 +556,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
                 }
             }
+            top = fmaxf(top, swap(top));
             const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
             // the sum of D products must stay in F32: a top of 2^14 leaves 2^98 for K
             const int up = (top > 0.0f && e < 128) ? max(-126, min(126, 14 - e)) : 0;
             const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
             const float mul = sign * __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-            const float fac = fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            // not 0: a hidden key's -inf has to stay -inf
+            const float fac = fmaxf(fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
             // a piece without key tiles issues no products and leaves Q alone
 #pragma unroll 1
-            for (int c0 = 0; c0 < (p.in0 < p.in1 ? D / 64 : 0); ++c0) {       // 64 dims = 32 columns at a time
-                uint32_t w[32];
+            for (int c0 = wg * (D / 64); c0 < (p.in0 < p.in1 ? (wg + 1) * (D / 64) : 0); ++c0) {       // 32 dims = 16 columns at a time
+                uint32_t w[16];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     float x[8];
                     if (a.q_vec) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * (8 * c0 + c));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * (4 * c0 + c));
                         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -530,13 +581,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = load16(qp + (64 * c0 + 8 * c + i) * a.q.nb_dim, a.q.bf16);
+                        for (int i = 0; i < 8; ++i) x[i] = load16(qp + (32 * c0 + 8 * c + i) * a.q.nb_dim, a.q.bf16);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         w[4 * c + i] = in ? pack_half2(x[tile_order<KT>(2 * i)] * mul, x[tile_order<KT>(2 * i + 1)] * mul) : 0u;
                 }
-                tc_st32(lanes + kColQ + 32 * c0, w);
+                tc_st16(lanes + kColQ + 16 * c0, w);
             }
             tc_wait_st();
             tc_fence_before();
@@ -545,31 +596,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
 
             float m = kNegInf, l = 0.0f;
             const uint32_t j0 = j;
-            for (int32_t n = p.in0; n < p.in1; ++n, ++j) {
+            const int32_t in1 = p.in1, kfull = p.kfull;
+#pragma unroll 1
+            for (int32_t n = p.in0; n < in1; ++n, ++j) {
                 const uint32_t st = j & 1u;
                 wait(&s_full[st], j >> 1);
                 // valid[] of this tile: written before k_full, which the products behind
                 // s_full waited for, and not again before the tile after next's products.
                 // (k_full itself may be a phase ahead here and must not be waited on.)
                 tc_fence_after();
-                uint32_t s0[32], s1[32];
-                tc_ld32(s0, lanes + kColS + st * kTileKeys);
-                tc_ld32(s1, lanes + kColS + st * kTileKeys + 32);
+                uint32_t s[32];
+                tc_ld32(s, lanes + kColS + st * kTileKeys + 32 * wg);
                 tc_wait_ld();
-                const uint4 ok4 = *reinterpret_cast<const uint4 *>(valid + 4 * (j & 3u));
-                const uint32_t ok0 = ok4.x | ok4.y << 16, ok1 = ok4.z | ok4.w << 16;
-                const int32_t key0 = n * kTileKeys;
-                if (key0 + kTileKeys > p.kfull || (ok0 & ok1) != 0xffffffffu) {
+                const uint2 ok2 = *reinterpret_cast<const uint2 *>(valid + 4 * (j & 3u) + 2 * wg);
+                const uint32_t ok = ok2.x | ok2.y << 16;
+                const int32_t key0 = n * kTileKeys + 32 * wg;
+                if (key0 + 32 > kfull || ok != 0xffffffffu) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (key0 + i >= lim || !((ok0 >> i) & 1u)) s0[i] = __float_as_uint(kNegInf);
-                        if (key0 + 32 + i >= lim || !((ok1 >> i) & 1u)) s1[i] = __float_as_uint(kNegInf);
-                    }
+                    for (int i = 0; i < 32; ++i)
+                        if (key0 + i >= lim || !((ok >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
                 }
                 float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) t4[i & 3] = fmaxf(t4[i & 3], fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
-                const float x = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                for (int i = 0; i < 32; i += 2)
+                    t4[(i >> 1) & 3] = fmaxf(fmaxf(t4[(i >> 1) & 3], __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
+                float x = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                x = fmaxf(x, swap(x));
                 const float mt = x == kNegInf ? kNegInf : x * fac;
                 if (__any_sync(0xffffffffu, mt > m + kSlack || (m == kNegInf && mt > m))) {
                     const float mn = fmaxf(m, mt);
@@ -578,13 +630,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                         wait(&v_free[(j - 1) & 1u], (j - 1) >> 1);
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tc_ld32(o, lanes + kColO + 32 * c);
+                        for (int c = wg * (D / 32); c < (wg + 1) * (D / 32); ++c) {
+                            uint32_t o[16];
+                            tc_ld16(o, lanes + kColO + 16 * c);
                             tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(m == mn ? __uint_as_float(o[i]) : __uint_as_float(o[i]) * f);
-                            tc_st32(lanes + kColO + 32 * c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(m == mn ? __uint_as_float(o[i]) : __uint_as_float(o[i]) * f);
+                            tc_st16(lanes + kColO + 16 * c, o);
                         }
                         tc_wait_st();
                     }
@@ -592,19 +644,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     m = mn;
                 }
                 const float ref = m == kNegInf ? 0.0f : kWeightLog - m;
-                uint32_t w[32];
-                float a0 = 0.0f, a1 = 0.0f;
+                const float2 fac2 = make_float2(fac, fac), ref2 = make_float2(ref, ref);
+                float2 sum2 = make_float2(0.0f, 0.0f);
+                uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint32_t *s = i < 16 ? s0 + 2 * i : s1 + 2 * (i - 16);
-                    const float p0 = exp2_approx(fmaf(__uint_as_float(s[0]), fac, ref));
-                    const float p1 = exp2_approx(fmaf(__uint_as_float(s[1]), fac, ref));
-                    a0 += p0;
-                    a1 += p1;
-                    w[i] = pack_half2(p0, p1);
+                for (int i = 0; i < 16; ++i) {
+                    const float2 y = f2_fma_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, ref2);
+                    const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                    sum2 = f2_add_rn(sum2, e);
+                    w[i] = pack_half2(e.x, e.y);
                 }
-                l += a0 + a1;
-                tc_st32(lanes + kColS + st * kTileKeys, w);
+                tc_st16(lanes + kColS + st * kTileKeys + 16 * wg, w);
+                l += sum2.x + sum2.y;
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -617,17 +668,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 tc_fence_after();
             }
             if (lost) l = __int_as_float(0x7fc00000);
+            l += swap(l);
             const bool whole = p.starts && p.ends;
             const bool odd = *reinterpret_cast<volatile uint32_t *>(&s_odd) != 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint8_t *part = whole ? nullptr : tile_part<D>(a, 2u * blockIdx.x + (p.starts ? 1u : 0u));
             uint8_t *op = const_cast<uint8_t *>(a.out.p) + at_tok * a.out.nb_tok + at_head * a.out.nb_head;
-            if (part) {
+            if (part && wg == 0) {
                 reinterpret_cast<float *>(part)[row] = m;
                 reinterpret_cast<float *>(part)[kTileRows + row] = l;
             }
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {
                 uint32_t o[32];
                 if (any) {
                     tc_ld32(o, lanes + kColO + 32 * c);
@@ -693,17 +745,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             described = described || (p.starts && !p.ends);
         }
         if (tid == 0 && !described) desc->parts = 0;
-    } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        // ======== K (warps 4-7) and V (warps 8-11): raw rows to operand tiles
-        const bool is_v = warp >= 8;
+    } else if (warp < 16) {
+        // ======== K (warps 8-11) and V (warps 12-15): raw rows to operand tiles
+        const bool is_v = warp >= 12;
         const int w4 = warp & 3;
         const int raw_bytes = is_v ? G::kRawV : G::kRawK;
         uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kRawK : 0) + w4 * NS * raw_bytes;
-        uint64_t *full = raw_full + (warp - 4) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
+        uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
         uint32_t *vmask = valid + w4;
-        uint32_t issued = 0;
-        while (walk.next(a, p)) {
+        uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring stage of the next load, of the next tile
+        while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0);
             const int32_t *trow = a.table + p.seq * a.table_stride;
             const uint64_t slice = static_cast<uint64_t>(p.head) * (is_v ? G::V::kBytes : G::K::kBytes);
@@ -712,23 +763,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < NS; ++i) ring_ok[i] = 0;
             // every lane computes the visible keys of the warp's 16 in tile n
+            const int32_t in0 = p.in0, kend = p.kend;
+            // the table entry of load i, fetched while load i - 1 is issued
+            auto entry = [&](int32_t i) -> int32_t {
+                const int32_t key0 = (in0 + i) * kTileKeys + w4 * 16;
+                return i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
+            };
+            int32_t slot_next = a.tma ? entry(0) : -1;
             auto load = [&](int32_t i) -> uint32_t {
-                uint8_t *st = ring + ((issued + i) % NS) * raw_bytes;
-                uint64_t *bar = &full[(issued + i) % NS];
-                const uint32_t key0 = static_cast<uint32_t>((p.in0 + i) * kTileKeys + w4 * 16);
-                const int32_t left = p.kend - static_cast<int32_t>(key0);
+                uint8_t *st = ring + in_at * raw_bytes;
+                uint64_t *bar = &full[in_at];
+                if (++in_at == NS) in_at = 0;
+                const uint32_t key0 = static_cast<uint32_t>((in0 + i) * kTileKeys + w4 * 16);
+                const int32_t left = kend - static_cast<int32_t>(key0);
                 if (a.tma) {
                     uint32_t ok = 0;
-                    if (left > 0) {
-                        const uint32_t blk = key0 / a.block_tokens;
-                        const int32_t slot = trow[blk];
-                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
-                            ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
-                            if (lane == 0) {
-                                const int32_t cell = static_cast<int32_t>(slot * a.block_tokens + (key0 - blk * a.block_tokens));
-                                mbar_arrive_expect_tx(bar, raw_bytes);
-                                tma_load_2d(st, is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u), cell, bar);
-                            }
+                    const int32_t slot = slot_next;
+                    slot_next = entry(i + 1);
+                    if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
+                        ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                        if (lane == 0) {
+                            const uint32_t in_block = key0 - attend_block(a, key0) * a.block_tokens;
+                            mbar_arrive_expect_tx(bar, raw_bytes);
+                            tma_load_2d(st, is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
+                                        static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
                         }
                     }
                     if (ok == 0 && lane == 0) mbar_arrive(bar);
@@ -736,8 +794,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 }
                 const uint32_t key = key0 + (lane & 15);
                 int32_t cell = -1;
-                if (static_cast<int32_t>(key) < p.kend) {
-                    const uint32_t blk = key / a.block_tokens;
+                if (static_cast<int32_t>(key) < kend) {
+                    const uint32_t blk = attend_block(a, key);
                     const int32_t slot = trow[blk];
                     if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
                         cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
@@ -763,10 +821,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 if (i < n_tiles) ring_ok[i] = load(i);
                 cp_async_commit();
             }
-            bool odd = false;
+#pragma unroll 1
             for (int32_t i = 0; i < n_tiles; ++i, ++j) {
                 if (NS == 1) ring_ok[0] = load(i);
-                if (a.tma) wait(&full[(issued + i) % NS], (issued + i) / NS);
+                if (a.tma) wait(&full[out_at], out_phase);
                 else if (NS == 1) cp_async_commit(), cp_async_wait<0>();
                 else cp_async_wait<(NS > 1 ? NS - 2 : 0)>();
                 __syncwarp();
@@ -777,27 +835,44 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     if (i + NS - 1 < n_tiles) ring_ok[NS - 2 < 0 ? 0 : NS - 2] = load(i + NS - 1);
                     cp_async_commit();
                 }
+                uint8_t *raw = ring + out_at * raw_bytes + lead;
+                if (ok != 0xffffu) {
+                    if (is_v) tile_clean<VT, D, false>(raw, ok, lane);
+                    else tile_clean<KT, D, false>(raw, ok, lane);
+                }
                 if (j >= 2) wait(&tile_free[j & 1u], (j >> 1) - 1u);
-                const uint8_t *raw = ring + ((issued + i) % NS) * raw_bytes + lead;
+                if (++out_at == NS) {
+                    out_at = 0;
+                    out_phase ^= 1u;
+                }
                 uint8_t *tile = smem + (is_v ? 2 * G::kOperand : 0) + (j & 1u) * G::kOperand;
-                if (is_v) tile_dequant<VT, D, true>(raw, tile, w4 * 16, ok, lane, &odd);
-                else tile_dequant<KT, D, false>(raw, tile, w4 * 16, ok, lane, &odd);
-                if (is_v && odd) *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
+                if (is_v) {
+                    if (__any_sync(0xffffffffu, tile_dequant<VT, D>(raw, tile, w4 * 16, lane))) {
+                        // the epilogue adds what is not finite; the products do without it
+                        tile_clean<VT, D, true>(raw, ok, lane);
+                        tile_dequant<VT, D>(raw, tile, w4 * 16, lane);
+                        *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
+                    }
+                } else {
+                    tile_dequant<KT, D>(raw, tile, w4 * 16, lane);
+                }
                 if (!is_v && lane == 0) vmask[4 * (j & 3u)] = ok;
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&tile_full[j & 1u]);
             }
-            issued += n_tiles;
             cp_async_wait<0>();
             __syncwarp();
         }
     } else {
         // ======== products, issued by one thread
         constexpr uint32_t kIdS = tc_idesc(kTileKeys, false), kIdO = tc_idesc(D, true);
-        const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + 2 * G::kOperand;
+        // descriptors of the first tiles; the others differ in the address field, which
+        // no addition here carries out of
+        const uint64_t k_desc = tc_desc(smem_u32(smem), 16, 1024);
+        const uint64_t v_desc = tc_desc(smem_u32(smem) + 2 * G::kOperand, kTileKeys * 128, 1024);
         uint32_t piece = 0;
-        while (walk.next(a, p)) {
+        while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0);
             if (n_tiles == 0) continue;
             wait(q_full, piece++);
@@ -806,11 +881,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             auto qk = [&](uint32_t t) {
                 wait(&k_full[t & 1u], t >> 1);
                 tc_fence_after();
+                const uint64_t base = k_desc + (t & 1u) * (G::kOperand / 16);
+                const uint32_t to = tmem + kColS + (t & 1u) * kTileKeys;
                 if (lane == 0) {
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s)
-                        tc_mma(tmem + kColS + (t & 1u) * kTileKeys, tmem + kColQ + 8 * s,
-                               tc_desc(k_tile + (t & 1u) * G::kOperand + (s >> 2) * (kTileKeys * 128) + (s & 3) * 32, 16, 1024), kIdS, s != 0);
+                        tc_mma(to, tmem + kColQ + 8 * s, base + ((s >> 2) * (kTileKeys * 128) + (s & 3) * 32) / 16, kIdS, s != 0);
                     tc_commit(&s_full[t & 1u]);
                     tc_commit(&k_free[t & 1u]);
                 }
@@ -822,11 +898,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 wait(&p_full[j & 1u], j >> 1);
                 wait(&v_full[j & 1u], j >> 1);
                 tc_fence_after();
+                const uint64_t base = v_desc + (j & 1u) * (G::kOperand / 16);
+                const uint32_t from = tmem + kColS + (j & 1u) * kTileKeys;
                 if (lane == 0) {
 #pragma unroll
                     for (int s = 0; s < kTileKeys / 16; ++s)
-                        tc_mma(tmem + kColO, tmem + kColS + (j & 1u) * kTileKeys + 8 * s,
-                               tc_desc(v_tile + (j & 1u) * G::kOperand + s * 2048, kTileKeys * 128, 1024), kIdO, i != 0 || s != 0);
+                        tc_mma(tmem + kColO, from + 8 * s, base + s * (2048 / 16), kIdO, i != 0 || s != 0);
                     tc_commit(&v_free[j & 1u]);
                 }
                 __syncwarp();
@@ -834,42 +911,53 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         }
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
     pdl_launch_dependents();
 }
 
-// One (split item, row) a CTA, a pair of dims a thread: out = sum w_i o_i / sum w_i,
-// w_i = l_i 2^(m_i - max).
+// out = sum w_i o_i / sum w_i, w_i = l_i 2^(m_i - max), over the pieces of every
+// split item: a group of D / 8 threads a row, eight dims a thread.
 template <int D>
-__global__ void __launch_bounds__(D / 2) attend_tile_join_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __grid_constant__ AttendArgs a, uint32_t ctas) {
+    constexpr uint32_t kGroup = D / 8, kPer = kJoinThreads / kGroup;
+    __shared__ JoinList list;
     pdl_wait();
-    const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + blockIdx.x;
-    const uint32_t parts = min(desc->parts, kAttendMaxCtas), r = blockIdx.y;
-    if (parts == 0 || r >= desc->rows) return;
-    auto part = [&](uint32_t i) { return tile_part<D>(a, i ? 2u * (blockIdx.x + i) : 2u * blockIdx.x + 1u); };
-    float top = -__builtin_huge_valf();
-    for (uint32_t i = 0; i < parts; ++i) top = fmaxf(top, reinterpret_cast<const float *>(part(i))[r]);
-    const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = 0; i < parts; ++i) {
-        const float *f = reinterpret_cast<const float *>(part(i));
-        const float w = f[kTileRows + r] * exp2_approx(f[r] - ref);
-        const float2 x = __half22float2(reinterpret_cast<const __half2 *>(part(i) + 8 * kTileRows)[(r * D) / 2 + threadIdx.x]);
-        sum += w;
-        if (w != 0.0f) {
-            o0 += w * x.x;
-            o1 += w * x.y;
+    join_list(a, ctas, 1, list);
+    for (uint32_t x = blockIdx.x * kPer + threadIdx.x / kGroup; x < list.total; x += gridDim.x * kPer) {
+        uint32_t r;
+        const uint32_t c = join_find(list, ctas, x, &r);
+        const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + c;
+        const uint32_t parts = min(desc->parts, ctas), d8 = threadIdx.x % kGroup;
+        auto part = [&](uint32_t i) { return tile_part<D>(a, i ? 2u * (c + i) : 2u * c + 1u); };
+        float top = -__builtin_huge_valf();
+        for (uint32_t i = 0; i < parts; ++i) top = fmaxf(top, reinterpret_cast<const float *>(part(i))[r]);
+        const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
+        float sum = 0.0f, o[8] = {};
+#pragma unroll 2
+        for (uint32_t i = 0; i < parts; ++i) {
+            const float *f = reinterpret_cast<const float *>(part(i));
+            const float w = f[kTileRows + r] * exp2_approx(f[r] - ref);
+            const uint4 v = *reinterpret_cast<const uint4 *>(part(i) + 8 * kTileRows + (r * D + 8 * d8) * 2);
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            sum += w;
+            if (w != 0.0f) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&u[k]));
+                    o[2 * k] += w * y.x;
+                    o[2 * k + 1] += w * y.y;
+                }
+            }
         }
+        const uint32_t rr = desc->first + r, tok = rr / a.group;
+        uint8_t *op = const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
+                      (static_cast<uint64_t>(desc->head) * a.group + rr % a.group) * a.out.nb_head;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) store16(op + (8 * d8 + k) * a.out.nb_dim, sum == 0.0f ? 0.0f : o[k] / sum, a.out.bf16);
     }
-    const uint32_t rr = desc->first + r, tok = rr / a.group;
-    uint8_t *op = const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
-                  (static_cast<uint64_t>(desc->head) * a.group + rr % a.group) * a.out.nb_head;
-    store16(op + 2 * threadIdx.x * a.out.nb_dim, sum == 0.0f ? 0.0f : o0 / sum, a.out.bf16);
-    store16(op + (2 * threadIdx.x + 1) * a.out.nb_dim, sum == 0.0f ? 0.0f : o1 / sum, a.out.bf16);
 }
 
 }  // namespace kvm

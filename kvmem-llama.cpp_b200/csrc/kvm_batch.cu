@@ -51,14 +51,12 @@ __device__ __forceinline__ uint64_t scan64(uint64_t v, uint64_t *warp_sums, uint
 __global__ void __launch_bounds__(kMapThreads) map_batch_kernel(const __grid_constant__ kvm_batch_map m) {
     __shared__ MapSmem s;
     __shared__ uint64_t sums[kMapThreads / 32];
-    __shared__ uint32_t s_idle, s_tokens;
-    __shared__ unsigned long long s_taken;
+    __shared__ uint32_t s_idle, s_tokens, s_taken;
     const int tid = threadIdx.x;
     const uint32_t T = m.block_tokens;
     const bool lead = blockIdx.x == 0;
     if (tid == 0) {
-        s_idle = s_tokens = 0;
-        s_taken = 0;
+        s_idle = s_tokens = s_taken = 0;
         s.start[0] = 0;
     }
     __syncthreads();
@@ -86,11 +84,16 @@ __global__ void __launch_bounds__(kMapThreads) map_batch_kernel(const __grid_con
             if (lead) {
                 m.d_q_start[i + 1] = s.start[i + 1];
                 m.d_kv_len[i] = runs ? static_cast<int32_t>(past + fresh) : 0;
-                if (!runs) atomicAdd(&s_idle, 1u);
-                if (runs) {
-                    atomicAdd(&s_tokens, static_cast<uint32_t>(fresh));
-                    if (need) atomicAdd(&s_taken, static_cast<unsigned long long>(need));
-                }
+            }
+        }
+        if (lead) {           // sums of a warp first: one shared atomic a warp
+            const uint32_t idle = __popc(__ballot_sync(0xffffffffu, in && !runs));
+            const uint32_t tokens = __reduce_add_sync(0xffffffffu, runs ? static_cast<uint32_t>(fresh) : 0u);
+            const uint32_t taken = __reduce_add_sync(0xffffffffu, runs ? static_cast<uint32_t>(need) : 0u);
+            if ((tid & 31) == 0) {
+                atomicAdd(&s_idle, idle);
+                atomicAdd(&s_tokens, tokens);
+                atomicAdd(&s_taken, taken);
             }
         }
     }

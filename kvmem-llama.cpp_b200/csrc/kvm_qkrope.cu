@@ -10,12 +10,12 @@
 // are F32 and each value is rounded once, at the store.
 //
 // Bound by HBM: every value is read and written once.  A thread owns the chunk
-// pair that a rotation mixes (8 values and their partners n_rot/2 further on) of
-// several heads of one token: its 8 cos / sin pairs and 16 weights stay in
-// registers for all of them, the rotation needs no exchange, and the norm only a
-// reduction over the head's head_dim/16 neighbouring threads.  No shared memory
-// and no barrier.  A token's heads are split over more threads while the tokens
-// alone do not fill the GPU (launch below).
+// pair that a rotation mixes (8 values and their partners n_rot/2 further on), so
+// the rotation needs no exchange and the norm only a reduction over the head's
+// head_dim/16 neighbouring threads.  A CTA takes one to four tokens at a time, all
+// heads: its threads first issue the loads of up to four heads each (8 vectors in
+// flight), then form the tokens' cos / sin once for all heads, in shared memory,
+// while those loads are under way.  Weights stay in registers across the tokens.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -42,37 +42,42 @@ struct RopeArgs {
     const int32_t *pos;
     float eps;
     uint32_t head_dim, n_rot, lanes;   // lanes: threads a head, a power of two >= head_dim / 16
-    uint32_t n, splits, per_split;     // a token's heads in `splits` ranges of per_split
+    uint32_t n, tokens;                // rows; rows a CTA takes at a time
+    float inv_dim;                     // 1 / head_dim
+};
+
+// Eight values as they lie in memory (16-bit types: four words).
+template <int TYPE>
+struct Raw8 {
+    uint32_t w[TYPE == KVM_TYPE_F32 ? 8 : 4];
 };
 
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void load8(const uint8_t *p, uint64_t nb_dim, float (&x)[8]) {
-    if constexpr (VEC && TYPE == KVM_TYPE_F32) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 16);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else if constexpr (VEC) {
-        const uint4 r = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+__device__ __forceinline__ void load8(const uint8_t *p, uint64_t nb_dim, Raw8<TYPE> &r) {
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (TYPE == KVM_TYPE_F16) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                x[2 * i] = f.x;
-                x[2 * i + 1] = f.y;
-            } else {
-                x[2 * i] = __uint_as_float(w[i] << 16);
-                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
+        for (int i = 0; i < (TYPE == KVM_TYPE_F32 ? 2 : 1); ++i) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
         }
+    } else if constexpr (TYPE == KVM_TYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = *reinterpret_cast<const uint32_t *>(p + i * nb_dim);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint8_t *e = p + i * nb_dim;
-            if constexpr (TYPE == KVM_TYPE_F32) x[i] = *reinterpret_cast<const float *>(e);
-            else if constexpr (TYPE == KVM_TYPE_F16) x[i] = __half2float(*reinterpret_cast<const __half *>(e));
-            else x[i] = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(e)) << 16);
-        }
+        for (int i = 0; i < 4; ++i)
+            r.w[i] = *reinterpret_cast<const uint16_t *>(p + 2 * i * nb_dim) |
+                     static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(p + (2 * i + 1) * nb_dim)) << 16;
+    }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void widen8(const Raw8<TYPE> &r, float2 (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == KVM_TYPE_F32) x[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+        else if constexpr (TYPE == KVM_TYPE_F16) x[i] = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[i]));
+        else x[i] = make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
     }
 }
 
@@ -88,125 +93,179 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void store8(uint8_t *p, uint64_t nb_dim, const float (&x)[8]) {
+__device__ __forceinline__ void store8(uint8_t *p, uint64_t nb_dim, const float2 (&x)[4]) {
     if constexpr (VEC && TYPE == KVM_TYPE_F32) {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(p + 16) = make_float4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+        *reinterpret_cast<float4 *>(p + 16) = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
     } else if constexpr (VEC) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3]),
-                                                   pack2<TYPE>(x[4], x[5]), pack2<TYPE>(x[6], x[7]));
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<TYPE>(x[0].x, x[0].y), pack2<TYPE>(x[1].x, x[1].y),
+                                                   pack2<TYPE>(x[2].x, x[2].y), pack2<TYPE>(x[3].x, x[3].y));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint8_t *e = p + i * nb_dim;
-            if constexpr (TYPE == KVM_TYPE_F32) *reinterpret_cast<float *>(e) = x[i];
-            else *reinterpret_cast<uint16_t *>(e) = static_cast<uint16_t>(pack2<TYPE>(x[i], 0.0f) & 0xffffu);
+            const float v = i & 1 ? x[i / 2].y : x[i / 2].x;
+            if constexpr (TYPE == KVM_TYPE_F32) *reinterpret_cast<float *>(e) = v;
+            else *reinterpret_cast<uint16_t *>(e) = static_cast<uint16_t>(pack2<TYPE>(v, 0.0f) & 0xffffu);
         }
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void load_weights(const float *w, uint32_t e, float (&x)[8]) {
-    if (!w) {
+__device__ __forceinline__ void load_weights(const float *w, uint32_t e, float2 (&x)[4]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 1.0f;
-    } else if constexpr (VEC) {
-        const float4 a = *reinterpret_cast<const float4 *>(w + e), b = *reinterpret_cast<const float4 *>(w + e + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = w[e + i];
+    for (int i = 0; i < 4; ++i) {
+        if (!w) x[i] = make_float2(1.0f, 1.0f);
+        else if constexpr (VEC) x[i] = *reinterpret_cast<const float2 *>(w + e + 2 * i);
+        else x[i] = make_float2(w[e + 2 * i], w[e + 2 * i + 1]);
     }
 }
 
+// Byte offset of a head of a row.  Vector accesses come with strides below 2^32
+// (two wide multiply-adds); others take any.
+template <bool VEC>
+__device__ __forceinline__ uint64_t head_offset(uint32_t tok, uint64_t s_tok, uint32_t h, uint64_t s_head) {
+    if constexpr (VEC)
+        return static_cast<uint64_t>(tok) * static_cast<uint32_t>(s_tok) + static_cast<uint64_t>(h) * static_cast<uint32_t>(s_head);
+    else
+        return tok * s_tok + h * s_head;
+}
+
+constexpr int kRopeTokens = 4;
+// floats between two threads' 8 cos (then 8 sin) values: 16-byte reads of eight
+// neighbouring threads fall into different banks
+constexpr int kRopePitch = 12;
+
 template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
-    const uint32_t heads = a.q.heads + a.k.heads;
-    const uint64_t unit = (static_cast<uint64_t>(blockIdx.x) * kRopeThreads + threadIdx.x) / a.lanes;   // (token, head range)
-    const uint32_t p = threadIdx.x & (a.lanes - 1);
-    const uint32_t tok = static_cast<uint32_t>(unit / a.splits), part = static_cast<uint32_t>(unit - static_cast<uint64_t>(tok) * a.splits);
-    const uint32_t h0 = part * a.per_split, h1 = min(heads, h0 + a.per_split);
-    const bool in = p < a.head_dim / 16 && tok < a.n && h0 < h1;
+__global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int kBatch = TYPE == KVM_TYPE_F32 ? 1 : 2;      // heads of a thread in flight
+    constexpr uint64_t kEs = TYPE == KVM_TYPE_F32 ? 4 : 2;
+    __shared__ __align__(16) float cs[2][kRopeTokens][kRopeMaxDim / 16 * kRopePitch];
     const uint32_t half = a.n_rot / 2, pairs = a.n_rot / 16;
-    const bool rot = p < pairs;
+    const uint32_t p = threadIdx.x & (a.lanes - 1), grp = threadIdx.x / a.lanes, groups = kRopeThreads / a.lanes;
+    const uint32_t heads = a.q.heads + a.k.heads;
+    const uint32_t rounds = (heads + groups - 1) / groups;
+    const bool in = p < a.head_dim / 16, rot = p < pairs;
     // the two chunks of 8 of this thread
     const uint32_t e0 = rot ? 8 * p : a.n_rot + 16 * (p - pairs), e1 = rot ? e0 + half : e0 + 8;
-    auto address = [&](uint32_t h, bool out) -> uint64_t {
-        const bool key = h >= a.q.heads;
-        const RopeTensor &t = key ? a.k : a.q;
-        const uint64_t hh = key ? h - a.q.heads : h;
-        return out ? reinterpret_cast<uint64_t>(t.dst) + tok * t.d_tok + hh * t.d_head
-                   : reinterpret_cast<uint64_t>(t.src) + tok * t.s_tok + hh * t.s_head;
-    };
-    auto fetch = [&](uint32_t h, float (&x0)[8], float (&x1)[8]) {
-        const uint64_t dim = h >= a.q.heads ? a.k.s_dim : a.q.s_dim;
-        const uint8_t *src = reinterpret_cast<const uint8_t *>(address(h, false));
-        load8<TYPE, VEC>(src + e0 * dim, dim, x0);
-        load8<TYPE, VEC>(src + e1 * dim, dim, x1);
-    };
-    float x0[8], x1[8], n0[8], n1[8], w0[8], w1[8], cs[8], sn[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+    float2 wq0[4], wq1[4];
     if (in) {
-        fetch(h0, x0, x1);
-        load_weights<VEC>(h0 < a.q.heads ? a.q.weight : a.k.weight, e0, w0);
-        load_weights<VEC>(h0 < a.q.heads ? a.q.weight : a.k.weight, e1, w1);
-        if (rot) {
-            const double pos = static_cast<double>(a.pos[tok]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double ang = pos * static_cast<double>(a.freqs[e0 + i]);
-                // in half turns: 1 / pi to 106 bits, its F64 value and the remainder
-                const double turn = ang * 0.31830988618379067154;
-                const double rest = fma(ang, 0.31830988618379067154, -turn) + ang * -1.9678676675182486e-17;
-                const double near = turn - 2.0 * rint(0.5 * turn);
-                sincospif(static_cast<float>(near + rest), &sn[i], &cs[i]);
-            }
-        }
+        load_weights<VEC>(a.q.weight, e0, wq0);
+        load_weights<VEC>(a.q.weight, e1, wq1);
     }
-    // every thread of the warp takes the same number of turns (per_split), so the
-    // head's threads can reduce with full-warp shuffles
-    for (uint32_t j = 0; j < a.per_split; ++j) {
-        const uint32_t h = h0 + j;
-        const bool on = in && h < h1;
-        if (in && h + 1 < h1) fetch(h + 1, n0, n1);
-        if (on && h == a.q.heads && j) {
-            load_weights<VEC>(a.k.weight, e0, w0);
-            load_weights<VEC>(a.k.weight, e1, w1);
-        }
-        float ss = 0.0f;
+    for (uint32_t tok0 = blockIdx.x * a.tokens; tok0 < a.n; tok0 += gridDim.x * a.tokens) {
+        const uint32_t toks = min(a.tokens, a.n - tok0);
+        // item: (token, round), this thread's head of it
+        const uint32_t items = toks * rounds;
+        bool ready = false;
+        uint32_t tk_in = 0, rd_in = 0, tk = 0, rd = 0;      // (token, round) of the next load, of the next result
+        for (uint32_t i0 = 0; i0 < items; i0 += kBatch) {
+            Raw8<TYPE> r0[kBatch], r1[kBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
-        for (uint32_t o = a.lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (on) {
-            const float rs = rsqrtf(ss / static_cast<float>(a.head_dim) + a.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y0 = x0[i] * rs * w0[i], y1 = x1[i] * rs * w1[i];
-                x0[i] = rot ? y0 * cs[i] - y1 * sn[i] : y0;
-                x1[i] = rot ? y1 * cs[i] + y0 * sn[i] : y1;
+            for (int k = 0; k < kBatch; ++k) {
+                const uint32_t h = rd_in * groups + grp;
+                if (in && tk_in < toks && h < heads) {
+                    const bool key = h >= a.q.heads;
+                    const RopeTensor &t = key ? a.k : a.q;
+                    const uint8_t *src = t.src + head_offset<VEC>(tok0 + tk_in, t.s_tok, key ? h - a.q.heads : h, t.s_head);
+                    load8<TYPE, VEC>(src + e0 * (VEC ? kEs : t.s_dim), t.s_dim, r0[k]);
+                    load8<TYPE, VEC>(src + e1 * (VEC ? kEs : t.s_dim), t.s_dim, r1[k]);
+                }
+                if (++rd_in == rounds) {
+                    rd_in = 0;
+                    ++tk_in;
+                }
             }
-            const uint64_t dim = h >= a.q.heads ? a.k.d_dim : a.q.d_dim;
-            uint8_t *dst = reinterpret_cast<uint8_t *>(address(h, true));
-            store8<TYPE, VEC>(dst + e0 * dim, dim, x0);
-            store8<TYPE, VEC>(dst + e1 * dim, dim, x1);
-        }
+            if (!ready) {
+                for (uint32_t x = threadIdx.x; x < toks * half; x += kRopeThreads) {
+                    const uint32_t of = x / half, i = x - of * half;
+                    const double ang = static_cast<double>(a.pos[tok0 + of]) * static_cast<double>(a.freqs[i]);
+                    // in half turns: 1 / pi to 106 bits, its F64 value and the remainder
+                    const double turn = ang * 0.31830988618379067154;
+                    const double rest = fma(ang, 0.31830988618379067154, -turn) + ang * -1.9678676675182486e-17;
+                    const double near = turn - 2.0 * rint(0.5 * turn);
+                    float sn, co;
+                    sincospif(static_cast<float>(near + rest), &sn, &co);
+                    const uint32_t at = (i / 8) * kRopePitch + (i & 7);
+                    cs[0][of][at] = co;
+                    cs[1][of][at] = sn;
+                }
+                __syncthreads();
+                ready = true;
+            }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x0[i] = n0[i];
-            x1[i] = n1[i];
+            for (int k = 0; k < kBatch; ++k) {
+                const uint32_t h = rd * groups + grp, row = tk;
+                if (row >= toks) break;            // alike in the whole CTA
+                if (++rd == rounds) {
+                    rd = 0;
+                    ++tk;
+                }
+                const bool on = in && h < heads, key = h >= a.q.heads;
+                float2 x0[4] = {}, x1[4] = {}, s2 = make_float2(0.0f, 0.0f);
+                if (on) {
+                    widen8<TYPE>(r0[k], x0);
+                    widen8<TYPE>(r1[k], x1);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s2 = f2_fma_rn(x1[e], x1[e], f2_fma_rn(x0[e], x0[e], s2));
+                float ss = s2.x + s2.y;
+                for (uint32_t o = a.lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (!on) continue;
+                const float rs = rsqrtf(ss * a.inv_dim + a.eps);
+                const float2 rs2 = make_float2(rs, rs);
+                if (key) {                         // few heads: weights from the cache
+                    float2 w0[4], w1[4];
+                    load_weights<VEC>(a.k.weight, e0, w0);
+                    load_weights<VEC>(a.k.weight, e1, w1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x0[e] = f2_mul_rn(x0[e], f2_mul_rn(rs2, w0[e]));
+                        x1[e] = f2_mul_rn(x1[e], f2_mul_rn(rs2, w1[e]));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x0[e] = f2_mul_rn(x0[e], f2_mul_rn(rs2, wq0[e]));
+                        x1[e] = f2_mul_rn(x1[e], f2_mul_rn(rs2, wq1[e]));
+                    }
+                }
+                if (rot) {
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float4 co = *reinterpret_cast<const float4 *>(&cs[0][row][p * kRopePitch + 2 * e]);
+                        const float4 sn = *reinterpret_cast<const float4 *>(&cs[1][row][p * kRopePitch + 2 * e]);
+                        const float2 c2[2] = {make_float2(co.x, co.y), make_float2(co.z, co.w)};
+                        const float2 t2[2] = {make_float2(sn.x, sn.y), make_float2(sn.z, sn.w)};
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 minus = make_float2(-t2[i].x, -t2[i].y);
+                            const float2 u = f2_fma_rn(x0[e + i], c2[i], f2_mul_rn(x1[e + i], minus));
+                            x1[e + i] = f2_fma_rn(x1[e + i], c2[i], f2_mul_rn(x0[e + i], t2[i]));
+                            x0[e + i] = u;
+                        }
+                    }
+                }
+                const RopeTensor &t = key ? a.k : a.q;
+                uint8_t *dst = t.dst + head_offset<VEC>(tok0 + row, t.d_tok, key ? h - a.q.heads : h, t.d_head);
+                store8<TYPE, VEC>(dst + e0 * (VEC ? kEs : t.d_dim), t.d_dim, x0);
+                store8<TYPE, VEC>(dst + e1 * (VEC ? kEs : t.d_dim), t.d_dim, x1);
+            }
         }
+        __syncthreads();                           // cos / sin are free for the next tokens
     }
 }
 
 template <int TYPE>
 void launch(const RopeArgs &a, uint32_t n, bool vec, cudaStream_t st) {
-    const uint64_t threads = static_cast<uint64_t>(n) * a.splits * a.lanes;
-    const uint32_t grid = static_cast<uint32_t>((threads + kRopeThreads - 1) / kRopeThreads);
+    // a few CTAs an SM, each looping over its rows
+    const uint64_t steps = (static_cast<uint64_t>(n) + a.tokens - 1) / a.tokens;
+    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(steps, 4ull * num_sms()));
     if (vec) qk_norm_rope_kernel<TYPE, true><<<grid, kRopeThreads, 0, st>>>(a);
     else qk_norm_rope_kernel<TYPE, false><<<grid, kRopeThreads, 0, st>>>(a);
 }
+
+bool rope_vec(const kvm_rows *r) { return rows_vec16(r) && ((r->nb_head | r->nb_tok) >> 32) == 0; }
 
 RopeTensor tensor(const kvm_rows *in, const kvm_rows *out, const float *w) {
     RopeTensor t{};
@@ -263,14 +322,14 @@ extern "C" kvm_status kvm_qk_norm_rope(kvm_stream stream, uint32_t n, const kvm_
     a.n_rot = n_rot;
     a.lanes = 1;
     while (a.lanes < D / 16u) a.lanes *= 2;
-    const uint32_t heads = a.q.heads + a.k.heads;
-    const uint64_t fill = 1024ull * num_sms(), have = static_cast<uint64_t>(n) * a.lanes;
     a.n = n;
-    a.per_split = heads;
-    if (have < fill) a.per_split = static_cast<uint32_t>(std::max<uint64_t>(1, heads * have / fill));
-    a.splits = (heads + a.per_split - 1) / a.per_split;
-    if (static_cast<uint64_t>(n) * a.splits * a.lanes / kRopeThreads > 0x7ffffff0ull) return layer_fail(KVM_EINVAL, "%s: too many rows", me);
-    const bool vec = ((reinterpret_cast<uintptr_t>(d_q_weight) | reinterpret_cast<uintptr_t>(d_k_weight)) & 15u) == 0 && rows_vec16(q) && rows_vec16(q_out) && (!k || (rows_vec16(k) && rows_vec16(k_out)));
+    a.inv_dim = 1.0f / static_cast<float>(D);
+    // as many rows at a time as keep a thread's batch of heads full, while every SM
+    // still has several CTAs' worth
+    const uint32_t groups = kRopeThreads / a.lanes, rounds = (a.q.heads + a.k.heads + groups - 1) / groups;
+    a.tokens = 1;
+    while (a.tokens < kRopeTokens && 2u * a.tokens * rounds <= 4u && n >= 8ull * a.tokens * num_sms()) a.tokens *= 2;
+    const bool vec = ((reinterpret_cast<uintptr_t>(d_q_weight) | reinterpret_cast<uintptr_t>(d_k_weight)) & 15u) == 0 && rope_vec(q) && rope_vec(q_out) && (!k || (rope_vec(k) && rope_vec(k_out)));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (q->type == KVM_TYPE_F32) launch<KVM_TYPE_F32>(a, n, vec, st);
     else if (q->type == KVM_TYPE_F16) launch<KVM_TYPE_F16>(a, n, vec, st);

@@ -295,7 +295,7 @@ def check_attend(got, want, spread, peak, q, k, scale, keys, bf16):
     D = q.shape[-1]
     with np.errstate(invalid="ignore"):
         k = np.abs(np.where(np.isfinite(k), k, 0.0)).max()
-        ds = scale * np.abs(q).max() * k * (np.sqrt(D) * 2.0 ** -11 + D * 2.0 ** -23)
+        ds = abs(scale) * np.abs(q).max() * k * (np.sqrt(D) * 2.0 ** -11 + D * 2.0 ** -23)
     tol = spread * (3 * 2.0 ** -11 + 2 * ds) + keys * 2.0 ** -39 * peak + np.abs(want) * (2.0 ** -8 if bf16 else 2.0 ** -11) + 2.0 ** -25
     assert np.isfinite(want).all()
     assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
@@ -498,6 +498,15 @@ def test_attend_queries_of_every_size(kvm_lib, new):
     got = w.run(q, [0, new], True, max_new=new)
     assert got[0, 2].isnan().all() and torch.equal(got[0, 0], want[0, 0]) and torch.equal(got[0, 3], want[0, 3])
     assert torch.isfinite(got[0, 1]).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attend_scales(kvm_lib, new, scale):
+    """A scale of 0 is a mean over the seen keys; a negative one turns the order."""
+    import torch
+    w = Window(kvm_lib, torch, 2, ("q4_0", "q5_0"), 1, 128, 32, [170])
+    w.check(queries(torch, w.rng, new, 4, 128, "bf16"), [0, new], True, scale=scale, max_new=new)
 
 
 @pytest.mark.parametrize("base", [0, 4, 16])
