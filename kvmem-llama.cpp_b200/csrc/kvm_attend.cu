@@ -29,7 +29,7 @@ bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const At
     if (!encode) return false;
     const cuuint64_t dims[2] = {row_bytes / 4u, static_cast<uint64_t>(a.n_slots) * a.block_tokens};
     const cuuint64_t strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_bytes / 4u, kAttendStep}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {box_bytes / 4u, kAttendBox}, step[2] = {1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -120,9 +120,10 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     a.out = rows_of(out);
     a.work = static_cast<uint8_t *>(d_work);
     a.align16 = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.row_k | a.row_v) & 15u) == 0;
-    a.tma = a.align16 && c->block_tokens % kAttendStep == 0;
+    a.tma = a.align16 && c->block_tokens % kAttendBox == 0;
     a.q_vec = rows_vec16(q);
     a.out_vec = rows_vec16(out);
+    a.max_keys = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(b->table_cols) * c->block_tokens, 0x7fffffffu));
     a.heads_cta = c->n_head_kv % 4u == 0 ? 4 : c->n_head_kv % 2u == 0 ? 2 : 1;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const uint64_t sms = static_cast<uint64_t>(num_sms());
@@ -138,19 +139,21 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     auto launch = [&](int nt, uint32_t min_rows, uint32_t max_rows) {
         a.min_rows = min_rows;
         a.max_rows = max_rows;
-        const uint32_t grid = nt ? ctas(8u * nt, kAttendStep, a.heads_cta) : ctas(128, 64, 1);
+        const uint32_t grid = nt ? ctas(8u * nt, 16u, a.heads_cta) : ctas(128, 64, 1);
         if (D == 64u) return launch_d<64>(a, c->type_k, c->type_v, nt, grid, st);
         if (D == 128u) return launch_d<128>(a, c->type_k, c->type_v, nt, grid, st);
         return launch_d<256>(a, c->type_k, c->type_v, nt, grid, st);
     };
     // Requests of up to 16 query rows go to the split kernel, longer ones to the tile
-    // kernel; the device sorts them, so a wrong max_new only costs time.  One
-    // request that should be long needs no second launch.
+    // kernel; the device sorts them, so a wrong max_new only costs time.  Alike
+    // requests (one, or drafts that fit a row tile with more than 8 rows on average)
+    // take one kernel: the tile kernel's time hardly depends on the rows in a tile,
+    // and eight drafts of 1 to 4 tokens over 16385 keys took 145 us in both.
     const uint64_t most = static_cast<uint64_t>(b->max_new) * a.group;
     cudaError_t e;
     if (most <= 16u) {
         e = launch(most <= 8u ? 1 : 2, 1, 0xffffffffu);
-    } else if (b->n_seq == 1) {
+    } else if (b->n_seq == 1 || (most <= 128u && static_cast<uint64_t>(b->n_rows) * a.group > 8ull * b->n_seq)) {
         e = launch(0, 1, 0xffffffffu);
     } else {
         e = launch(2, 1, 16);

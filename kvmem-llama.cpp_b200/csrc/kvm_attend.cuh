@@ -42,6 +42,8 @@ struct AttendArgs {
     uint32_t tma;              // the cache's rows come through map_k, map_v (steps lie in one block)
     uint32_t q_vec, out_vec;   // contiguous heads, 16-byte aligned
     uint32_t heads_cta;        // KV heads that a CTA takes together: 1, 2 or 4
+    uint32_t whole;            // split kernel: no segment is shared (all are short), so nothing is joined
+    uint32_t max_keys;         // keys that the table's columns can hold, at most 2^31 - 1
     uint32_t min_rows, max_rows;   // query rows (tokens * group) a sequence needs to be taken by this launch
     CUtensorMap map_k, map_v;      // [cells][row bytes / 4] of 32-bit words
 };
@@ -145,13 +147,15 @@ __device__ __forceinline__ bool mbar_wait_near(uint64_t *bar, uint32_t parity) {
 }
 
 // ------------------------------------------------------- split bookkeeping --
-// The keys of every (sequence, row tile, KV head) are cut into steps of 16;
+// The keys of every (sequence, row tile, KV heads) are cut into steps of 16 or 32;
 // all steps of the call form one line that the CTAs share evenly, so ragged
 // batches balance without the host knowing a length.  A segment that one CTA
 // holds whole is written to `out`; one that several CTAs share leaves partial
 // results (max, sum, unnormalised output in F32) that attend_join_kernel adds
 // in CTA order.
-constexpr int kAttendStep = 16;
+constexpr int kAttendBox = 16;                // rows of a TMA box
+constexpr int kAttendMinSteps = 4;            // steps of 16 keys that a warp takes at least
+constexpr int kAttendSegmentSteps = 24;       // steps of 16 keys that beginning a segment is worth
 constexpr uint32_t kAttendMaxCtas = 592;      // descriptors in the workspace
 constexpr uint32_t kAttendDescBytes = 32;
 struct AttendDesc {                           // segment that starts in CTA c and goes on in c + 1 ...

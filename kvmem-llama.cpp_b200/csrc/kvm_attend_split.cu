@@ -20,9 +20,11 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
         a.tma = 0;
     const uint64_t slot = static_cast<uint64_t>(a.heads_cta) * attend_part_floats<D, NT>() * 4u;
     grid = static_cast<uint32_t>(std::min<uint64_t>(grid, (KVM_ATTEND_WORK_BYTES - kAttendMaxCtas * kAttendDescBytes) / (2 * slot)));
+    // segments that the least share would hold whole are not cut at all
+    a.whole = (a.max_keys + G::kStep - 1u) / G::kStep <= static_cast<uint32_t>(kAttendMinSteps / G::kTiles * (G::kWarps / a.heads_cta));
     attend_split_kernel<D, KT, VT, NT><<<grid, G::kThreads, smem, st>>>(a);
     cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || grid == 1) return e;
+    if (e != cudaSuccess || grid == 1 || a.whole) return e;
     return launch_after_prev(attend_join_kernel<D, NT>, dim3(std::min<uint32_t>(2u * num_sms(), grid * 8u * NT * a.heads_cta)), dim3(kJoinThreads), 0, st, a, grid);
 }
 

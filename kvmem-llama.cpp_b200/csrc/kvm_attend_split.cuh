@@ -26,12 +26,12 @@
 // straight from the rows' bytes, and P^T goes from the accumulators to the B
 // operand by one 8x8 transpose a half.  Which 16 elements of a block form one
 // K = 16 product is free as long as q agrees, so every lane takes the bytes of
-// one word.  A warp streams its own keys (16 a step) of one KV head through its
+// one word.  A warp streams its own keys (32 or 16 a step) of one KV head through its
 // own ring in shared memory and keeps its own running maximum, sum and output;
 // the warps of a CTA meet once a segment.  A CTA takes up to four KV heads of the
 // same keys: their slices share 32-byte sectors, and read by different CTAs at
 // different times they cost 1.7 times the window's bytes (961 of 569 MB over 32
-// windows).  The slices come by TMA, one 2D box a step, where a step lies in one
+// windows).  The slices come by TMA, 2D boxes of 16 rows, where those lie in one
 // block and rows are multiples of 16 bytes, else by cp.async.
 #pragma once
 
@@ -43,20 +43,37 @@ template <int D, int KT, int VT, int NT>
 struct SplitGeom {
     using K = Slice<KT, D>;
     using V = Slice<VT, D>;
-    static constexpr int kStage = kAttendStep * (K::kStride + V::kStride);
-    static constexpr int kRoom = 200 * 1024;
-    // twelve warps where the registers (D / 4 a row tile for the output) and two
-    // stages of each warp allow it
-    static constexpr int kWarps = (D * NT <= 256 && 24 * kStage <= kRoom) ? 12 : 16 * kStage <= kRoom ? 8 : 4;
+    static constexpr int kRoom = 226 * 1024;
+    // shared memory of a warp with `tiles` 16-key tiles a step and `stages` steps:
+    // rows; K scales as F16 and F32, V scales as F16; two barriers and a mask a step
+    static constexpr int warp_bytes(int tiles, int stages) {
+        return stages * tiles * 16 * (K::kStride + V::kStride) + 1024 * tiles + stages * 24;
+    }
+    static constexpr bool fits(int warps, int tiles, int stages) { return warps * warp_bytes(tiles, stages) + 128 <= kRoom; }
+    // 32 keys a step where they fit: the step's fixed work (ring, statistics,
+    // shuffles) is half of the instructions at 16 keys.  Twelve warps where the
+    // registers (D / 4 a row tile for the output) and the rows allow it.  K and V have
+    // barriers of their own, so that one stage is enough: K's next rows are under way
+    // during the V products and the other way round.
+    static constexpr int kMany = D * NT <= 256 ? 12 : 8;
+    static constexpr int kTiles = fits(8, 2, 1) ? 2 : 1;                   // 16-key tiles a step
+    static constexpr int kStep = 16 * kTiles;
+    static constexpr int kWarps = fits(kMany, kTiles, 1) ? kMany : fits(8, kTiles, 1) ? 8 : 4;
     static constexpr int kThreads = kWarps * 32;
-    static constexpr int kBudget = kRoom / (kWarps * kStage);
-    static constexpr int kStages = kBudget > 6 ? 6 : kBudget < 2 ? 2 : kBudget;
-    static constexpr int kScaleBytes = 1024;      // per warp: K f16, K f32, V f16
+    static constexpr int kStages = fits(kWarps, kTiles, 3) ? 3 : fits(kWarps, kTiles, 2) ? 2 : 1;
+    static constexpr int kRowsK = kStep * K::kStride, kRowsV = kStep * V::kStride;
+    static constexpr int kStage = kRowsK + kRowsV;
+    static constexpr int kScaleBytes = 1024 * kTiles;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kMerge = kWarps * 8 * NT * (D + 4 + 2) * 4;
     static constexpr int kBig = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
-    static constexpr int kSmem = kBig + kWarps * (kScaleBytes + kStages * 16);
+    static constexpr int kSmem = kBig + kWarps * (kScaleBytes + kStages * 24);
 };
+
+// a / b, by a 32-bit division where a allows it (the 64-bit routine is ten times as long)
+__device__ __forceinline__ unsigned long long div_small(unsigned long long a, uint32_t b) {
+    return (a >> 32) == 0 ? static_cast<uint32_t>(a) / b : a / b;
+}
 
 __device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ uint32_t lds16(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
@@ -187,6 +204,11 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
     using SK = Slice<KT, D>;
     using SV = Slice<VT, D>;
     constexpr int NB = D / 32, W = G::kWarps, kThreads = G::kThreads, NS = G::kStages, R = 8 * NT;
+    constexpr int MT = G::kTiles, kStep = G::kStep;
+    // beginning a segment (its queries, the first rows, the warps' merge) counts as
+    // this many steps in the shares
+    const uint32_t kLead = a.whole ? 0u : kAttendSegmentSteps / MT;
+    constexpr uint32_t kAll = MT == 2 ? 0xffffffffu : 0xffffu;
     constexpr bool kCodesK = KT != KVM_TYPE_F16, kCodesV = VT != KVM_TYPE_F16;
     constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 14.0f;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -194,16 +216,21 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
     const int hg = static_cast<int>(a.heads_cta), hsub = warp % hg, sub = warp / hg, nsub = W / hg;
     uint8_t *ring = smem + warp * NS * G::kStage;
     uint8_t *scales = smem + G::kBig + warp * G::kScaleBytes;
-    __half *k16 = reinterpret_cast<__half *>(scales);              // [16 keys][8 blocks]
-    float *k32 = reinterpret_cast<float *>(scales + 256);          // [16][8]
-    __half *v16 = reinterpret_cast<__half *>(scales + 768);        // [8 blocks][16 keys, a lane's four together]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBig + W * G::kScaleBytes) + warp * NS;
-    uint32_t *valid = reinterpret_cast<uint32_t *>(smem + G::kBig + W * (G::kScaleBytes + NS * 8)) + warp * NS;
+    // K scales in F32 [key][8 blocks]; V scales in F16, for each 16 keys [8 blocks][a lane's four keys
+    // together], 20 halves a block (its readers' and writers' banks differ)
+    float *k32 = reinterpret_cast<float *>(scales);
+    __half *v16 = reinterpret_cast<__half *>(scales + 512 * MT);
+    constexpr int kVBlock = 20, kVTile = 8 * kVBlock;
+    uint64_t *k_bar = reinterpret_cast<uint64_t *>(smem + G::kBig + W * G::kScaleBytes) + warp * NS, *v_bar = k_bar + W * NS;
+    uint32_t *valid = reinterpret_cast<uint32_t *>(smem + G::kBig + W * (G::kScaleBytes + NS * 16)) + warp * NS;
     __shared__ unsigned long long s_scan[W], s_off;
     __shared__ uint32_t s_seq;
 
     if (lane == 0)
-        for (int i = 0; i < NS; ++i) mbar_init(&bars[i], 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&k_bar[i], MT);
+            mbar_init(&v_bar[i], MT);
+        }
     fence_mbar_init();
 
     // ---- this CTA's share of the line of steps
@@ -211,8 +238,8 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         const AttendSeq q = attend_seq(a, s);
         const uint64_t rows = static_cast<uint64_t>(q.n_new) * a.group;
         if (q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) return 0ull;
-        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kAttendStep - 1u) / kAttendStep);
-        return ((rows + R - 1) / R) * (a.n_head_kv / hg) * steps;
+        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kStep - 1u) / kStep);
+        return ((rows + R - 1) / R) * (a.n_head_kv / hg) * (a.whole ? 1u : steps + kLead);
     };
     // inclusive sum of n over the CTA's threads; *all gets the total
     auto scan = [&](unsigned long long n, unsigned long long *all) -> unsigned long long {
@@ -238,8 +265,9 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
     unsigned long long mine = 0, total = 0;
     for (uint32_t s = tid; s < a.n_seq; s += kThreads) mine += units(s);
     const unsigned long long upto = scan(mine, &total);
-    unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < static_cast<unsigned long long>(nsub)) share = nsub;
+    unsigned long long share = div_small(total + gridDim.x - 1, gridDim.x);
+    // a few steps a warp at least: sharing less costs more in the join than it saves
+    if (!a.whole) share = max(share, static_cast<unsigned long long>(kAttendMinSteps / MT * nsub));
     const unsigned long long u0 = share * blockIdx.x;
     const unsigned long long u1 = min(u0 + share, total);
     AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
@@ -266,7 +294,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
     uint32_t seq = s_seq;
     unsigned long long off = s_off;
     bool described = false;
-    uint32_t issued = 0;                      // ring position of the warp's next load
+    uint32_t stage_at = 0, phase = 0;         // ring stage of the warp's next step
     bool lost = false;                        // a bounded wait ran out
 
     for (unsigned long long pos = u0; pos < u1;) {
@@ -280,17 +308,136 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 continue;
             }
         }
-        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kAttendStep - 1u) / kAttendStep);
-        const uint32_t seg = static_cast<uint32_t>(off / steps);
-        const uint32_t in0 = static_cast<uint32_t>(off - static_cast<unsigned long long>(seg) * steps);
-        const uint32_t left = steps - in0;
+        const uint32_t steps = max(1u, (static_cast<uint32_t>(q.keys) + kStep - 1u) / kStep);
+        const uint32_t length = a.whole ? 1u : steps + kLead;
+        const uint32_t seg = static_cast<uint32_t>(div_small(off, length));
+        const uint32_t at0 = static_cast<uint32_t>(off - static_cast<unsigned long long>(seg) * length);
+        const uint32_t left = length - at0;
         const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(left), u1 - pos));
+        // its steps: those behind the lead
+        const uint32_t in0 = at0 > kLead ? at0 - kLead : 0u, in_end = a.whole ? steps : at0 + take > kLead ? at0 + take - kLead : 0u;
         const uint32_t head0 = seg % (a.n_head_kv / hg) * hg, head = head0 + hsub;
         const uint32_t first = seg / (a.n_head_kv / hg) * R;
         const uint32_t all_rows = static_cast<uint32_t>(q.n_new) * a.group;
         const uint32_t rows = min(static_cast<uint32_t>(R), all_rows - first);
         const int32_t kend = attend_limit(a, q, (first + rows - 1) / a.group);
         const int32_t kfull = attend_limit(a, q, first / a.group);      // every row sees the keys below
+
+        // ---- the warp's steps: in0 + sub, + nsub, ...
+        const uint32_t kstart = in0 * kStep;
+        const uint32_t in1 = min(in_end, (static_cast<uint32_t>(kend) + kStep - 1u) / kStep);
+        const int n_steps = in1 > in0 + sub ? static_cast<int>((in1 - in0 - sub + nsub - 1) / nsub) : 0;
+        const int32_t *trow = a.table + seq * a.table_stride;
+        const uint8_t *kbase = a.k + static_cast<uint64_t>(head) * SK::kBytes;
+        const uint8_t *vbase = a.v + static_cast<uint64_t>(head) * SV::kBytes;
+
+        // bytes between the slice and the 16-byte boundary its box starts at
+        const int lead_k = a.tma ? static_cast<int>(head * SK::kBytes & 15u) : 0;
+        const int lead_v = a.tma ? static_cast<int>(head * SV::kBytes & 15u) : 0;
+
+        // TMA: lane h < MT brings the h-th 16 keys of a step, which lie in one block;
+        // the block's slot is fetched while the load before is issued
+        const int32_t lane_key = static_cast<int32_t>(kstart) + sub * kStep + 16 * lane;
+        const int32_t x_k = static_cast<int32_t>(head * SK::kBytes / 16u * 4u), x_v = static_cast<int32_t>(head * SV::kBytes / 16u * 4u);
+        auto entry = [&](int i) -> int32_t {
+            const int32_t key = lane_key + i * nsub * kStep;
+            return lane < MT && key < kend ? trow[attend_block(a, static_cast<uint32_t>(key))] : -1;
+        };
+        int32_t slot_next = a.tma ? entry(0) : -1;
+
+        // load(i, side, stage): K (side 0), then V (side 1) of step i; K's call looks the
+        // cells up for both
+        int32_t cell = -1;
+        auto load = [&](int i, auto side, uint32_t to) {
+            constexpr bool kIsV = decltype(side)::value != 0;
+            using S = std::conditional_t<kIsV, SV, SK>;
+            uint8_t *dst = ring + to * G::kStage + (kIsV ? G::kRowsK : 0);
+            if (a.tma) {
+                if constexpr (!kIsV) {
+                    const int32_t slot = slot_next;
+                    slot_next = entry(i + 1);
+                    if (lane < MT) {
+                        const int32_t key = lane_key + i * nsub * kStep, left = kend - key;
+                        const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots;
+                        reinterpret_cast<uint16_t *>(valid + to)[lane] =
+                            static_cast<uint16_t>(!ok ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1u);
+                        const uint32_t in_block = static_cast<uint32_t>(key) - attend_block(a, static_cast<uint32_t>(key)) * a.block_tokens;
+                        cell = ok ? static_cast<int32_t>(slot * a.block_tokens + in_block) : -1;
+                    }
+                }
+                if (lane < MT) {
+                    uint64_t *bar = (kIsV ? v_bar : k_bar) + to;
+                    if (cell >= 0) {
+                        mbar_arrive_expect_tx(bar, 16 * S::kStride);
+                        tma_load_2d(dst + lane * 16 * S::kStride, kIsV ? &a.map_v : &a.map_k, kIsV ? x_v : x_k, cell, bar);
+                    } else {
+                        mbar_arrive(bar);
+                    }
+                }
+                return;
+            }
+            if constexpr (!kIsV) {
+                const uint32_t key = kstart + (sub + i * nsub) * kStep + (lane & (kStep - 1));
+                cell = -1;
+                if (key < static_cast<uint32_t>(kend)) {
+                    const uint32_t blk = attend_block(a, key);
+                    const int32_t slot = trow[blk];
+                    if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
+                        cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
+                }
+                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & kAll;
+                if (lane == 0) valid[to] = ok;
+            }
+            const uint8_t *base = kIsV ? vbase : kbase;
+            const uint64_t row_bytes = kIsV ? a.row_v : a.row_k;
+            auto pieces = [&](auto width) {
+                constexpr int V = decltype(width)::value, C = S::kBytes / V;
+#pragma unroll 4
+                for (int y = 0; y < (kStep * C + 31) / 32; ++y) {
+                    const int x = lane + 32 * y, row = min(x / C, kStep - 1), c = x - row * C;
+                    const int32_t cr = __shfl_sync(0xffffffffu, cell, row);
+                    const uint8_t *src = base + (cr >= 0 ? cr * row_bytes + c * V : 0ull);
+                    const uint32_t d = smem_u32(dst + row * S::kStride + c * V);
+                    if (x < kStep * C) {
+                        if constexpr (V == 16) cp_async16(d, src, cr >= 0 ? 16u : 0u);
+                        else cp_async4(d, src, cr >= 0 ? 4u : 0u);
+                    }
+                }
+            };
+            if constexpr (S::kBytes % 16 == 0) {
+                if (a.align16) {
+                    pieces(std::integral_constant<int, 16>{});
+                    return;
+                }
+            }
+            pieces(std::integral_constant<int, 4>{});
+        };
+        constexpr std::integral_constant<int, 0> kSideK{};
+        constexpr std::integral_constant<int, 1> kSideV{};
+        auto arrived = [&](uint64_t *bar) {
+            if (a.tma) {
+                if (!lost && !mbar_wait_near(bar, phase)) lost = true;
+            } else {
+                cp_async_wait<2 * NS - 1>();
+            }
+            __syncwarp();
+        };
+        auto hidden = [&](uint8_t *rows, auto slice, uint32_t ok) {     // a box brings the bytes of hidden rows too: drop them
+            using S = decltype(slice);
+            for (int x = lane; x < kStep * (S::kBytes / 4); x += 32)
+                if (!((ok >> (x % kStep)) & 1u)) *reinterpret_cast<uint32_t *>(rows + (x % kStep) * S::kStride + 4 * (x / kStep)) = 0u;
+            fence_proxy_async_smem();
+            __syncwarp();
+        };
+
+#pragma unroll 1
+        for (int i = 0; i < NS; ++i) {
+            const uint32_t to = stage_at + i < NS ? stage_at + i : stage_at + i - NS;
+            if (i < n_steps) load(i, kSideK, to);
+            cp_async_commit();
+            if (i < n_steps) load(i, kSideV, to);
+            cp_async_commit();
+        }
 
         // ---- q of this lane's columns: row first + nt*8 + g
         uint32_t qf[NT][NB][4];
@@ -349,7 +496,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
             // two steps: a factor of 2^(want - e) alone may be out of F32's range
             const int up = (top > 0.0f && e < 128) ? max(-126, min(126, want - e)) : 0;
-            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+            const float mul = (a.scale_log2 < 0.0f ? -1.0f : 1.0f) * __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
             uint32_t hi[NB / 2 ? NB / 2 : 1], lo[NB / 2 ? NB / 2 : 1];
             float sums[NB];
 #pragma unroll
@@ -379,7 +526,8 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 }
             }
             // columns 2t, 2t+1 of the accumulators: their factor and limit
-            const float f = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            // not 0: a hidden key's -inf has to stay -inf
+            const float f = fmaxf(fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
             const int32_t l = in ? attend_limit(a, q, static_cast<int32_t>(tok)) : kend;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -388,11 +536,11 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             }
         }
 
-        float o[NT][NB][2][4], m[NT][2], l[NT][2];
+        float o[NT][NB][2][4], m[NT][2], l[NT][2], bias[NT][2];      // bias: kWeightLog - m, 0 while m is -inf
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = kNegInf;
-            l[nt][0] = l[nt][1] = 0.0f;
+            l[nt][0] = l[nt][1] = bias[nt][0] = bias[nt][1] = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -400,242 +548,120 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         }
         int vexp = 15;                        // o holds the output times 2^(vexp - 24)
 
-        // ---- the warp's steps: in0 + sub, + nsub, ...
-        const uint32_t kstart = in0 * kAttendStep;
-        const uint32_t in1 = min(in0 + take, (static_cast<uint32_t>(kend) + kAttendStep - 1u) / kAttendStep);
-        const int n_steps = in1 > in0 + sub ? static_cast<int>((in1 - in0 - sub + nsub - 1) / nsub) : 0;
-        const int32_t *trow = a.table + seq * a.table_stride;
-        const uint8_t *kbase = a.k + static_cast<uint64_t>(head) * SK::kBytes;
-        const uint8_t *vbase = a.v + static_cast<uint64_t>(head) * SV::kBytes;
-
-        // bytes between the slice and the 16-byte boundary its box starts at
-        const int lead_k = a.tma ? static_cast<int>(head * SK::kBytes & 15u) : 0;
-        const int lead_v = a.tma ? static_cast<int>(head * SV::kBytes & 15u) : 0;
-
-        auto load = [&](int i) {
-            const uint32_t slot_at = (issued + i) % NS;
-            uint8_t *st = ring + slot_at * G::kStage;
-            const uint32_t key0 = kstart + (sub + i * nsub) * kAttendStep;
-            if (a.tma) {                      // all 16 keys lie in one block
-                if (lane == 0) {
-                    const uint32_t blk = attend_block(a, key0);
-                    const int32_t slot = trow[blk];
-                    const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots;
-                    const uint32_t left = static_cast<uint32_t>(kend) - key0;
-                    valid[slot_at] = ok ? (left >= 16u ? 0xffffu : (1u << left) - 1u) : 0u;
-                    if (ok) {
-                        const int32_t cell = static_cast<int32_t>(slot * a.block_tokens + (key0 - blk * a.block_tokens));
-                        mbar_arrive_expect_tx(&bars[slot_at], G::kStage);
-                        tma_load_2d(st, &a.map_k, static_cast<int32_t>(head * SK::kBytes / 16u * 4u), cell, &bars[slot_at]);
-                        tma_load_2d(st + kAttendStep * SK::kStride, &a.map_v, static_cast<int32_t>(head * SV::kBytes / 16u * 4u),
-                                    cell, &bars[slot_at]);
-                    } else {
-                        mbar_arrive(&bars[slot_at]);
-                    }
-                }
-                return;
-            }
-            const uint32_t key = key0 + (lane & 15);
-            int32_t cell = -1;
-            if (key < static_cast<uint32_t>(kend)) {
-                const uint32_t blk = attend_block(a, key);
-                const int32_t slot = trow[blk];
-                if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
-                    cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
-            }
-            const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
-            if (lane == 0) valid[slot_at] = ok;
-            auto copy = [&](auto slice, uint8_t *dst, const uint8_t *base, uint64_t row_bytes) {
-                using S = decltype(slice);
-                auto pieces = [&](auto width) {
-                    constexpr int V = decltype(width)::value, C = S::kBytes / V;
-#pragma unroll 4
-                    for (int y = 0; y < (kAttendStep * C + 31) / 32; ++y) {
-                        const int x = lane + 32 * y, r = min(x / C, kAttendStep - 1), c = x - r * C;
-                        const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
-                        const uint8_t *src = base + (cr >= 0 ? cr * row_bytes + c * V : 0ull);
-                        const uint32_t d = smem_u32(dst + r * S::kStride + c * V);
-                        if (x < kAttendStep * C) {
-                            if constexpr (V == 16) cp_async16(d, src, cr >= 0 ? 16u : 0u);
-                            else cp_async4(d, src, cr >= 0 ? 4u : 0u);
-                        }
-                    }
-                };
-                if constexpr (S::kBytes % 16 == 0) {
-                    if (a.align16) {
-                        pieces(std::integral_constant<int, 16>{});
-                        return;
-                    }
-                }
-                pieces(std::integral_constant<int, 4>{});
-            };
-            copy(SK{}, st, kbase, a.row_k);
-            copy(SV{}, st + kAttendStep * SK::kStride, vbase, a.row_v);
-        };
-
-#pragma unroll 1
-        for (int i = 0; i < NS - 1; ++i) {
-            if (i < n_steps) load(i);
-            cp_async_commit();
-        }
 #pragma unroll 1
         for (int i = 0; i < n_steps; ++i) {
-            const uint32_t at = (issued + i) % NS;
-            if (a.tma) {
-                if (!lost && !mbar_wait_near(&bars[at], ((issued + i) / NS) & 1u)) lost = true;
-            } else {
-                cp_async_wait<NS - 2>();
-            }
-            __syncwarp();
+            const uint32_t at = stage_at;
+            uint8_t *kr = ring + at * G::kStage + lead_k;
+            uint8_t *vr = ring + at * G::kStage + G::kRowsK + lead_v;
+            const int32_t key0 = static_cast<int32_t>(kstart) + (sub + i * nsub) * kStep;
+            arrived(&k_bar[at]);
             const uint32_t ok = valid[at];
-            if (i + NS - 1 < n_steps) load(i + NS - 1);
-            cp_async_commit();
-            if (ok == 0) continue;
-            const uint8_t *kr = ring + at * G::kStage + lead_k;
-            const uint8_t *vr = ring + at * G::kStage + kAttendStep * SK::kStride + lead_v;
-            const int32_t key0 = static_cast<int32_t>(kstart + (sub + i * nsub) * kAttendStep);
-            if (a.tma && ok != 0xffffu) {     // a box brings the bytes of hidden rows too: drop them
-                for (int x = lane; x < 16 * (SK::kBytes / 4 + SV::kBytes / 4); x += 32) {
-                    const int r = x & 15, w = x >> 4;
-                    if ((ok >> r) & 1u) continue;
-                    uint8_t *p = ring + at * G::kStage;
-                    p += w < SK::kBytes / 4 ? lead_k + r * SK::kStride + 4 * w
-                                            : kAttendStep * SK::kStride + lead_v + r * SV::kStride + 4 * (w - SK::kBytes / 4);
-                    *reinterpret_cast<uint32_t *>(p) = 0u;
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
+            if (a.tma && ok != kAll) hidden(kr, SK{}, ok);
 
-            // ---- the step's scales, laid out for the products
-            bool odd_values = false;          // an infinite or NaN V value
+            // ---- K's scales, laid out for the products
+            // lane (g, t) takes blocks 2t, 2t + 1 of keys g, g + 8, ...: no two lanes' banks meet
+            uint32_t kd[2 * MT];              // F16 pairs: A operand of the offsets' product
             if constexpr (kCodesK) {
 #pragma unroll
-                for (int x = lane; x < 16 * NB; x += 32) {
-                    const int key = x & 15, b = x >> 4;
-                    const __half d = *reinterpret_cast<const __half *>(kr + key * SK::kStride + b * SK::kBlock);
-                    k16[key * 8 + b] = d;
-                    k32[key * 8 + b] = __half2float(d);
-                }
-            }
-            if constexpr (kCodesV) {
-                uint32_t d[NB / 2], top = 0;
-#pragma unroll
-                for (int y = 0; y < NB / 2; ++y) {
-                    const int x = lane + 32 * y;
-                    d[y] = lds16(vr + (x & 15) * SV::kStride + (x >> 4) * SV::kBlock);
-                    const uint32_t size = d[y] & 0x7fffu;
-                    odd_values = odd_values || size >= 0x7c00u;
-                    top = max(top, size >= 0x7c00u ? 0u : size);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                odd_values = __any_sync(0xffffffffu, odd_values);
-                const int need = min(15, 15 - static_cast<int>(top >> 10));
-                if (need < vexp) {            // the largest scale so far to [1, 2)
-                    const float f = __uint_as_float(static_cast<uint32_t>(need - vexp + 127) << 23);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                o[nt][b][0][j] *= f;
-                                o[nt][b][1][j] *= f;
-                            }
-                    vexp = need;
-                }
-                const __half mul = vexp >= -14 ? __ushort_as_half(static_cast<uint16_t>((vexp + 15) << 10))
-                                               : __ushort_as_half(static_cast<uint16_t>(0x0200u));   // 2^-15
-#pragma unroll
-                for (int y = 0; y < NB / 2; ++y) {
-                    const int x = lane + 32 * y, key = x & 15;
-                    const int at = (key & 6) * 2 + (key & 1) + (key >> 3) * 2;
-                    v16[(x >> 4) * 16 + at] = __hmul(__ushort_as_half(static_cast<uint16_t>(d[y])), mul);
+                for (int i8 = 0; i8 < 2 * MT; ++i8) {
+                    kd[i8] = 0;
+                    if (2 * t < NB) {
+                        const uint8_t *p = kr + (8 * i8 + g) * SK::kStride + 2 * t * SK::kBlock;
+                        kd[i8] = lds16(p) | lds16(p + SK::kBlock) << 16;
+                        *reinterpret_cast<float2 *>(k32 + (8 * i8 + g) * 8 + 2 * t) =
+                            __half22float2(*reinterpret_cast<const __half2 *>(&kd[i8]));
+                    }
                 }
             }
             __syncwarp();
 
             // ---- S^T = K Q^T
-            float s[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+            float s[NT][MT][4];
             const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const uint8_t *row0 = kr + g * SK::kStride, *row1 = row0 + 8 * SK::kStride;
-            float dk[2][NB < 4 ? 4 : NB];     // scales of keys g, g + 8
-            if constexpr (kCodesK) {
 #pragma unroll
-                for (int b = 0; b < NB; b += 4) {
-                    *reinterpret_cast<float4 *>(&dk[0][b]) = *reinterpret_cast<const float4 *>(k32 + g * 8 + b);
-                    *reinterpret_cast<float4 *>(&dk[1][b]) = *reinterpret_cast<const float4 *>(k32 + (g + 8) * 8 + b);
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[nt][mt][j] = 0.0f;
+                const uint8_t *row0 = kr + (16 * mt + g) * SK::kStride, *row1 = row0 + 8 * SK::kStride;
+                float dk[2][NB < 4 ? 4 : NB];     // scales of keys g, g + 8
+                if constexpr (kCodesK) {
+#pragma unroll
+                    for (int b = 0; b < NB; b += 4) {
+                        *reinterpret_cast<float4 *>(&dk[0][b]) = *reinterpret_cast<const float4 *>(k32 + (16 * mt + g) * 8 + b);
+                        *reinterpret_cast<float4 *>(&dk[1][b]) = *reinterpret_cast<const float4 *>(k32 + (16 * mt + g + 8) * 8 + b);
+                    }
                 }
-            }
 #pragma unroll
-            for (int p = 0; p < NB / 2; ++p) {
-                uint32_t c0[2][2][2], c1[2][2][2];
-                k_codes<KT>(row0 + p * 2 * SK::kBlock, t, c0);
-                k_codes<KT>(row1 + p * 2 * SK::kBlock, t, c1);
+                for (int p = 0; p < NB / 2; ++p) {
+                    uint32_t c0[2][2][2], c1[2][2][2];
+                    k_codes<KT>(row0 + p * 2 * SK::kBlock, t, c0);
+                    k_codes<KT>(row1 + p * 2 * SK::kBlock, t, c1);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint32_t a0[4] = {c0[b][0][0], c1[b][0][0], c0[b][0][1], c1[b][0][1]};
-                    const uint32_t a1[4] = {c0[b][1][0], c1[b][1][0], c0[b][1][1], c1[b][1][1]};
-                    const float d0 = dk[0][2 * p + b], d1 = dk[1][2 * p + b];
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t a0[4] = {c0[b][0][0], c1[b][0][0], c0[b][0][1], c1[b][0][1]};
+                        const uint32_t a1[4] = {c0[b][1][0], c1[b][1][0], c0[b][1][1], c1[b][1][1]};
+                        const float d0 = dk[0][2 * p + b], d1 = dk[1][2 * p + b];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint32_t *qq = qf[nt][2 * p + b];
-                        if constexpr (kCodesK) {
-                            float part[4];
-                            mma_f16(part, a0, qq[0], qq[1], zero);
-                            mma_f16(part, a1, qq[2], qq[3], part);
-                            s[nt][0] = fmaf(d0, part[0], s[nt][0]);
-                            s[nt][1] = fmaf(d0, part[1], s[nt][1]);
-                            s[nt][2] = fmaf(d1, part[2], s[nt][2]);
-                            s[nt][3] = fmaf(d1, part[3], s[nt][3]);
-                        } else {
-                            mma_f16(s[nt], a0, qq[0], qq[1], s[nt]);
-                            mma_f16(s[nt], a1, qq[2], qq[3], s[nt]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t *qq = qf[nt][2 * p + b];
+                            float(&sum)[4] = s[nt][mt];
+                            if constexpr (kCodesK) {
+                                float part[4];
+                                mma_f16(part, a0, qq[0], qq[1], zero);
+                                mma_f16(part, a1, qq[2], qq[3], part);
+                                sum[0] = fmaf(d0, part[0], sum[0]);
+                                sum[1] = fmaf(d0, part[1], sum[1]);
+                                sum[2] = fmaf(d1, part[2], sum[2]);
+                                sum[3] = fmaf(d1, part[3], sum[3]);
+                            } else {
+                                mma_f16(sum, a0, qq[0], qq[1], sum);
+                                mma_f16(sum, a1, qq[2], qq[3], sum);
+                            }
                         }
                     }
                 }
-            }
-            if constexpr (kCodesK) {
-                const bool has = 2 * t < NB;
-                const uint32_t w0 = has ? *reinterpret_cast<const uint32_t *>(k16 + g * 8 + 2 * t) : 0u;
-                const uint32_t w1 = has ? *reinterpret_cast<const uint32_t *>(k16 + (g + 8) * 8 + 2 * t) : 0u;
-                const uint32_t aw[4] = {w0, w1, w0, w1};
+                if constexpr (kCodesK) {
+                    const uint32_t aw[4] = {kd[2 * mt], kd[2 * mt + 1], kd[2 * mt], kd[2 * mt + 1]};
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float c[4];
-                    mma_f16(c, aw, qc[nt][0], qc[nt][1], zero);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float c[4];
+                        mma_f16(c, aw, qc[nt][0], qc[nt][1], zero);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[nt][j] = fmaf(s[nt][j], 16777216.0f, c[j]);
+                        for (int j = 0; j < 4; ++j) s[nt][mt][j] = fmaf(s[nt][mt][j], 16777216.0f, c[j]);
+                    }
                 }
             }
 
+            __syncwarp();                     // every lane is done with this step's K rows
+            if (i + NS < n_steps) load(i + NS, kSideK, at);
+            cp_async_commit();
+
             // ---- softmax step
-            const bool mixed = key0 + kAttendStep > kfull || ok != 0xffffu;
-            uint32_t pb[NT][2];
-            float pr[NT][4];
-            bool grew = false;
+            const bool mixed = key0 + kStep > kfull || ok != kAll;
+            uint32_t pb[NT][MT][2];
             float mn[NT][2];
+            bool grew = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                if (mixed) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[nt][j] *= fac[nt][j & 1];
-                    if (mixed) {
-                        const int kk = g + (j >> 1) * 8;
-                        if (key0 + kk >= lim[nt][j & 1] || !((ok >> kk) & 1u)) s[nt][j] = kNegInf;
-                    }
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int kk = 16 * mt + g + (j >> 1) * 8;
+                            if (key0 + kk >= lim[nt][j & 1] || !((ok >> kk) & 1u)) s[nt][mt][j] = kNegInf;
+                        }
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float x = fmaxf(s[nt][i], s[nt][i + 2]);
+                    float x = fmaxf(s[nt][0][i], s[nt][0][i + 2]);
+                    if constexpr (MT == 2) x = fmaxf(x, fmaxf(s[nt][MT - 1][i], s[nt][MT - 1][i + 2]));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    mn[nt][i] = fmaxf(m[nt][i], x);
+                    mn[nt][i] = fmaxf(m[nt][i], x == kNegInf ? kNegInf : x * fac[nt][i]);
                     grew = grew || mn[nt][i] > m[nt][i];
                 }
             }
@@ -648,6 +674,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                         f[i] = mn[nt][i] > m[nt][i] ? exp2_approx(m[nt][i] - mn[nt][i]) : 1.0f;
                         l[nt][i] *= f[i];
                         m[nt][i] = mn[nt][i];
+                        bias[nt][i] = kWeightLog - (m[nt][i] == kNegInf ? kWeightLog : m[nt][i]);
                     }
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
@@ -659,21 +686,78 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float mm = m[nt][j & 1] == kNegInf ? 0.0f : m[nt][j & 1] - kWeightLog;
-                    pr[nt][j] = exp2_approx(s[nt][j] - mm);
-                    l[nt][j & 1] += pr[nt][j];
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[nt][mt][j] = exp2_approx(fmaf(s[nt][mt][j], fac[nt][j & 1], bias[nt][j & 1]));
+                        l[nt][j & 1] += s[nt][mt][j];
+                    }
+                    pb[nt][mt][0] = transpose8(pack_half2(s[nt][mt][0], s[nt][mt][1]));
+                    pb[nt][mt][1] = transpose8(pack_half2(s[nt][mt][2], s[nt][mt][3]));
                 }
-                pb[nt][0] = transpose8(pack_half2(pr[nt][0], pr[nt][1]));
-                pb[nt][1] = transpose8(pack_half2(pr[nt][2], pr[nt][3]));
-            }
 
+            // ---- V's rows and scales
+            arrived(&v_bar[at]);
+            if (a.tma && ok != kAll) hidden(vr, SV{}, ok);
+            bool odd_values = false;          // an infinite or NaN V value
+            if constexpr (kCodesV) {
+                uint32_t d[2 * MT], top = 0;  // pairs of blocks 2t, 2t + 1
+#pragma unroll
+                for (int i8 = 0; i8 < 2 * MT; ++i8) {
+                    d[i8] = 0;
+                    if (2 * t < NB) {
+                        const uint8_t *p = vr + (8 * i8 + g) * SV::kStride + 2 * t * SV::kBlock;
+                        d[i8] = lds16(p) | lds16(p + SV::kBlock) << 16;
+                    }
+                    top = __vmaxu2(top, d[i8] & 0x7fff7fffu);
+                }
+                // rarely: a scale beyond the range that vexp covers, or one that is not finite
+                const uint32_t over = static_cast<uint32_t>(16 - vexp) << 10;      // the smallest scale's bits out of range
+                if (__any_sync(0xffffffffu, (top & 0xffffu) >= over || (top >> 16) >= over)) {
+                    uint32_t finite = 0;
+#pragma unroll
+                    for (int i8 = 0; i8 < 2 * MT; ++i8)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t size = (d[i8] >> (16 * h)) & 0x7fffu;
+                            odd_values = odd_values || size >= 0x7c00u;
+                            finite = max(finite, size >= 0x7c00u ? 0u : size);
+                        }
+                    odd_values = __any_sync(0xffffffffu, odd_values);
+                    const int need = 15 - static_cast<int>(__reduce_max_sync(0xffffffffu, finite) >> 10);
+                    if (need < vexp) {        // the largest scale so far to [1, 2)
+                        const float f = __uint_as_float(static_cast<uint32_t>(need - vexp + 127) << 23);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    o[nt][b][0][j] *= f;
+                                    o[nt][b][1][j] *= f;
+                                }
+                        vexp = need;
+                    }
+                }
+                const uint32_t mul = 0x10001u * (vexp >= -14 ? static_cast<uint32_t>(vexp + 15) << 10 : 0x0200u);   // 2^vexp
+                if (2 * t < NB) {
+#pragma unroll
+                    for (int i8 = 0; i8 < 2 * MT; ++i8) {
+                        const uint32_t ds = mul_half2(d[i8], mul);
+                        // key g of the half i8 & 1 of its 16: behind the pair's other key
+                        __half *to = v16 + (i8 >> 1) * kVTile + 2 * t * kVBlock + (g >> 1) * 4 + (i8 & 1) * 2 + (g & 1);
+                        to[0] = __ushort_as_half(static_cast<uint16_t>(ds & 0xffffu));
+                        to[kVBlock] = __ushort_as_half(static_cast<uint16_t>(ds >> 16));
+                    }
+                }
+            }
+            __syncwarp();
             if constexpr (!kCodesV) {
                 if (mixed) {                  // a hidden key's infinity must not meet p = 0 in a product
-                    for (int x = lane; x < 16 * (D / 2); x += 32) {
-                        const uint32_t u = lds32(vr + (x & 15) * SV::kStride + (x >> 4) * 4);
+                    for (int x = lane; x < kStep * (D / 2); x += 32) {
+                        const uint32_t u = lds32(vr + (x % kStep) * SV::kStride + (x / kStep) * 4);
                         odd_values = odd_values || (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
                     }
                     odd_values = __any_sync(0xffffffffu, odd_values);
@@ -683,30 +767,34 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             // ---- O^T += V^T P^T
             if (!odd_values) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t x[2][2], y[2][2];
-                    v_codes<VT>(vr + 2 * t * SV::kStride, vr + (2 * t + 1) * SV::kStride, b, g, x);
-                    v_codes<VT>(vr + (2 * t + 8) * SV::kStride, vr + (2 * t + 9) * SV::kStride, b, g, y);
-                    uint2 ds = make_uint2(0u, 0u);
-                    if constexpr (kCodesV) ds = *reinterpret_cast<const uint2 *>(v16 + b * 16 + 4 * t);
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint8_t *v0 = vr + (16 * mt + 2 * t) * SV::kStride;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        uint32_t b0 = pb[nt][0], b1 = pb[nt][1];
-                        if constexpr (kCodesV) {
-                            b0 = mul_half2(b0, ds.x);
-                            b1 = mul_half2(b1, ds.y);
-                        }
+                    for (int b = 0; b < NB; ++b) {
+                        uint32_t x[2][2], y[2][2];
+                        v_codes<VT>(v0, v0 + SV::kStride, b, g, x);
+                        v_codes<VT>(v0 + 8 * SV::kStride, v0 + 9 * SV::kStride, b, g, y);
+                        uint2 ds = make_uint2(0u, 0u);
+                        if constexpr (kCodesV) ds = *reinterpret_cast<const uint2 *>(v16 + mt * kVTile + b * kVBlock + 4 * t);
 #pragma unroll
-                        for (int tile = 0; tile < 2; ++tile) {
-                            const uint32_t av[4] = {x[tile][0], x[tile][1], y[tile][0], y[tile][1]};
-                            mma_f16(o[nt][b][tile], av, b0, b1, o[nt][b][tile]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t b0 = pb[nt][mt][0], b1 = pb[nt][mt][1];
                             if constexpr (kCodesV) {
-                                // the constant -offset (times 16 in the high-nibble tile) * 2^-24
-                                constexpr uint32_t c0 = 0x8000u | SV::kOffset;
-                                constexpr uint32_t c1 = 0x8000u | (SV::kNibble ? 16 * SV::kOffset : SV::kOffset);
-                                const uint32_t cc = tile ? c1 * 0x10001u : c0 * 0x10001u;
-                                const uint32_t ac[4] = {cc, cc, cc, cc};
-                                mma_f16(o[nt][b][tile], ac, b0, b1, o[nt][b][tile]);
+                                b0 = mul_half2(b0, ds.x);
+                                b1 = mul_half2(b1, ds.y);
+                            }
+#pragma unroll
+                            for (int tile = 0; tile < 2; ++tile) {
+                                const uint32_t av[4] = {x[tile][0], x[tile][1], y[tile][0], y[tile][1]};
+                                mma_f16(o[nt][b][tile], av, b0, b1, o[nt][b][tile]);
+                                if constexpr (kCodesV) {
+                                    // the constant -offset (times 16 in the high-nibble tile) * 2^-24
+                                    constexpr uint32_t n0 = 0x8000u | SV::kOffset;
+                                    constexpr uint32_t n1 = 0x8000u | (SV::kNibble ? 16 * SV::kOffset : SV::kOffset);
+                                    const uint32_t cc = tile ? n1 * 0x10001u : n0 * 0x10001u;
+                                    const uint32_t ac[4] = {cc, cc, cc, cc};
+                                    mma_f16(o[nt][b][tile], ac, b0, b1, o[nt][b][tile]);
+                                }
                             }
                         }
                     }
@@ -714,32 +802,40 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             } else {
                 // values that are not finite: by the definition, p = 0 leaves them out
                 const float unit = kCodesV ? __uint_as_float(static_cast<uint32_t>(vexp - 24 + 127) << 23) : 1.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll 1
-                for (int k = 0; k < 16; ++k) {
-                    const uint8_t *row = vr + k * SV::kStride;
+                    for (int k = 0; k < 16; ++k) {
+                        const uint8_t *row = vr + (16 * mt + k) * SV::kStride;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const int from = (k & 7) * 4 + t;
-                        const float p0 = __shfl_sync(0xffffffffu, k < 8 ? pr[nt][0] : pr[nt][2], from);
-                        const float p1 = __shfl_sync(0xffffffffu, k < 8 ? pr[nt][1] : pr[nt][3], from);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const int from = (k & 7) * 4 + t;
+                            const float p0 = __shfl_sync(0xffffffffu, k < 8 ? s[nt][mt][0] : s[nt][mt][2], from);
+                            const float p1 = __shfl_sync(0xffffffffu, k < 8 ? s[nt][mt][1] : s[nt][mt][3], from);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
+                            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int tile = 0; tile < 2; ++tile)
+                                for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const float up = SV::kNibble && tile ? 16.0f : 1.0f;
-                                    const float v = row_value<VT>(row, v_dim<VT>(b, tile, h, g)) * unit * up;
-                                    if (p0 != 0.0f) o[nt][b][tile][2 * h] += p0 * v;
-                                    if (p1 != 0.0f) o[nt][b][tile][2 * h + 1] += p1 * v;
-                                }
+                                    for (int h = 0; h < 2; ++h) {
+                                        const float up = SV::kNibble && tile ? 16.0f : 1.0f;
+                                        const float v = row_value<VT>(row, v_dim<VT>(b, tile, h, g)) * unit * up;
+                                        if (p0 != 0.0f) o[nt][b][tile][2 * h] += p0 * v;
+                                        if (p1 != 0.0f) o[nt][b][tile][2 * h + 1] += p1 * v;
+                                    }
+                        }
                     }
-                }
+            }
+            __syncwarp();                     // ... and with its V rows
+            if (i + NS < n_steps) load(i + NS, kSideV, at);
+            cp_async_commit();
+            if (++stage_at == NS) {
+                stage_at = 0;
+                phase ^= 1u;
             }
         }
 
         // ---- the warps' results together
-        issued += n_steps;
         if (lost) l[0][0] = __int_as_float(0x7fc00000);       // no result rather than a wrong one
         cp_async_wait<0>();
         __syncthreads();
@@ -772,31 +868,50 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                     }
         }
         __syncthreads();
-        const bool starts = in0 == 0, ends = take == left;
-        const bool whole = starts && ends;
-        for (int x = tid; x < hg * static_cast<int>(rows) * D; x += kThreads) {
-            const int hr = x / D, d = x - hr * D, hs = hr / static_cast<int>(rows), r = hr - hs * static_cast<int>(rows);
-            float top = kNegInf;
-            for (int w = hs; w < W; w += hg) top = fmaxf(top, sm_m[w * R + r]);
-            const float ref = top == kNegInf ? 0.0f : top;
-            float sum = 0.0f, acc = 0.0f;
+        const bool starts = at0 == 0, ends = take == left, whole = starts && ends;
+        // a thread a (head, row): the warps' weights; then four dims a thread
+        if (tid < hg * R) {
+            const int hs = tid / R, row = tid % R;
+            float top = kNegInf, sum = 0.0f;
+            for (int w = hs; w < W; w += hg) top = fmaxf(top, sm_m[w * R + row]);
+            const float to = top == kNegInf ? 0.0f : top;
             for (int w = hs; w < W; w += hg) {
-                const float f = exp2_approx(sm_m[w * R + r] - ref);
-                sum += f * sm_l[w * R + r];
-                acc += f * sm_o[(w * R + r) * OS + d];
+                const float f = exp2_approx(sm_m[w * R + row] - to);
+                sum += f * sm_l[w * R + row];
+                sm_m[w * R + row] = f;
+            }
+            if (whole) {              // weights that already divide by the sum
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                for (int w = hs; w < W; w += hg) sm_m[w * R + row] *= inv;
+            } else {
+                float *part = attend_part<D, NT>(a, 2u * blockIdx.x + (starts ? 1u : 0u), hs);
+                part[row] = top;
+                part[R + row] = sum;
+            }
+        }
+        __syncthreads();
+        for (int x = tid; x < hg * R * (D / 4); x += kThreads) {
+            const int hr = x / (D / 4), d = (x % (D / 4)) * 4, hs = hr / R, row = hr % R;
+            if (row >= static_cast<int>(rows)) continue;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int w = hs; w < W; w += hg) {
+                const float f = sm_m[w * R + row];
+                const float4 y = *reinterpret_cast<const float4 *>(sm_o + (w * R + row) * OS + d);
+                acc.x += f * y.x;
+                acc.y += f * y.y;
+                acc.z += f * y.z;
+                acc.w += f * y.w;
             }
             if (!whole) {
-                float *part = attend_part<D, NT>(a, 2u * blockIdx.x + (starts ? 1u : 0u), hs);
-                if (d == 0) {
-                    part[r] = top;
-                    part[R + r] = sum;
-                }
-                part[2 * R + r * D + d] = acc;
+                *reinterpret_cast<float4 *>(attend_part<D, NT>(a, 2u * blockIdx.x + (starts ? 1u : 0u), hs) + 2 * R + row * D + d) = acc;
             } else {
-                const uint32_t rr = first + r, tok = rr / a.group;
-                store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(q.row0) + tok) * a.out.nb_tok +
-                            (static_cast<uint64_t>(head0 + hs) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim,
-                        sum == 0.0f ? 0.0f : acc / sum, a.out.bf16);
+                const uint32_t rr = first + row, tok = rr / a.group;
+                uint8_t *to = const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(q.row0) + tok) * a.out.nb_tok +
+                              (static_cast<uint64_t>(head0 + hs) * a.group + rr % a.group) * a.out.nb_head + d * a.out.nb_dim;
+                store16(to, acc.x, a.out.bf16);
+                store16(to + a.out.nb_dim, acc.y, a.out.bf16);
+                store16(to + 2 * a.out.nb_dim, acc.z, a.out.bf16);
+                store16(to + 3 * a.out.nb_dim, acc.w, a.out.bf16);
             }
         }
         if (starts && !ends && tid == 0) {

@@ -49,7 +49,7 @@ struct TileGeom {
     using K = Slice<KT, D>;
     using V = Slice<VT, D>;
     static constexpr int kOperand = kTileKeys * D * 2;             // one K or V tile
-    static constexpr int kRawK = kAttendStep * K::kStride, kRawV = kAttendStep * V::kStride;   // a warp's 16 keys
+    static constexpr int kRawK = kAttendBox * K::kStride, kRawV = kAttendBox * V::kStride;   // a warp's 16 keys
     static constexpr int kRoom = 218 * 1024 - 4 * kOperand;
     static constexpr int kFit = kRoom / (4 * (kRawK + kRawV));
     static constexpr int kStages = kFit > 6 ? 6 : kFit < 1 ? 1 : kFit;
@@ -805,10 +805,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     using S = decltype(slice_t);
                     constexpr int C = S::kBytes / 4;
 #pragma unroll 4
-                    for (int y = 0; y < (kAttendStep * C + 31) / 32; ++y) {
-                        const int x = lane + 32 * y, r = min(x / C, kAttendStep - 1), c = x - r * C;
+                    for (int y = 0; y < (kAttendBox * C + 31) / 32; ++y) {
+                        const int x = lane + 32 * y, r = min(x / C, kAttendBox - 1), c = x - r * C;
                         const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
-                        if (x < kAttendStep * C)
+                        if (x < kAttendBox * C)
                             cp_async4(smem_u32(st + r * S::kStride + c * 4), base + (cr >= 0 ? cr * row_bytes + c * 4 : 0ull), cr >= 0 ? 4u : 0u);
                     }
                 };
