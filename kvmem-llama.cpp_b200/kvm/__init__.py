@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -235,13 +236,12 @@ def lib():
             "kvm_stageout_item_bytes": (u64, [vp]),
             "kvm_select_groups": (C.c_int, [vp, vp, vp, vp, u32, vp, u32]),
             "kvm_stagein_packed": (C.c_int, [vp, vp, C.POINTER(PackedSource), C.POINTER(Window)]),
-            "kvm_map_batch": (C.c_int, [vp, C.POINTER(_BatchMap)]),
-            "kvm_qk_norm_rope": (C.c_int, [vp, u32, C.POINTER(Rows), C.POINTER(Rows), vp, vp, C.c_float,
-                                           vp, u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
-            "kvm_write_rows": (C.c_int, [vp, C.POINTER(_Cache), u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
-            "kvm_read_rows": (C.c_int, [vp, C.POINTER(_Cache), u32, vp, C.POINTER(Rows), C.POINTER(Rows)]),
-            "kvm_attend": (C.c_int, [vp, C.POINTER(_Cache), C.POINTER(_AttendBatch), C.POINTER(Rows),
-                                     C.POINTER(Rows), vp, u64]),
+            # structs by address (packed bytes or a ctypes.Structure)
+            "kvm_map_batch": (C.c_int, [vp, vp]),
+            "kvm_qk_norm_rope": (C.c_int, [vp, u32, vp, vp, vp, vp, C.c_float, vp, u32, vp, vp, vp]),
+            "kvm_write_rows": (C.c_int, [vp, vp, u32, vp, vp, vp]),
+            "kvm_read_rows": (C.c_int, [vp, vp, u32, vp, vp, vp]),
+            "kvm_attend": (C.c_int, [vp, vp, vp, vp, vp, vp, u64]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -311,7 +311,7 @@ def _bad(what):
 
 
 def _layer_check(st):
-    if st != KVM_OK:
+    if st:
         raise KvmError(st, lib().kvm_last_error(None).decode())
 
 
@@ -346,21 +346,28 @@ def _layer_stream(stream, dev):
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+# The calls' argument structs, packed: a ctypes.Structure takes several times as
+# long to fill.  The layouts are those of Rows, _BatchMap and _AttendBatch.
+_PACK_ROWS = struct.Struct("=QiIIIQQQ").pack
+_PACK_MAP = struct.Struct("=QQQQQIIIIIIQQQQQQ").pack
+_PACK_ATTEND = struct.Struct("=QQIIQQIIIf").pack
+
+
 def _act(t, what, dev):
-    """kvm_rows of [rows, heads, head_dim], any strides."""
+    """kvm_rows of [rows, heads, head_dim], any strides, and its shape."""
     ty = _Torch.rows.get(t.dtype)
     if ty is None or t.dim() != 3 or t.get_device() != dev:
         _bad(f"{what}: float32, float16 or bfloat16 [rows, heads, head_dim] on cuda:{dev}, "
              f"not {t.dtype} {tuple(t.shape)} on {t.device}")
     es = ty[1]
-    _, heads, dim = t.shape
+    shape = t.shape
     st, sh, sd = t.stride()
-    return Rows(t.data_ptr(), ty[0], heads, dim, 0, sd * es, sh * es, st * es)
+    return _PACK_ROWS(t.data_ptr(), ty[0], shape[1], shape[2], 0, sd * es, sh * es, st * es), shape
 
 
 def _index(t, dtype, n, what, dev):
     """Address of a contiguous vector of at least n entries."""
-    if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev or t.shape[0] < n:
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
         _bad(f"{what}: a contiguous {dtype} vector of at least {n} on cuda:{dev}, "
              f"not {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -385,14 +392,15 @@ class Cache(_Cache):
     the contiguous tensors k and v."""
 
     def __init__(self, k, v, type_k, type_v, n_head_kv, head_dim, block_tokens, n_slots):
-        self.device = _device(k, "cache k")
+        self.device = dev = _device(k, "cache k")
         cells, width = block_tokens * n_slots, n_head_kv * head_dim
-        for t, ty, what in ((k, type_k, "k"), (v, type_v, "v")):
-            if ty not in _BLOCK_BYTES or width <= 0 or width % 32 or cells <= 0:
-                _bad(f"cache {what}: F16, Q8_0, Q5_0 or Q4_0 rows of blocks of 32, at least one cell")
-            want = cells * (width // 32 * _BLOCK_BYTES[ty])
-            if not t.is_contiguous() or t.get_device() != self.device or t.numel() * t.element_size() < want:
-                _bad(f"cache {what}: a contiguous tensor of at least {want} bytes on cuda:{self.device}")
+        bk, bv = _BLOCK_BYTES.get(type_k), _BLOCK_BYTES.get(type_v)
+        if bk is None or bv is None or width <= 0 or width & 31 or cells <= 0:
+            _bad("cache: F16, Q8_0, Q5_0 or Q4_0 rows of blocks of 32, at least one cell")
+        for t, size, what in ((k, bk, "k"), (v, bv, "v")):
+            want = cells * (width // 32 * size)
+            if t.get_device() != dev or not t.is_contiguous() or t.numel() * t.element_size() < want:
+                _bad(f"cache {what}: a contiguous tensor of at least {want} bytes on cuda:{dev}")
         super().__init__(k.data_ptr(), v.data_ptr(), type_k, type_v, n_head_kv, head_dim, block_tokens, n_slots)
         self.tensors = (k, v)
 
@@ -403,14 +411,14 @@ def map_batch(past, new, free_slots, block_tokens, table, q_start, kv_len, cells
     updated; out: q_start int32 [n+1], kv_len int32 [n], cells int64 [rows], pos
     and seq int32 [rows], info int32 [4]."""
     dev = _device(past, "past")
-    i32, n, rows = _Torch.i32, past.shape[0], cells.shape[0]
+    i32, n, rows = _Torch.i32, past.numel(), cells.numel()
     tab, stride, cols = _table(table, n, dev)
-    m = _BatchMap(_index(past, i32, n, "past", dev), _index(new, i32, n, "new", dev),
-                  _index(free_slots, i32, 0, "free_slots", dev), tab, stride, cols, n, free_slots.shape[0], block_tokens,
+    m = _PACK_MAP(_index(past, i32, n, "past", dev), _index(new, i32, n, "new", dev),
+                  _index(free_slots, i32, 0, "free_slots", dev), tab, stride, cols, n, free_slots.numel(), block_tokens,
                   rows, 0, _index(q_start, i32, n + 1, "q_start", dev), _index(kv_len, i32, n, "kv_len", dev),
                   _index(cells, _Torch.i64, rows, "cells", dev), _index(pos, i32, rows, "pos", dev),
                   _index(seq, i32, rows, "seq", dev), _index(info, i32, 4, "info", dev))
-    _layer_check(lib().kvm_map_batch(_layer_stream(stream, dev), C.byref(m)))
+    _layer_check(lib().kvm_map_batch(_layer_stream(stream, dev), m))
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, eps, freqs, pos, q_out, k_out, stream=None):
@@ -419,31 +427,40 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps, freqs, pos, q_out, k_out, stream
     float32 [head_dim] or None; freqs float32 [n_rot / 2] or None; k and k_out
     may be None."""
     dev = _device(q, "q")
-    n, _, d = q.shape
-    a, ao = _act(q, "q", dev), _act(q_out, "q_out", dev)
-    if q_out.shape != q.shape:
+    a, shape = _act(q, "q", dev)
+    ao, out_shape = _act(q_out, "q_out", dev)
+    n, _, d = shape
+    if out_shape != shape:
         _bad("q_out: shape of q")
     b = bo = None
     if k is not None or k_out is not None:
-        if k is None or k_out is None or k_out.shape != k.shape or k.shape[0] != n:
+        if k is None or k_out is None:
+            _bad("k and k_out go together")
+        b, shape = _act(k, "k", dev)
+        bo, out_shape = _act(k_out, "k_out", dev)
+        if out_shape != shape or shape[0] != n:
             _bad("k and k_out: [rows of q, heads, head_dim]")
-        b, bo = C.byref(_act(k, "k", dev)), C.byref(_act(k_out, "k_out", dev))
-    f32, half = _Torch.f32, 0 if freqs is None else freqs.shape[0]
+    f32, half = _Torch.f32, 0 if freqs is None else freqs.numel()
     _layer_check(lib().kvm_qk_norm_rope(
-        _layer_stream(stream, dev), n, C.byref(a), b,
+        _layer_stream(stream, dev), n, a, b,
         None if q_weight is None else _index(q_weight, f32, d, "q_weight", dev),
         None if k_weight is None else _index(k_weight, f32, d, "k_weight", dev), eps,
         None if freqs is None else _index(freqs, f32, half, "freqs", dev), 2 * half,
-        None if pos is None else _index(pos, _Torch.i32, n, "pos", dev), C.byref(ao), bo))
+        None if pos is None else _index(pos, _Torch.i32, n, "pos", dev), ao, bo))
 
 
 def _rows_call(fn, cache, cells, k, v, stream):
-    dev, n = cache.device, cells.shape[0]
-    if (k is not None and k.shape[0] != n) or (v is not None and v.shape[0] != n):
-        _bad("k and v: one row a cell")
-    _layer_check(fn(_layer_stream(stream, dev), C.byref(cache), n, _index(cells, _Torch.i64, n, "cells", dev),
-                    None if k is None else C.byref(_act(k, "k", dev)),
-                    None if v is None else C.byref(_act(v, "v", dev))))
+    dev, n = cache.device, cells.numel()
+    a = b = None
+    if k is not None:
+        a, shape = _act(k, "k", dev)
+        if shape[0] != n:
+            _bad("k: one row a cell")
+    if v is not None:
+        b, shape = _act(v, "v", dev)
+        if shape[0] != n:
+            _bad("v: one row a cell")
+    _layer_check(fn(_layer_stream(stream, dev), C.byref(cache), n, _index(cells, _Torch.i64, n, "cells", dev), a, b))
 
 
 def write_rows(cache, cells, k, v, stream=None):
@@ -463,17 +480,18 @@ def attend(cache, q, q_start, kv_len, table, out, work, scale, causal=True, max_
     q_start int32 [n+1], kv_len int32 [n], table int32 [n, blocks]; work: a
     tensor of ATTEND_WORK_BYTES for this call alone while it runs; max_new: the
     most rows of a request, as far as the caller knows."""
-    dev, n = cache.device, kv_len.shape[0]
-    a, b = _act(q, "q", dev), _act(out, "out", dev)
-    if out.shape != q.shape:
+    dev, n = cache.device, kv_len.numel()
+    a, shape = _act(q, "q", dev)
+    b, out_shape = _act(out, "out", dev)
+    if out_shape != shape:
         _bad("out: shape of q")
     if work.get_device() != dev or not work.is_contiguous():
         _bad(f"work: a contiguous tensor on cuda:{dev}")
     tab, stride, cols = _table(table, n, dev)
     i32 = _Torch.i32
-    batch = _AttendBatch(tab, stride, cols, n, _index(q_start, i32, n + 1, "q_start", dev),
-                         _index(kv_len, i32, n, "kv_len", dev), q.shape[0], max_new, ATTEND_CAUSAL if causal else 0, scale)
-    _layer_check(lib().kvm_attend(_layer_stream(stream, dev), C.byref(cache), C.byref(batch), C.byref(a), C.byref(b),
+    batch = _PACK_ATTEND(tab, stride, cols, n, _index(q_start, i32, n + 1, "q_start", dev),
+                         _index(kv_len, i32, n, "kv_len", dev), shape[0], max_new, ATTEND_CAUSAL if causal else 0, scale)
+    _layer_check(lib().kvm_attend(_layer_stream(stream, dev), C.byref(cache), batch, a, b,
                                   work.data_ptr(), work.numel() * work.element_size()))
 
 

@@ -118,6 +118,16 @@ def test_calls_with_no_rows_do_nothing():
         assert fn(None, C.byref(cache()), 0, None, C.byref(rows(2)), None) == kvm.KVM_OK
 
 
+def test_packed_structs_match_ctypes():
+    """The binding packs its structs by format strings: the same bytes as ctypes'."""
+    r = (0x1122334455667788, 30, 7, 128, 0, 2, 256, 1 << 40)
+    assert kvm._PACK_ROWS(*r) == bytes(kvm.Rows(*r))
+    m = tuple(range(3, 20))
+    assert kvm._PACK_MAP(*m) == bytes(kvm._BatchMap(*m))
+    b = (1, 2, 3, 4, 5, 6, 7, 8, 9, 0.25)
+    assert kvm._PACK_ATTEND(*b) == bytes(kvm._AttendBatch(*b))
+
+
 def test_struct_layouts_match_c(tmp_path):
     import os
     import subprocess
