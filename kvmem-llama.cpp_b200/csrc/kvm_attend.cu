@@ -12,7 +12,7 @@ cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t gr
 template <int D, int KT>
 cudaError_t launch_attend_tile(const AttendArgs &a, int vt, uint32_t grid, cudaStream_t st);
 
-bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes) {
+bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes, uint32_t box_rows) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -29,7 +29,7 @@ bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const At
     if (!encode) return false;
     const cuuint64_t dims[2] = {row_bytes / 4u, static_cast<uint64_t>(a.n_slots) * a.block_tokens};
     const cuuint64_t strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_bytes / 4u, kAttendBox}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {box_bytes / 4u, box_rows}, step[2] = {1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

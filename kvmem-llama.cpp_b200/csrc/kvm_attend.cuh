@@ -48,9 +48,9 @@ struct AttendArgs {
     CUtensorMap map_k, map_v;      // [cells][row bytes / 4] of 32-bit words
 };
 
-// Tensor map of one side of the cache: rows of 32-bit words, boxes of a step's
-// 16 rows by box_bytes.  False when the driver cannot make it.
-bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes);
+// Tensor map of one side of the cache: rows of 32-bit words, boxes of
+// box_rows rows by box_bytes.  False when the driver cannot make it.
+bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes, uint32_t box_rows);
 
 // A sequence as the kernels see it; nothing read from device memory is trusted
 // to stay inside the tables.

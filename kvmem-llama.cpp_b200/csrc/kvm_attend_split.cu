@@ -16,7 +16,7 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
     static_assert(smem <= 227 * 1024, "shared memory");
     if (!attr_once(attr, reinterpret_cast<const void *>(attend_split_kernel<D, KT, VT, NT>), smem))
         return cudaErrorInvalidValue;
-    if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride)))
+    if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride, kAttendBox) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride, kAttendBox)))
         a.tma = 0;
     const uint64_t slot = static_cast<uint64_t>(a.heads_cta) * attend_part_floats<D, NT>() * 4u;
     grid = static_cast<uint32_t>(std::min<uint64_t>(grid, (KVM_ATTEND_WORK_BYTES - kAttendMaxCtas * kAttendDescBytes) / (2 * slot)));

@@ -71,7 +71,7 @@ struct SplitGeom {
 };
 
 // a / b, by a 32-bit division where a allows it (the 64-bit routine is ten times as long)
-__device__ __forceinline__ unsigned long long div_small(unsigned long long a, uint32_t b) {
+__host__ __device__ __forceinline__ unsigned long long div_small(unsigned long long a, uint32_t b) {
     return (a >> 32) == 0 ? static_cast<uint32_t>(a) / b : a / b;
 }
 

@@ -13,7 +13,7 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
     static std::atomic<uint64_t> attr{0};
     static_assert(G::kSmem <= 227 * 1024, "shared memory");
     if (!attr_once(attr, reinterpret_cast<const void *>(attend_tile_kernel<D, KT, VT>), G::kSmem)) return cudaErrorInvalidValue;
-    if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride)))
+    if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride, kAttendBox) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride, kAttendBox)))
         a.tma = 0;
     grid = std::min<uint32_t>(grid, (KVM_ATTEND_WORK_BYTES - kAttendMaxCtas * kAttendDescBytes) / (2u * tile_part_bytes<D>()));
     attend_tile_kernel<D, KT, VT><<<grid, kTileThreads, G::kSmem, st>>>(a);

@@ -144,7 +144,8 @@ __host__ __device__ __forceinline__ TileSeq tile_seq(const AttendArgs &a, uint32
 
 // Key tiles of row tile i: those its last row sees, at least one.
 __host__ __device__ __forceinline__ int64_t tile_steps(const AttendArgs &a, const TileSeq &t, int64_t i) {
-    const int64_t last = min(((i + 1) * kTileRows - 1) / static_cast<int64_t>(a.group), static_cast<int64_t>(t.q.n_new) - 1);
+    // rows of a sequence number less than 2^31
+    const int64_t last = min(static_cast<int64_t>((static_cast<uint32_t>(i + 1) * kTileRows - 1u) / a.group), static_cast<int64_t>(t.q.n_new) - 1);
     const int64_t keys = attend_limit(a, t.q, static_cast<int32_t>(last));
     return max(static_cast<int64_t>(1), (keys + kTileKeys - 1) / kTileKeys);
 }
@@ -156,6 +157,7 @@ __host__ __device__ __forceinline__ int64_t tile_steps(const AttendArgs &a, cons
 __host__ __device__ inline int64_t tile_prefix(const AttendArgs &a, const TileSeq &t, int64_t n) {
     const int64_t most = max(static_cast<int64_t>(1), (t.cap + kTileKeys - 1) / kTileKeys);
     if (!a.causal) return n * most;
+    if (n <= 1) return n ? tile_steps(a, t, 0) : 0;
     const int64_t g = a.group, shift = t.q.shift;
     auto first_with = [&](int64_t keys) -> int64_t {      // first tile whose last row sees at least `keys`, unclamped
         const int64_t need = g * (keys - shift - 1) - (kTileRows - 1);    // 128 i >= need
@@ -200,7 +202,7 @@ struct TileWalk {
         tile = lo;
         steps = tile_steps(a, t, tile);
         off -= heads * tile_prefix(a, t, lo);
-        head = off / steps;
+        head = static_cast<int64_t>(div_small(static_cast<unsigned long long>(off), static_cast<uint32_t>(steps)));
         in0 = off - head * steps;
     }
 
@@ -463,11 +465,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         __syncthreads();
         return x + before;
     };
+    const bool once = a.n_seq <= kTileThreads;
     unsigned long long mine = 0, total = 0;
     for (uint32_t s = tid; s < a.n_seq; s += kTileThreads) mine += units(s);
-    scan(mine, &total);
-    unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share == 0) share = 1;
+    const unsigned long long upto = scan(mine, &total);
+    const unsigned long long share = max(1ull, div_small(total + gridDim.x - 1, gridDim.x));
     const unsigned long long u0 = share * blockIdx.x, u1 = min(u0 + share, total);
     AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
     if (u0 >= total) {
@@ -477,8 +479,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
     unsigned long long carry = 0;
     for (uint32_t base = 0; base < a.n_seq; base += kTileThreads) {
         const uint32_t s = base + tid;
-        unsigned long long all;
-        const unsigned long long n = s < a.n_seq ? units(s) : 0ull, x = carry + scan(n, &all);
+        unsigned long long n = mine, x = upto, all = total;
+        if (!once) {
+            n = s < a.n_seq ? units(s) : 0ull;
+            x = carry + scan(n, &all);
+        }
         if (n != 0 && x - n <= u0 && u0 < x) {
             s_seq = s;
             s_off = u0 - (x - n);
@@ -512,6 +517,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
     bool lost = false;                         // a bounded wait ran out: go on without waiting
     auto wait = [&](uint64_t *bar, uint32_t phase) {
         if (!lost && !mbar_wait_near(bar, phase & 1u)) lost = true;
+        // together: a lane that went ahead could let the phase after this one complete
+        // while another still polls for this one
+        __syncwarp();
     };
     uint32_t j = 0;                            // running key tile of the CTA: stage j & 1, phase j >> 1
 
@@ -535,64 +543,57 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             const uint64_t at_tok = static_cast<uint64_t>(p.q.row0) + tok, at_head = static_cast<uint64_t>(p.head) * a.group + rr % a.group;
             const uint8_t *qp = a.q.p + at_tok * a.q.nb_tok + at_head * a.q.nb_head;
             const int32_t lim = in ? attend_limit(a, p.q, static_cast<int32_t>(tok)) : p.kend;
-            // the row's largest element to [2^14, 2^15)
-            float top = 0.0f;
-#pragma unroll 4
-            for (int c = wg * (D / 16); c < (wg + 1) * (D / 16); ++c) {
-                uint32_t u[4];
+            // this thread's half of the row, all of it in flight at once; a piece without
+            // key tiles issues no products and leaves Q alone
+            constexpr int kWords = D / 4;              // of two values
+            const bool work = p.in0 < p.in1;
+            float fac = 0.0f;
+            if (work) {
+                uint32_t u[kWords];
                 if (a.q_vec) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * c);
-                    u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+#pragma unroll
+                    for (int c = 0; c < kWords / 4; ++c) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(qp + wg * D + 16 * c);
+                        u[4 * c] = v.x; u[4 * c + 1] = v.y; u[4 * c + 2] = v.z; u[4 * c + 3] = v.w;
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        u[i] = *reinterpret_cast<const uint16_t *>(qp + (8 * c + 2 * i) * a.q.nb_dim) |
-                               static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(qp + (8 * c + 2 * i + 1) * a.q.nb_dim)) << 16;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = a.q.bf16 ? __uint_as_float(u[i] << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] & 0xffffu)));
-                    const float y = a.q.bf16 ? __uint_as_float(u[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] >> 16)));
-                    top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
-                }
-            }
-            top = fmaxf(top, swap(top));
-            const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
-            // the sum of D products must stay in F32: a top of 2^14 leaves 2^98 for K
-            const int up = (top > 0.0f && e < 128) ? max(-126, min(126, 14 - e)) : 0;
-            const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
-            const float mul = sign * __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-            // not 0: a hidden key's -inf has to stay -inf
-            const float fac = fmaxf(fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
-            // a piece without key tiles issues no products and leaves Q alone
-#pragma unroll 1
-            for (int c0 = wg * (D / 64); c0 < (p.in0 < p.in1 ? (wg + 1) * (D / 64) : 0); ++c0) {       // 32 dims = 16 columns at a time
-                uint32_t w[16];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[8];
-                    if (a.q_vec) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(qp + 16 * (4 * c0 + c));
-                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[2 * i] = a.q.bf16 ? __uint_as_float(u[i] << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] & 0xffffu)));
-                            x[2 * i + 1] = a.q.bf16 ? __uint_as_float(u[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<uint16_t>(u[i] >> 16)));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = load16(qp + (32 * c0 + 8 * c + i) * a.q.nb_dim, a.q.bf16);
+                    for (int c = 0; c < kWords; ++c) {
+                        const uint8_t *e = qp + (wg * (D / 2) + 2 * c) * a.q.nb_dim;
+                        u[c] = *reinterpret_cast<const uint16_t *>(e) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(e + a.q.nb_dim)) << 16;
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[4 * c + i] = in ? pack_half2(x[tile_order<KT>(2 * i)] * mul, x[tile_order<KT>(2 * i + 1)] * mul) : 0u;
                 }
-                tc_st16(lanes + kColQ + 16 * c0, w);
+                auto value = [&](int i) -> float {     // value i of the half row
+                    const uint32_t w = u[i >> 1];
+                    if (a.q.bf16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+                    return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? w >> 16 : w & 0xffffu)));
+                };
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 2 * kWords; ++i) top = fmaxf(top, fabsf(value(i)));
+                // the row's largest element to [2^14, 2^15): the sum of D products stays in
+                // F32, 2^98 are left for K
+                top = fmaxf(top, swap(top));
+                const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
+                const int up = (top > 0.0f && e < 128) ? max(-126, min(126, 14 - e)) : 0;
+                const float mul = (a.scale_log2 < 0.0f ? -1.0f : 1.0f) * __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+                // not 0: a hidden key's -inf has to stay -inf
+                fac = fmaxf(fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+#pragma unroll
+                for (int c0 = 0; c0 < D / 64; ++c0) {  // 32 dims = 16 columns at a time
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = 32 * c0 + 8 * (i / 4), x = 2 * (i % 4);
+                        w[i] = in ? pack_half2(value(at + tile_order<KT>(x)) * mul, value(at + tile_order<KT>(x + 1)) * mul) : 0u;
+                    }
+                    tc_st16(lanes + kColQ + wg * (D / 4) + 16 * c0, w);
+                }
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0 && p.in0 < p.in1) mbar_arrive(q_full);
+            if (lane == 0 && work) mbar_arrive(q_full);
 
             float m = kNegInf, l = 0.0f;
             const uint32_t j0 = j;
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 reinterpret_cast<float *>(part)[kTileRows + row] = l;
             }
 #pragma unroll 1
-            for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {
+            for (int c = wg * (D / 64); c < (static_cast<uint32_t>(warp & 3) * 32u < p.rows ? (wg + 1) * (D / 64) : 0); ++c) {
                 uint32_t o[32];
                 if (any) {
                     tc_ld32(o, lanes + kColO + 32 * c);
@@ -704,13 +705,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                         }
                     }
                 }
-                if (part) {
+                if (part && in) {
                     uint4 *to = reinterpret_cast<uint4 *>(part + 8 * kTileRows + (row * D + 32 * c) * 2);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         to[k] = make_uint4(pack_half2(y[8 * k], y[8 * k + 1]), pack_half2(y[8 * k + 2], y[8 * k + 3]),
                                            pack_half2(y[8 * k + 4], y[8 * k + 5]), pack_half2(y[8 * k + 6], y[8 * k + 7]));
-                } else if (in) {
+                } else if (!part && in) {
                     if (a.out_vec) {
                         uint4 *to = reinterpret_cast<uint4 *>(op + 64 * c);
 #pragma unroll
