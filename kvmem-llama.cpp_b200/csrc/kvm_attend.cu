@@ -10,7 +10,7 @@ namespace kvm {
 template <int D, int KT>
 cudaError_t launch_attend_split(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st);
 template <int D, int KT>
-cudaError_t launch_attend_tile(const AttendArgs &a, int vt, uint32_t grid, cudaStream_t st);
+cudaError_t launch_attend_tile(const AttendArgs &a, int vt, bool pair, uint32_t grid, cudaStream_t st);
 
 bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes, uint32_t box_rows) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -37,10 +37,11 @@ bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const At
 
 namespace {
 
-// One of the two kernels: split with row tiles of 8 * nt rows, or (nt = 0) tile.
+// One of the kernels: split with row tiles of 8 * nt rows, or tile by single CTAs
+// (nt = 0) or by pairs (-1).
 template <int D, int KT>
 cudaError_t launch_kt(const AttendArgs &a, int vt, int nt, uint32_t grid, cudaStream_t st) {
-    return nt ? launch_attend_split<D, KT>(a, vt, nt, grid, st) : launch_attend_tile<D, KT>(a, vt, grid, st);
+    return nt > 0 ? launch_attend_split<D, KT>(a, vt, nt, grid, st) : launch_attend_tile<D, KT>(a, vt, nt < 0, grid, st);
 }
 
 template <int D>
@@ -139,7 +140,8 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     auto launch = [&](int nt, uint32_t min_rows, uint32_t max_rows) {
         a.min_rows = min_rows;
         a.max_rows = max_rows;
-        const uint32_t grid = nt ? ctas(8u * nt, 16u, a.heads_cta) : ctas(128, 64, 1);
+        const uint32_t grid = nt > 0 ? ctas(8u * nt, 16u, a.heads_cta) : nt == 0 ? ctas(128, 64, 1) :
+                                                                                 static_cast<uint32_t>(std::min<uint64_t>(2u * ctas(256, 128, 1), sms & ~1ull));
         if (D == 64u) return launch_d<64>(a, c->type_k, c->type_v, nt, grid, st);
         if (D == 128u) return launch_d<128>(a, c->type_k, c->type_v, nt, grid, st);
         return launch_d<256>(a, c->type_k, c->type_v, nt, grid, st);
@@ -154,10 +156,10 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     if (most <= 16u) {
         e = launch(most <= 8u ? 1 : 2, 1, 0xffffffffu);
     } else if (b->n_seq == 1 || (most <= 128u && static_cast<uint64_t>(b->n_rows) * a.group > 8ull * b->n_seq)) {
-        e = launch(0, 1, 0xffffffffu);
+        e = launch(most > 128u ? -1 : 0, 1, 0xffffffffu);
     } else {
         e = launch(2, 1, 16);
-        if (e == cudaSuccess) e = launch(0, 17, 0xffffffffu);
+        if (e == cudaSuccess) e = launch(most > 128u ? -1 : 0, 17, 0xffffffffu);
     }
     return layer_cuda(e, me);
 }

@@ -42,18 +42,22 @@
 
 namespace kvm {
 
-constexpr int kTileRows = 128, kTileKeys = 64, kTileThreads = 17 * 32;
+constexpr int kTileRows = 128, kTileThreads = 17 * 32;      // rows of a CTA
 
-template <int D, int KT, int VT>
+template <int D, int KT, int VT, bool PAIR>
 struct TileGeom {
+    static constexpr int kRows = PAIR ? 256 : 128, kKeys = PAIR ? 128 : 64;      // an item's rows, a key tile
     using K = Slice<KT, D>;
-    using V = Slice<VT, D>;
-    static constexpr int kOperand = kTileKeys * D * 2;             // one K or V tile
-    static constexpr int kRawK = kAttendBox * K::kStride, kRawV = kAttendBox * V::kStride;   // a warp's 16 keys
-    static constexpr int kRoom = 218 * 1024 - 4 * kOperand;
+    using V = Slice<VT, PAIR ? D / 2 : D>;                         // the dims of V that a CTA dequantizes
+    static constexpr int kSlices = PAIR ? 2 : 1;                   // V slices a head
+    static constexpr int kBoxesV = PAIR ? 2 : 1;                   // 16-key boxes of V a warp and tile
+    static constexpr int kOperand = 64 * D * 2;                    // a CTA's part of one K or V tile
+    static constexpr int kQ = PAIR ? kTileRows * D * 2 : 0;        // Q in shared memory (else TMEM)
+    static constexpr int kRawK = kAttendBox * K::kStride, kRawV = kBoxesV * kAttendBox * V::kStride;   // a warp's rows of a tile
+    static constexpr int kRoom = 218 * 1024 - 4 * kOperand - kQ;
     static constexpr int kFit = kRoom / (4 * (kRawK + kRawV));
     static constexpr int kStages = kFit > 6 ? 6 : kFit < 1 ? 1 : kFit;
-    static constexpr int kRaw = 4 * kOperand;                      // offset of the raw rings
+    static constexpr int kRaw = 4 * kOperand + kQ;                 // offset of the raw rings
     static constexpr int kBars = kRaw + 4 * kStages * (kRawK + kRawV);
     static constexpr int kSmem = kBars + 1024 + 1024;              // barriers; alignment of the operand tiles
 };
@@ -71,6 +75,66 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
         : "memory");
+}
+// The same by a CTA pair: 256 rows, this CTA's and its peer's; A from TMEM or, with
+// an operand descriptor, from shared memory (the same offsets in both CTAs).
+__device__ __forceinline__ void tc_mma_pair(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+// Arrives on the barrier of both CTAs when the products issued so far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+// Arrives on the barrier at the same offset in CTA `rank` of the cluster.
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}"
+        ::"r"(smem_u32(bar)), "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ void st_shared_at(uint32_t *p, uint32_t v, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tst.shared::cluster.u32 [ra], %1;\n\t}"
+        ::"r"(smem_u32(p)), "r"(v), "r"(rank)
+        : "memory");
+}
+// Bounded wait with cluster-scope acquire (arrivals come from both CTAs).
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((i & 1023u) == 1023u) {
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > kWaitLimitNs) return false;
+        }
+    }
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tc_ld32(uint32_t (&r)[32], uint32_t addr) {
     asm volatile(
@@ -104,9 +168,9 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_
     return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | static_cast<uint64_t>((lbo >> 4) & 0x3fffu) << 16 |
            static_cast<uint64_t>((sbo >> 4) & 0x3fffu) << 32 | 1ull << 46 | 2ull << 61;
 }
-// Instruction descriptor: F16 x F16 -> F32, M = 128.
-constexpr uint32_t tc_idesc(int n, bool b_mn_major) {
-    return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | static_cast<uint32_t>(n / 8) << 17 | (128u / 16) << 24;
+// Instruction descriptor: F16 x F16 -> F32.
+constexpr uint32_t tc_idesc(int m, int n, bool b_mn_major) {
+    return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | static_cast<uint32_t>(n / 8) << 17 | static_cast<uint32_t>(m / 16) << 24;
 }
 
 // ------------------------------------------------------------- work line --
@@ -133,41 +197,44 @@ struct TileSeq {
     int64_t cap;         // keys its last row sees
 };
 
+template <int ROWS>
 __host__ __device__ __forceinline__ TileSeq tile_seq(const AttendArgs &a, uint32_t s) {
     TileSeq t;
     t.q = attend_seq(a, s);
     const int64_t rows = static_cast<int64_t>(t.q.n_new) * a.group;
-    t.tiles = (t.q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) ? 0 : (rows + kTileRows - 1) / kTileRows;
+    t.tiles = (t.q.n_new <= 0 || rows < a.min_rows || rows > a.max_rows) ? 0 : (rows + ROWS - 1) / ROWS;
     t.cap = t.q.n_new > 0 ? attend_limit(a, t.q, t.q.n_new - 1) : 0;
     return t;
 }
 
 // Key tiles of row tile i: those its last row sees, at least one.
+template <int ROWS, int KEYS>
 __host__ __device__ __forceinline__ int64_t tile_steps(const AttendArgs &a, const TileSeq &t, int64_t i) {
     // rows of a sequence number less than 2^31
-    const int64_t last = min(static_cast<int64_t>((static_cast<uint32_t>(i + 1) * kTileRows - 1u) / a.group), static_cast<int64_t>(t.q.n_new) - 1);
+    const int64_t last = min(static_cast<int64_t>((static_cast<uint32_t>(i + 1) * ROWS - 1u) / a.group), static_cast<int64_t>(t.q.n_new) - 1);
     const int64_t keys = attend_limit(a, t.q, static_cast<int32_t>(last));
-    return max(static_cast<int64_t>(1), (keys + kTileKeys - 1) / kTileKeys);
+    return max(static_cast<int64_t>(1), (keys + KEYS - 1) / KEYS);
 }
 
 // Key tiles of the first n row tiles.  Row tile i's last token is
-// floor((128 i + 127) / group) (the sequence's last for the last tile), so its
-// count is floor((group (shift + 64) + 128 i + 127) / (64 group)) between the
+// floor((ROWS (i + 1) - 1) / group) (the sequence's last for the last tile), so its
+// count is floor((group (shift + KEYS) + ROWS (i + 1) - 1) / (KEYS group)) between the
 // tiles that need one key tile and those that see `cap` keys.
+template <int ROWS, int KEYS>
 __host__ __device__ inline int64_t tile_prefix(const AttendArgs &a, const TileSeq &t, int64_t n) {
-    const int64_t most = max(static_cast<int64_t>(1), (t.cap + kTileKeys - 1) / kTileKeys);
+    const int64_t most = max(static_cast<int64_t>(1), (t.cap + KEYS - 1) / KEYS);
     if (!a.causal) return n * most;
-    if (n <= 1) return n ? tile_steps(a, t, 0) : 0;
+    if (n <= 1) return n ? tile_steps<ROWS, KEYS>(a, t, 0) : 0;
     const int64_t g = a.group, shift = t.q.shift;
     auto first_with = [&](int64_t keys) -> int64_t {      // first tile whose last row sees at least `keys`, unclamped
-        const int64_t need = g * (keys - shift - 1) - (kTileRows - 1);    // 128 i >= need
-        const int64_t i = need <= 0 ? 0 : (need + kTileRows - 1) / kTileRows;
+        const int64_t need = g * (keys - shift - 1) - (ROWS - 1);    // ROWS i >= need
+        const int64_t i = need <= 0 ? 0 : (need + ROWS - 1) / ROWS;
         return i < n ? i : n;
     };
-    const int64_t ones = first_with(kTileKeys + 1), full = max(ones, first_with(t.cap));
+    const int64_t ones = first_with(KEYS + 1), full = max(ones, first_with(t.cap));
     int64_t sum = ones + (n - full) * most;
     if (full > ones)
-        sum += floor_sum(full - ones, kTileKeys * g, kTileRows, g * (shift + kTileKeys) + kTileRows * ones + kTileRows - 1);
+        sum += floor_sum(full - ones, KEYS * g, ROWS, g * (shift + KEYS) + ROWS * ones + ROWS - 1);
     return sum;
 }
 
@@ -182,6 +249,7 @@ struct TilePiece {
 };
 
 // Walks the pieces of a CTA; every thread of the CTA runs it alike.
+template <int ROWS, int KEYS>
 struct TileWalk {
     uint64_t pos, u1, share;
     uint32_t seq;
@@ -191,17 +259,17 @@ struct TileWalk {
     // Position `off` of sequence s's items.
     __host__ __device__ __forceinline__ void seek(const AttendArgs &a, uint32_t s, int64_t off) {
         seq = s;
-        t = tile_seq(a, s);
+        t = tile_seq<ROWS>(a, s);
         const int64_t heads = a.n_head_kv;
         int64_t lo = 0, hi = t.tiles;    // the last tile whose items start at or before off
         while (hi - lo > 1) {
             const int64_t mid = (lo + hi) / 2;
-            if (heads * tile_prefix(a, t, mid) <= off) lo = mid;
+            if (heads * tile_prefix<ROWS, KEYS>(a, t, mid) <= off) lo = mid;
             else hi = mid;
         }
         tile = lo;
-        steps = tile_steps(a, t, tile);
-        off -= heads * tile_prefix(a, t, lo);
+        steps = tile_steps<ROWS, KEYS>(a, t, tile);
+        off -= heads * tile_prefix<ROWS, KEYS>(a, t, lo);
         head = static_cast<int64_t>(div_small(static_cast<unsigned long long>(off), static_cast<uint32_t>(steps)));
         in0 = off - head * steps;
     }
@@ -213,25 +281,25 @@ struct TileWalk {
             if (++head < a.n_head_kv) break;
             head = 0;
             if (++tile < t.tiles) {
-                steps = tile_steps(a, t, tile);
+                steps = tile_steps<ROWS, KEYS>(a, t, tile);
                 break;
             }
             tile = 0;
-            do t = tile_seq(a, ++seq);
+            do t = tile_seq<ROWS>(a, ++seq);
             while (t.tiles == 0);        // u1 is within the line, so there is one
-            steps = tile_steps(a, t, 0);
+            steps = tile_steps<ROWS, KEYS>(a, t, 0);
         }
         const int64_t left = steps - in0;
         const int64_t take = min(left, static_cast<int64_t>(u1 - pos));
         p.q = t.q;
         p.seq = seq;
         p.head = static_cast<uint32_t>(head);
-        p.first = static_cast<uint32_t>(tile) * kTileRows;
-        p.rows = min(static_cast<uint32_t>(kTileRows), static_cast<uint32_t>(t.q.n_new) * a.group - p.first);
+        p.first = static_cast<uint32_t>(tile) * ROWS;
+        p.rows = min(static_cast<uint32_t>(ROWS), static_cast<uint32_t>(t.q.n_new) * a.group - p.first);
         p.in0 = static_cast<int32_t>(in0);
         p.kend = attend_limit(a, t.q, static_cast<int32_t>((p.first + p.rows - 1) / a.group));
         p.kfull = attend_limit(a, t.q, static_cast<int32_t>(p.first / a.group));
-        p.in1 = min(static_cast<int32_t>(in0 + take), (p.kend + kTileKeys - 1) / kTileKeys);
+        p.in1 = min(static_cast<int32_t>(in0 + take), (p.kend + KEYS - 1) / KEYS);
         p.starts = in0 == 0;
         p.ends = take == left;
         p.more = p.ends ? 0u : static_cast<uint32_t>((pos + left - u1 + share - 1) / share);
@@ -243,18 +311,19 @@ struct TileWalk {
 
 // A warp's walk in shared memory: its state is needed once a piece and would
 // otherwise hold forty registers through the inner loops.
+template <int ROWS, int KEYS>
 struct WarpWalk {
-    TileWalk walk;
+    TileWalk<ROWS, KEYS> walk;
     TilePiece piece;
     uint32_t more;
 };
 
 // A piece's results in the workspace: maxima, sums, then rows of D halves.
-template <int D>
-__host__ __device__ constexpr uint32_t tile_part_bytes() { return kTileRows * (8u + 2u * D); }
-template <int D>
+template <int D, int ROWS>
+__host__ __device__ constexpr uint32_t tile_part_bytes() { return ROWS * (8u + 2u * D); }
+template <int D, int ROWS>
 __device__ __forceinline__ uint8_t *tile_part(const AttendArgs &a, uint32_t slot) {
-    return a.work + kAttendMaxCtas * kAttendDescBytes + static_cast<uint64_t>(slot) * tile_part_bytes<D>();
+    return a.work + kAttendMaxCtas * kAttendDescBytes + static_cast<uint64_t>(slot) * tile_part_bytes<D, ROWS>();
 }
 
 // ------------------------------------------------------------ dequantizing --
@@ -296,17 +365,17 @@ __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
 }
 
 // Writes 16 keys' slices as F16 values into the operand tile; `raw` is the warp's
-// 16 rows, `key0` its first row of the tile's 64.  An eighth of a warp takes eight
+// 16 rows, `key0` its first row of the tile's ROWS.  An eighth of a warp takes eight
 // keys' same 16-byte chunk, so reads and swizzled stores are free of bank
 // conflicts.  Returns whether a scale (F16: a value) of this lane is not finite.
-template <int T, int D>
+template <int T, int D, int ROWS>
 __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
     uint32_t top = 0;              // largest magnitude bits of the scales
     using S = Slice<T, D>;
     const int k8 = lane & 7, quad = lane >> 3;
     auto put = [&](int key, int dim8, uint4 v) {       // dims 8 dim8 .. 8 dim8 + 7 of a key
         const int row = key0 + key;
-        *reinterpret_cast<uint4 *>(tile + (dim8 >> 3) * (kTileKeys * 128) + row * 128 + (((dim8 & 7) ^ (row & 7)) << 4)) = v;
+        *reinterpret_cast<uint4 *>(tile + (dim8 >> 3) * (ROWS * 128) + row * 128 + (((dim8 & 7) ^ (row & 7)) << 4)) = v;
     };
     auto scale_at = [&](const uint8_t *p) -> uint32_t {
         const uint32_t d = lds16(p);
@@ -409,34 +478,35 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
 }
 
 // ------------------------------------------------------------------ kernel --
-template <int D, int KT, int VT>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __grid_constant__ AttendArgs a) {
-    using G = TileGeom<D, KT, VT>;
-    constexpr int NS = G::kStages;
+template <int D, int KT, int VT, bool PAIR>
+__device__ __forceinline__ void attend_tile(const AttendArgs &a) {
+    using G = TileGeom<D, KT, VT, PAIR>;
+    constexpr int NS = G::kStages, kKeys = G::kKeys, kRows = G::kRows, kCtas = PAIR ? 2 : 1;
     constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 7.0f, kSlack = 8.0f;
-    constexpr uint32_t kColS = 0, kColO = 2 * kTileKeys, kColQ = kColO + D;
+    constexpr uint32_t kColS = 0, kColO = 2 * kKeys, kColQ = kColO + D;       // kColQ: single CTAs only
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBars);
     uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
              *q_full = bars + 12, *raw_full = bars + 13;          // raw_full [8 warps][NS]
-    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][4 warps]
+    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][4 warps of each CTA]
+    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = blockIdx.x / kCtas, n_units = gridDim.x / kCtas;
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
     __shared__ uint32_t s_seq, s_tmem, s_odd;
     __shared__ float s_swap[2][2 * kTileRows];
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&v_full[i], 4);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&k_full[i], 4 * kCtas);
+            mbar_init(&v_full[i], 4 * kCtas);
+            mbar_init(&p_full[i], 8 * kCtas);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
         }
-        mbar_init(q_full, 8);
-        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
+        mbar_init(q_full, 8 * kCtas);
+        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], i < 4 * NS ? 1 : G::kBoxesV);
         s_odd = 0;
         fence_mbar_init();
     }
@@ -444,8 +514,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
 
     // ---- this CTA's share of the line of (item, key tile)
     auto units = [&](uint32_t s) -> unsigned long long {
-        const TileSeq t = tile_seq(a, s);
-        return t.tiles ? static_cast<unsigned long long>(a.n_head_kv * tile_prefix(a, t, t.tiles)) : 0ull;
+        const TileSeq t = tile_seq<kRows>(a, s);
+        return t.tiles ? static_cast<unsigned long long>(a.n_head_kv * tile_prefix<kRows, kKeys>(a, t, t.tiles)) : 0ull;
     };
     auto scan = [&](unsigned long long n, unsigned long long *all) -> unsigned long long {
         unsigned long long x = n;
@@ -469,11 +539,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
     unsigned long long mine = 0, total = 0;
     for (uint32_t s = tid; s < a.n_seq; s += kTileThreads) mine += units(s);
     const unsigned long long upto = scan(mine, &total);
-    const unsigned long long share = max(1ull, div_small(total + gridDim.x - 1, gridDim.x));
-    const unsigned long long u0 = share * blockIdx.x, u1 = min(u0 + share, total);
-    AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + blockIdx.x;
+    const unsigned long long share = max(1ull, div_small(total + n_units - 1, n_units));
+    const unsigned long long u0 = share * unit, u1 = min(u0 + share, total);
+    AttendDesc *desc = reinterpret_cast<AttendDesc *>(a.work) + unit;
     if (u0 >= total) {
-        if (tid == 0) desc->parts = 0;
+        if (tid == 0 && rank == 0) desc->parts = 0;
         return;
     }
     unsigned long long carry = 0;
@@ -492,15 +562,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         if (carry > u0) break;
     }
     if (warp == 16) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
         tc_fence_before();
     }
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();        // the peer's barriers and TMEM are there
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    __shared__ WarpWalk s_walk[kTileThreads / 32];
-    WarpWalk &mywalk = s_walk[warp];
+    __shared__ WarpWalk<kRows, kKeys> s_walk[kTileThreads / 32];
+    WarpWalk<kRows, kKeys> &mywalk = s_walk[warp];
     const TilePiece &p = mywalk.piece;
     if (lane == 0) {
         mywalk.walk.pos = u0;
@@ -521,11 +597,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         // while another still polls for this one
         __syncwarp();
     };
+    // barriers that the products wait on are the first CTA's
+    auto arrive = [&](uint64_t *bar) {
+        if constexpr (PAIR) mbar_arrive_at(bar, 0);
+        else mbar_arrive(bar);
+    };
     uint32_t j = 0;                            // running key tile of the CTA: stage j & 1, phase j >> 1
 
     if (warp < 8) {
-        // ======== rows: Q into TMEM, softmax, epilogue; thread (row, wg) has columns 32 wg .. of S
-        // and dims D / 2 wg .. of Q and O
+        // ======== rows: Q, softmax, epilogue; thread (row, wg) has one half of S's columns and
+        // of Q's and O's dims
+        constexpr int kHalf = kKeys / 2;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) * 32u << 16);
         const int row = tid & 127, wg = tid >> 7;
         uint32_t swaps = 0;
@@ -538,8 +620,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         };
         bool described = false;
         while (next_piece()) {
-            const bool in = static_cast<uint32_t>(row) < p.rows;
-            const uint32_t rr = p.first + (in ? row : 0), tok = rr / a.group;
+            const uint32_t item_row = rank * kTileRows + row;
+            const bool in = item_row < p.rows;
+            const uint32_t rr = p.first + (in ? item_row : 0), tok = rr / a.group;
             const uint64_t at_tok = static_cast<uint64_t>(p.q.row0) + tok, at_head = static_cast<uint64_t>(p.head) * a.group + rr % a.group;
             const uint8_t *qp = a.q.p + at_tok * a.q.nb_tok + at_head * a.q.nb_head;
             const int32_t lim = in ? attend_limit(a, p.q, static_cast<int32_t>(tok)) : p.kend;
@@ -587,13 +670,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                         const int at = 32 * c0 + 8 * (i / 4), x = 2 * (i % 4);
                         w[i] = in ? pack_half2(value(at + tile_order<KT>(x)) * mul, value(at + tile_order<KT>(x + 1)) * mul) : 0u;
                     }
-                    tc_st16(lanes + kColQ + wg * (D / 4) + 16 * c0, w);
+                    if constexpr (PAIR) {              // K-major with the 128-byte swizzle, 64 dims a chunk
+                        const int dim8 = wg * (D / 16) + 4 * c0;
+                        uint8_t *to = smem + 4 * G::kOperand + row * 128;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<uint4 *>(to + ((dim8 + i) >> 3) * (kTileRows * 128) + ((((dim8 + i) & 7) ^ (row & 7)) << 4)) =
+                                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    } else {
+                        tc_st16(lanes + kColQ + wg * (D / 4) + 16 * c0, w);
+                    }
                 }
             }
-            tc_wait_st();
+            if constexpr (PAIR) fence_proxy_async_smem();
+            else tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0 && work) mbar_arrive(q_full);
+            if (lane == 0 && work) arrive(q_full);
 
             float m = kNegInf, l = 0.0f;
             const uint32_t j0 = j;
@@ -606,22 +699,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 // s_full waited for, and not again before the tile after next's products.
                 // (k_full itself may be a phase ahead here and must not be waited on.)
                 tc_fence_after();
+                // 32 columns at a time; a pair's thread has two such chunks and reads them twice
                 uint32_t s[32];
-                tc_ld32(s, lanes + kColS + st * kTileKeys + 32 * wg);
-                tc_wait_ld();
-                const uint2 ok2 = *reinterpret_cast<const uint2 *>(valid + 4 * (j & 3u) + 2 * wg);
-                const uint32_t ok = ok2.x | ok2.y << 16;
-                const int32_t key0 = n * kTileKeys + 32 * wg;
-                if (key0 + 32 > kfull || ok != 0xffffffffu) {
+                auto columns = [&](int c) {
+                    tc_ld32(s, lanes + kColS + st * kKeys + wg * kHalf + 32 * c);
+                    tc_wait_ld();
+                    const uint2 ok2 = *reinterpret_cast<const uint2 *>(valid + (kKeys / 16) * (j & 3u) + wg * (kHalf / 16) + 2 * c);
+                    const uint32_t ok = ok2.x | ok2.y << 16;
+                    const int32_t key0 = n * kKeys + wg * kHalf + 32 * c;
+                    if (key0 + 32 > kfull || ok != 0xffffffffu) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (key0 + i >= lim || !((ok >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
+                        for (int i = 0; i < 32; ++i)
+                            if (key0 + i >= lim || !((ok >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
+                    }
+                };
+                float x = kNegInf;
+#pragma unroll
+                for (int c = 0; c < kHalf / 32; ++c) {
+                    columns(c);
+                    float t4[4] = {x, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        t4[(i >> 1) & 3] = fmaxf(fmaxf(t4[(i >> 1) & 3], __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
+                    x = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                 }
-                float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-                for (int i = 0; i < 32; i += 2)
-                    t4[(i >> 1) & 3] = fmaxf(fmaxf(t4[(i >> 1) & 3], __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
-                float x = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                 x = fmaxf(x, swap(x));
                 const float mt = x == kNegInf ? kNegInf : x * fac;
                 if (__any_sync(0xffffffffu, mt > m + kSlack || (m == kNegInf && mt > m))) {
@@ -647,20 +748,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 const float ref = m == kNegInf ? 0.0f : kWeightLog - m;
                 const float2 fac2 = make_float2(fac, fac), ref2 = make_float2(ref, ref);
                 float2 sum2 = make_float2(0.0f, 0.0f);
-                uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 y = f2_fma_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, ref2);
-                    const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                    sum2 = f2_add_rn(sum2, e);
-                    w[i] = pack_half2(e.x, e.y);
+                for (int c = 0; c < kHalf / 32; ++c) {
+                    if (kHalf > 32) columns(c);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = f2_fma_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, ref2);
+                        const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                        sum2 = f2_add_rn(sum2, e);
+                        w[i] = pack_half2(e.x, e.y);
+                    }
+                    // over the thread's own columns, those it has read for the last time
+                    tc_st16(lanes + kColS + st * kKeys + wg * kHalf + 16 * c, w);
                 }
-                tc_st16(lanes + kColS + st * kTileKeys + 16 * wg, w);
                 l += sum2.x + sum2.y;
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[st]);
+                if (lane == 0) arrive(&p_full[st]);
             }
             // ---- epilogue
             const bool any = j != j0;
@@ -673,14 +779,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             const bool whole = p.starts && p.ends;
             const bool odd = *reinterpret_cast<volatile uint32_t *>(&s_odd) != 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t *part = whole ? nullptr : tile_part<D>(a, 2u * blockIdx.x + (p.starts ? 1u : 0u));
+            uint8_t *part = whole ? nullptr : tile_part<D, kRows>(a, 2u * unit + (p.starts ? 1u : 0u));
             uint8_t *op = const_cast<uint8_t *>(a.out.p) + at_tok * a.out.nb_tok + at_head * a.out.nb_head;
             if (part && wg == 0) {
-                reinterpret_cast<float *>(part)[row] = m;
-                reinterpret_cast<float *>(part)[kTileRows + row] = l;
+                reinterpret_cast<float *>(part)[item_row] = m;
+                reinterpret_cast<float *>(part)[kRows + item_row] = l;
             }
 #pragma unroll 1
-            for (int c = wg * (D / 64); c < (static_cast<uint32_t>(warp & 3) * 32u < p.rows ? (wg + 1) * (D / 64) : 0); ++c) {
+            for (int c = wg * (D / 64); c < (rank * kTileRows + static_cast<uint32_t>(warp & 3) * 32u < p.rows ? (wg + 1) * (D / 64) : 0); ++c) {
                 uint32_t o[32];
                 if (any) {
                     tc_ld32(o, lanes + kColO + 32 * c);
@@ -690,13 +796,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[(i & ~7) | tile_order<VT>(i & 7)] = any ? __uint_as_float(o[i]) * inv : 0.0f;
                 if (odd && in) {                       // values the tiles left out: infinities and NaN that this row sees
-                    const int32_t hi = min(lim, p.in1 * kTileKeys);
-                    for (int32_t key = p.in0 * kTileKeys; key < hi; ++key) {
-                        const uint32_t blk = static_cast<uint32_t>(key) / a.block_tokens;
+                    const int32_t hi = min(lim, p.in1 * kKeys);
+                    for (int32_t key = p.in0 * kKeys; key < hi; ++key) {
+                        const uint32_t blk = attend_block(a, static_cast<uint32_t>(key));
                         const int32_t slot = a.table[p.seq * a.table_stride + blk];
                         if (slot < 0 || static_cast<uint32_t>(slot) >= a.n_slots) continue;
                         const uint64_t cell = static_cast<uint64_t>(slot) * a.block_tokens + (key - blk * a.block_tokens);
-                        const uint8_t *v = a.v + cell * a.row_v + static_cast<uint64_t>(p.head) * G::V::kBytes;
+                        const uint8_t *v = a.v + cell * a.row_v + static_cast<uint64_t>(p.head) * (G::kSlices * G::V::kBytes);
                         if (VT != KVM_TYPE_F16 && (*reinterpret_cast<const uint16_t *>(v + c * G::V::kBlock) & 0x7c00u) != 0x7c00u) continue;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
@@ -706,7 +812,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     }
                 }
                 if (part && in) {
-                    uint4 *to = reinterpret_cast<uint4 *>(part + 8 * kTileRows + (row * D + 32 * c) * 2);
+                    uint4 *to = reinterpret_cast<uint4 *>(part + 8 * kRows + (item_row * D + 32 * c) * 2);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         to[k] = make_uint4(pack_half2(y[8 * k], y[8 * k + 1]), pack_half2(y[8 * k + 2], y[8 * k + 3]),
@@ -736,7 +842,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 }
             }
             tc_fence_before();                         // O and Q are free for the next piece's products
-            if (tid == 0 && p.starts && !p.ends) {
+            if (tid == 0 && rank == 0 && p.starts && !p.ends) {
                 desc->row0 = p.q.row0;
                 desc->head = p.head;
                 desc->first = p.first;
@@ -745,7 +851,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
             }
             described = described || (p.starts && !p.ends);
         }
-        if (tid == 0 && !described) desc->parts = 0;
+        if (tid == 0 && rank == 0 && !described) desc->parts = 0;
     } else if (warp < 16) {
         // ======== K (warps 8-11) and V (warps 12-15): raw rows to operand tiles
         const bool is_v = warp >= 12;
@@ -753,47 +859,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
         const int raw_bytes = is_v ? G::kRawV : G::kRawK;
         uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kRawK : 0) + w4 * NS * raw_bytes;
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
-        uint32_t *vmask = valid + w4;
         uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring stage of the next load, of the next tile
         while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0);
             const int32_t *trow = a.table + p.seq * a.table_stride;
-            const uint64_t slice = static_cast<uint64_t>(p.head) * (is_v ? G::V::kBytes : G::K::kBytes);
+            const uint64_t slice = is_v ? (static_cast<uint64_t>(p.head) * G::kSlices + rank) * G::V::kBytes : static_cast<uint64_t>(p.head) * G::K::kBytes;
             const int lead = a.tma ? static_cast<int>(slice & 15u) : 0;
             uint32_t ring_ok[NS];                      // visible keys of the loads in flight
 #pragma unroll
             for (int i = 0; i < NS; ++i) ring_ok[i] = 0;
-            // every lane computes the visible keys of the warp's 16 in tile n
+            // the warp's keys of a tile: 16 from `mine` on, or (V of a pair) twice 16, bits 0-15
+            // and 16-31 of a mask
             const int32_t in0 = p.in0, kend = p.kend;
-            // the table entry of load i, fetched while load i - 1 is issued
+            const int32_t mine = is_v ? w4 * 16 * G::kBoxesV : static_cast<int32_t>(rank) * 64 + w4 * 16;
+            const int boxes = is_v ? G::kBoxesV : 1;
+            // TMA: lane b brings box b; its table entry is fetched while the load before is issued
             auto entry = [&](int32_t i) -> int32_t {
-                const int32_t key0 = (in0 + i) * kTileKeys + w4 * 16;
-                return i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
+                const int32_t key0 = (in0 + i) * kKeys + mine + 16 * lane;
+                return lane < boxes && i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
             };
             int32_t slot_next = a.tma ? entry(0) : -1;
             auto load = [&](int32_t i) -> uint32_t {
                 uint8_t *st = ring + in_at * raw_bytes;
                 uint64_t *bar = &full[in_at];
                 if (++in_at == NS) in_at = 0;
-                const uint32_t key0 = static_cast<uint32_t>((in0 + i) * kTileKeys + w4 * 16);
-                const int32_t left = kend - static_cast<int32_t>(key0);
+                const int32_t first = (in0 + i) * kKeys + mine;
                 if (a.tma) {
                     uint32_t ok = 0;
-                    const int32_t slot = slot_next;
+                    const int32_t slot = slot_next, key0 = first + 16 * lane, left = kend - key0;
                     slot_next = entry(i + 1);
-                    if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
-                        ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
-                        if (lane == 0) {
-                            const uint32_t in_block = key0 - attend_block(a, key0) * a.block_tokens;
-                            mbar_arrive_expect_tx(bar, raw_bytes);
-                            tma_load_2d(st, is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
+                    if (lane < boxes) {
+                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
+                            ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                            const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
+                            mbar_arrive_expect_tx(bar, raw_bytes / boxes);
+                            tma_load_2d(st + lane * (raw_bytes / boxes), is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
                                         static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
+                        } else {
+                            mbar_arrive(bar);
                         }
                     }
-                    if (ok == 0 && lane == 0) mbar_arrive(bar);
-                    return ok;
+                    return __shfl_sync(0xffffffffu, ok, 0) | (boxes > 1 ? __shfl_sync(0xffffffffu, ok, 1) << 16 : 0u);
                 }
-                const uint32_t key = key0 + (lane & 15);
+                const int rows = 16 * boxes;
+                const uint32_t key = first + (lane & (rows - 1));
                 int32_t cell = -1;
                 if (static_cast<int32_t>(key) < kend) {
                     const uint32_t blk = attend_block(a, key);
@@ -801,15 +910,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
                         cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
                 }
-                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
+                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & (boxes > 1 ? 0xffffffffu : 0xffffu);
                 auto copy = [&](auto slice_t, const uint8_t *base, uint64_t row_bytes) {
                     using S = decltype(slice_t);
                     constexpr int C = S::kBytes / 4;
 #pragma unroll 4
-                    for (int y = 0; y < (kAttendBox * C + 31) / 32; ++y) {
-                        const int x = lane + 32 * y, r = min(x / C, kAttendBox - 1), c = x - r * C;
+                    for (int y = 0; y < (rows * C + 31) / 32; ++y) {
+                        const int x = lane + 32 * y, r = min(x / C, rows - 1), c = x - r * C;
                         const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
-                        if (x < kAttendBox * C)
+                        if (x < rows * C)
                             cp_async4(smem_u32(st + r * S::kStride + c * 4), base + (cr >= 0 ? cr * row_bytes + c * 4 : 0ull), cr >= 0 ? 4u : 0u);
                     }
                 };
@@ -837,9 +946,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                     cp_async_commit();
                 }
                 uint8_t *raw = ring + out_at * raw_bytes + lead;
-                if (ok != 0xffffu) {
-                    if (is_v) tile_clean<VT, D, false>(raw, ok, lane);
-                    else tile_clean<KT, D, false>(raw, ok, lane);
+                constexpr int kVD = PAIR ? D / 2 : D, kBoxV = kAttendBox * G::V::kStride;
+                if (is_v) {
+#pragma unroll
+                    for (int b = 0; b < G::kBoxesV; ++b)
+                        if (((ok >> (16 * b)) & 0xffffu) != 0xffffu) tile_clean<VT, kVD, false>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
+                } else if (ok != 0xffffu) {
+                    tile_clean<KT, D, false>(raw, ok, lane);
                 }
                 if (j >= 2) wait(&tile_free[j & 1u], (j >> 1) - 1u);
                 if (++out_at == NS) {
@@ -848,80 +961,120 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __gr
                 }
                 uint8_t *tile = smem + (is_v ? 2 * G::kOperand : 0) + (j & 1u) * G::kOperand;
                 if (is_v) {
-                    if (__any_sync(0xffffffffu, tile_dequant<VT, D>(raw, tile, w4 * 16, lane))) {
-                        // the epilogue adds what is not finite; the products do without it
-                        tile_clean<VT, D, true>(raw, ok, lane);
-                        tile_dequant<VT, D>(raw, tile, w4 * 16, lane);
-                        *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
-                    }
+#pragma unroll
+                    for (int b = 0; b < G::kBoxesV; ++b)
+                        if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw + b * kBoxV, tile, mine + 16 * b, lane))) {
+                            // the epilogue adds what is not finite; the products do without it
+                            tile_clean<VT, kVD, true>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
+                            tile_dequant<VT, kVD, kKeys>(raw + b * kBoxV, tile, mine + 16 * b, lane);
+                            if (lane < kCtas) {
+                                if constexpr (PAIR) st_shared_at(&s_odd, 1u, lane);
+                                else *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
+                            }
+                        }
                 } else {
-                    tile_dequant<KT, D>(raw, tile, w4 * 16, lane);
+                    tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
+                    if (lane < kCtas) {
+                        uint32_t *to = valid + (kKeys / 16) * (j & 3u) + mine / 16;
+                        if constexpr (PAIR) st_shared_at(to, ok, lane);
+                        else *to = ok;
+                    }
                 }
-                if (!is_v && lane == 0) vmask[4 * (j & 3u)] = ok;
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&tile_full[j & 1u]);
+                if (lane == 0) arrive(&tile_full[j & 1u]);
             }
             cp_async_wait<0>();
             __syncwarp();
         }
-    } else {
-        // ======== products, issued by one thread
-        constexpr uint32_t kIdS = tc_idesc(kTileKeys, false), kIdO = tc_idesc(D, true);
+    } else if (rank == 0) {
+        // ======== products, issued by one thread (of a pair: the first CTA's, for both)
+        constexpr uint32_t kIdS = tc_idesc(kRows, kKeys, false), kIdO = tc_idesc(kRows, D, true);
         // descriptors of the first tiles; the others differ in the address field, which
         // no addition here carries out of
         const uint64_t k_desc = tc_desc(smem_u32(smem), 16, 1024);
-        const uint64_t v_desc = tc_desc(smem_u32(smem) + 2 * G::kOperand, kTileKeys * 128, 1024);
+        const uint64_t v_desc = tc_desc(smem_u32(smem) + 2 * G::kOperand, kKeys * 128, 1024);
+        const uint64_t q_desc = tc_desc(smem_u32(smem) + 4 * G::kOperand, 16, 1024);      // pair only
+        auto wait_all = [&](uint64_t *bar, uint32_t phase) {
+            if constexpr (PAIR) {
+                if (!lost && !mbar_wait_cluster(bar, phase & 1u)) lost = true;
+                __syncwarp();
+            } else {
+                wait(bar, phase);
+            }
+        };
+        auto commit = [&](uint64_t *bar) {
+            if constexpr (PAIR) tc_commit_pair(bar);
+            else tc_commit(bar);
+        };
         uint32_t piece = 0;
         while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0);
             if (n_tiles == 0) continue;
-            wait(q_full, piece++);
+            wait_all(q_full, piece++);
             tc_fence_after();
             const uint32_t j0 = j;
             auto qk = [&](uint32_t t) {
-                wait(&k_full[t & 1u], t >> 1);
+                wait_all(&k_full[t & 1u], t >> 1);
                 tc_fence_after();
                 const uint64_t base = k_desc + (t & 1u) * (G::kOperand / 16);
-                const uint32_t to = tmem + kColS + (t & 1u) * kTileKeys;
+                const uint32_t to = tmem + kColS + (t & 1u) * kKeys;
                 if (lane == 0) {
 #pragma unroll
-                    for (int s = 0; s < D / 16; ++s)
-                        tc_mma(to, tmem + kColQ + 8 * s, base + ((s >> 2) * (kTileKeys * 128) + (s & 3) * 32) / 16, kIdS, s != 0);
-                    tc_commit(&s_full[t & 1u]);
-                    tc_commit(&k_free[t & 1u]);
+                    for (int s = 0; s < D / 16; ++s) {
+                        const uint64_t b = base + ((s >> 2) * (64 * 128) + (s & 3) * 32) / 16;
+                        if constexpr (PAIR) tc_mma_pair(to, q_desc + ((s >> 2) * (kTileRows * 128) + (s & 3) * 32) / 16, b, kIdS, s != 0);
+                        else tc_mma(to, tmem + kColQ + 8 * s, b, kIdS, s != 0);
+                    }
+                    commit(&s_full[t & 1u]);
+                    commit(&k_free[t & 1u]);
                 }
                 __syncwarp();
             };
             qk(j0);
             for (int32_t i = 0; i < n_tiles; ++i, ++j) {
                 if (i + 1 < n_tiles) qk(j + 1);
-                wait(&p_full[j & 1u], j >> 1);
-                wait(&v_full[j & 1u], j >> 1);
+                wait_all(&p_full[j & 1u], j >> 1);
+                wait_all(&v_full[j & 1u], j >> 1);
                 tc_fence_after();
                 const uint64_t base = v_desc + (j & 1u) * (G::kOperand / 16);
-                const uint32_t from = tmem + kColS + (j & 1u) * kTileKeys;
+                const uint32_t from = tmem + kColS + (j & 1u) * kKeys;
                 if (lane == 0) {
 #pragma unroll
-                    for (int s = 0; s < kTileKeys / 16; ++s)
-                        tc_mma(tmem + kColO, from + 8 * s, base + s * (2048 / 16), kIdO, i != 0 || s != 0);
-                    tc_commit(&v_free[j & 1u]);
+                    for (int s = 0; s < kKeys / 16; ++s) {
+                        // P of the first half of the keys lies at column 0, of the second at kKeys / 2
+                        const uint32_t at = from + (s >= kKeys / 32 ? kKeys / 2 + 8 * (s - kKeys / 32) : 8 * s);
+                        if constexpr (PAIR) tc_mma_pair(tmem + kColO, at, base + s * (2048 / 16), kIdO, i != 0 || s != 0);
+                        else tc_mma(tmem + kColO, at, base + s * (2048 / 16), kIdO, i != 0 || s != 0);
+                    }
+                    commit(&v_free[j & 1u]);
                 }
                 __syncwarp();
             }
         }
     }
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();        // no product reads the peer's memory any more
     if (warp == 16) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
     pdl_launch_dependents();
 }
 
+template <int D, int KT, int VT>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const __grid_constant__ AttendArgs a) {
+    attend_tile<D, KT, VT, false>(a);
+}
+template <int D, int KT, int VT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) attend_pair_kernel(const __grid_constant__ AttendArgs a) {
+    attend_tile<D, KT, VT, true>(a);
+}
+
 // out = sum w_i o_i / sum w_i, w_i = l_i 2^(m_i - max), over the pieces of every
 // split item: a group of D / 8 threads a row, eight dims a thread.
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __grid_constant__ AttendArgs a, uint32_t ctas) {
     constexpr uint32_t kGroup = D / 8, kPer = kJoinThreads / kGroup;
     __shared__ JoinList list;
@@ -932,7 +1085,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __
         const uint32_t c = join_find(list, ctas, x, &r);
         const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + c;
         const uint32_t parts = min(desc->parts, ctas), d8 = threadIdx.x % kGroup;
-        auto part = [&](uint32_t i) { return tile_part<D>(a, i ? 2u * (c + i) : 2u * c + 1u); };
+        auto part = [&](uint32_t i) { return tile_part<D, ROWS>(a, i ? 2u * (c + i) : 2u * c + 1u); };
         float top = -__builtin_huge_valf();
         for (uint32_t i = 0; i < parts; ++i) top = fmaxf(top, reinterpret_cast<const float *>(part(i))[r]);
         const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
@@ -940,8 +1093,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __
 #pragma unroll 2
         for (uint32_t i = 0; i < parts; ++i) {
             const float *f = reinterpret_cast<const float *>(part(i));
-            const float w = f[kTileRows + r] * exp2_approx(f[r] - ref);
-            const uint4 v = *reinterpret_cast<const uint4 *>(part(i) + 8 * kTileRows + (r * D + 8 * d8) * 2);
+            const float w = f[ROWS + r] * exp2_approx(f[r] - ref);
+            const uint4 v = *reinterpret_cast<const uint4 *>(part(i) + 8 * ROWS + (r * D + 8 * d8) * 2);
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
             sum += w;
             if (w != 0.0f) {
