@@ -99,11 +99,14 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
         ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
-// Arrives on the barrier at the same offset in CTA `rank` of the cluster.
+// Arrives on the barrier at the same offset in CTA `rank` of the cluster.  What the
+// arrival announces lies in this SM (TMEM, shared memory) and has been completed by
+// tcgen05.wait or a proxy fence before; a cluster-scope release would wait for every
+// other access too, over a thousand cycles.
 __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
     asm volatile(
         "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}"
+        "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}"
         ::"r"(smem_u32(bar)), "r"(rank)
         : "memory");
 }
@@ -112,26 +115,6 @@ __device__ __forceinline__ void st_shared_at(uint32_t *p, uint32_t v, uint32_t r
         "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tst.shared::cluster.u32 [ra], %1;\n\t}"
         ::"r"(smem_u32(p)), "r"(v), "r"(rank)
         : "memory");
-}
-// Bounded wait with cluster-scope acquire (arrivals come from both CTAs).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 0;; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if ((i & 1023u) == 1023u) {
-            const uint64_t now = global_timer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitLimitNs) return false;
-        }
-    }
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -490,7 +473,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBars);
     uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
              *q_full = bars + 12, *raw_full = bars + 13;          // raw_full [8 warps][NS]
-    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][4 warps of each CTA]
+    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][kKeys / 16], a bit a key
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = blockIdx.x / kCtas, n_units = gridDim.x / kCtas;
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
     __shared__ uint32_t s_seq, s_tmem, s_odd;
@@ -873,10 +856,14 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             const int32_t in0 = p.in0, kend = p.kend;
             const int32_t mine = is_v ? w4 * 16 * G::kBoxesV : static_cast<int32_t>(rank) * 64 + w4 * 16;
             const int boxes = is_v ? G::kBoxesV : 1;
+            // the second 16 keys of a mask: V's second box, or (K of a pair) those that the peer's
+            // warp brings, of which only the visibility is wanted here
+            const int32_t second = is_v ? 16 : rank == 0 ? 64 : -64;
+            constexpr int kLooks = kCtas;
             // TMA: lane b brings box b; its table entry is fetched while the load before is issued
             auto entry = [&](int32_t i) -> int32_t {
-                const int32_t key0 = (in0 + i) * kKeys + mine + 16 * lane;
-                return lane < boxes && i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
+                const int32_t key0 = (in0 + i) * kKeys + mine + second * lane;
+                return lane < kLooks && i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
             };
             int32_t slot_next = a.tma ? entry(0) : -1;
             auto load = [&](int32_t i) -> uint32_t {
@@ -886,23 +873,25 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 const int32_t first = (in0 + i) * kKeys + mine;
                 if (a.tma) {
                     uint32_t ok = 0;
-                    const int32_t slot = slot_next, key0 = first + 16 * lane, left = kend - key0;
+                    const int32_t slot = slot_next, key0 = first + second * lane, left = kend - key0;
                     slot_next = entry(i + 1);
-                    if (lane < boxes) {
-                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) {
-                            ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
-                            const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
-                            mbar_arrive_expect_tx(bar, raw_bytes / boxes);
-                            tma_load_2d(st + lane * (raw_bytes / boxes), is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
-                                        static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
-                        } else {
-                            mbar_arrive(bar);
+                    if (lane < kLooks) {
+                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                        if (lane < boxes) {
+                            if (ok != 0) {
+                                const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
+                                mbar_arrive_expect_tx(bar, raw_bytes / boxes);
+                                tma_load_2d(st + lane * (raw_bytes / boxes), is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
+                                            static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
+                            } else {
+                                mbar_arrive(bar);
+                            }
                         }
                     }
-                    return __shfl_sync(0xffffffffu, ok, 0) | (boxes > 1 ? __shfl_sync(0xffffffffu, ok, 1) << 16 : 0u);
+                    return __shfl_sync(0xffffffffu, ok, 0) | (kLooks > 1 ? __shfl_sync(0xffffffffu, ok, 1) << 16 : 0u);
                 }
                 const int rows = 16 * boxes;
-                const uint32_t key = first + (lane & (rows - 1));
+                const uint32_t key = first + (kLooks > 1 ? (lane & 15) + second * (lane >> 4) : lane & 15);
                 int32_t cell = -1;
                 if (static_cast<int32_t>(key) < kend) {
                     const uint32_t blk = attend_block(a, key);
@@ -910,7 +899,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
                         cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
                 }
-                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & (boxes > 1 ? 0xffffffffu : 0xffffu);
+                const uint32_t ok = __ballot_sync(0xffffffffu, cell >= 0) & (kLooks > 1 ? 0xffffffffu : 0xffffu);
                 auto copy = [&](auto slice_t, const uint8_t *base, uint64_t row_bytes) {
                     using S = decltype(slice_t);
                     constexpr int C = S::kBytes / 4;
@@ -951,8 +940,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
 #pragma unroll
                     for (int b = 0; b < G::kBoxesV; ++b)
                         if (((ok >> (16 * b)) & 0xffffu) != 0xffffu) tile_clean<VT, kVD, false>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
-                } else if (ok != 0xffffu) {
-                    tile_clean<KT, D, false>(raw, ok, lane);
+                } else if ((ok & 0xffffu) != 0xffffu) {
+                    tile_clean<KT, D, false>(raw, ok & 0xffffu, lane);
                 }
                 if (j >= 2) wait(&tile_free[j & 1u], (j >> 1) - 1u);
                 if (++out_at == NS) {
@@ -967,18 +956,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                             // the epilogue adds what is not finite; the products do without it
                             tile_clean<VT, kVD, true>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
                             tile_dequant<VT, kVD, kKeys>(raw + b * kBoxV, tile, mine + 16 * b, lane);
-                            if (lane < kCtas) {
-                                if constexpr (PAIR) st_shared_at(&s_odd, 1u, lane);
-                                else *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
+                            if constexpr (PAIR) {
+                                if (lane < kCtas) st_shared_at(&s_odd, 1u, lane);
+                                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                            } else {
+                                *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
                             }
                         }
                 } else {
                     tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
-                    if (lane < kCtas) {
-                        uint32_t *to = valid + (kKeys / 16) * (j & 3u) + mine / 16;
-                        if constexpr (PAIR) st_shared_at(to, ok, lane);
-                        else *to = ok;
-                    }
+                    if (lane < kLooks) valid[(kKeys / 16) * (j & 3u) + (mine + second * lane) / 16] = (ok >> (16 * lane)) & 0xffffu;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -995,14 +982,6 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         const uint64_t k_desc = tc_desc(smem_u32(smem), 16, 1024);
         const uint64_t v_desc = tc_desc(smem_u32(smem) + 2 * G::kOperand, kKeys * 128, 1024);
         const uint64_t q_desc = tc_desc(smem_u32(smem) + 4 * G::kOperand, 16, 1024);      // pair only
-        auto wait_all = [&](uint64_t *bar, uint32_t phase) {
-            if constexpr (PAIR) {
-                if (!lost && !mbar_wait_cluster(bar, phase & 1u)) lost = true;
-                __syncwarp();
-            } else {
-                wait(bar, phase);
-            }
-        };
         auto commit = [&](uint64_t *bar) {
             if constexpr (PAIR) tc_commit_pair(bar);
             else tc_commit(bar);
@@ -1011,11 +990,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0);
             if (n_tiles == 0) continue;
-            wait_all(q_full, piece++);
+            wait(q_full, piece++);
             tc_fence_after();
             const uint32_t j0 = j;
             auto qk = [&](uint32_t t) {
-                wait_all(&k_full[t & 1u], t >> 1);
+                wait(&k_full[t & 1u], t >> 1);
                 tc_fence_after();
                 const uint64_t base = k_desc + (t & 1u) * (G::kOperand / 16);
                 const uint32_t to = tmem + kColS + (t & 1u) * kKeys;
@@ -1034,8 +1013,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             qk(j0);
             for (int32_t i = 0; i < n_tiles; ++i, ++j) {
                 if (i + 1 < n_tiles) qk(j + 1);
-                wait_all(&p_full[j & 1u], j >> 1);
-                wait_all(&v_full[j & 1u], j >> 1);
+                wait(&p_full[j & 1u], j >> 1);
+                wait(&v_full[j & 1u], j >> 1);
                 tc_fence_after();
                 const uint64_t base = v_desc + (j & 1u) * (G::kOperand / 16);
                 const uint32_t from = tmem + kColS + (j & 1u) * kKeys;
