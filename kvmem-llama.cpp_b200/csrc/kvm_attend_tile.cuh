@@ -50,16 +50,16 @@ struct TileGeom {
     using K = Slice<KT, D>;
     using V = Slice<VT, PAIR ? D / 2 : D>;                         // the dims of V that a CTA dequantizes
     static constexpr int kSlices = PAIR ? 2 : 1;                   // V slices a head
-    static constexpr int kBoxesV = PAIR ? 2 : 1;                   // 16-key boxes of V a warp and tile
+    static constexpr int kBoxesV = PAIR ? 2 : 1;                   // 16-key boxes of V a warp and tile (of K one)
     static constexpr int kOperand = 64 * D * 2;                    // a CTA's part of one K or V tile
     static constexpr int kQ = PAIR ? kTileRows * D * 2 : 0;        // Q in shared memory (else TMEM)
-    static constexpr int kRawK = kAttendBox * K::kStride, kRawV = kBoxesV * kAttendBox * V::kStride;   // a warp's rows of a tile
-    static constexpr int kRoom = 218 * 1024 - 4 * kOperand - kQ;
-    static constexpr int kFit = kRoom / (4 * (kRawK + kRawV));
-    static constexpr int kStages = kFit > 6 ? 6 : kFit < 1 ? 1 : kFit;
+    static constexpr int kBoxK = kAttendBox * K::kStride, kBoxV = kAttendBox * V::kStride;
+    static constexpr int kRoom = 220 * 1024 - 4 * kOperand - kQ;
+    static constexpr int kFit = kRoom / (4 * (kBoxK + kBoxV));
+    static constexpr int kStages = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;     // boxes a warp's raw ring holds
     static constexpr int kRaw = 4 * kOperand + kQ;                 // offset of the raw rings
-    static constexpr int kBars = kRaw + 4 * kStages * (kRawK + kRawV);
-    static constexpr int kSmem = kBars + 1024 + 1024;              // barriers; alignment of the operand tiles
+    static constexpr int kBars = kRaw + 4 * kStages * (kBoxK + kBoxV);
+    static constexpr int kSmem = kBars + 512 + 1024;               // barriers; alignment of the operand tiles
 };
 
 // ------------------------------------------------------------- tcgen05 PTX --
@@ -489,7 +489,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             mbar_init(&s_full[i], 1);
         }
         mbar_init(q_full, 8 * kCtas);
-        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], i < 4 * NS ? 1 : G::kBoxesV);
+        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
         s_odd = 0;
         fence_mbar_init();
     }
@@ -836,65 +836,64 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         }
         if (tid == 0 && rank == 0 && !described) desc->parts = 0;
     } else if (warp < 16) {
-        // ======== K (warps 8-11) and V (warps 12-15): raw rows to operand tiles
+        // ======== K (warps 8-11) and V (warps 12-15): raw rows to operand tiles, a box of 16 keys at
+        // a time; a tile is one box of every K warp and one or (V of a pair) two of every V warp
         const bool is_v = warp >= 12;
         const int w4 = warp & 3;
-        const int raw_bytes = is_v ? G::kRawV : G::kRawK;
-        uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kRawK : 0) + w4 * NS * raw_bytes;
+        const int raw_bytes = is_v ? G::kBoxV : G::kBoxK, boxes = is_v ? G::kBoxesV : 1;
+        uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kBoxK : 0) + w4 * NS * raw_bytes;
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
-        uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring stage of the next load, of the next tile
+        uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring slot of the next load, of the next box
+        // a pair's K warp also looks up the 16 keys that the peer's warp brings (their
+        // visibility is wanted here too): lane 1
+        constexpr int kLooks = kCtas;
+        const int32_t mine = is_v ? w4 * 16 * G::kBoxesV : static_cast<int32_t>(rank) * 64 + w4 * 16;
+        const int32_t theirs = is_v ? 0 : rank == 0 ? 64 : -64;
         while (next_piece()) {
-            const int32_t n_tiles = max(0, p.in1 - p.in0);
+            const int32_t n_tiles = max(0, p.in1 - p.in0), n_boxes = n_tiles * boxes;
             const int32_t *trow = a.table + p.seq * a.table_stride;
             const uint64_t slice = is_v ? (static_cast<uint64_t>(p.head) * G::kSlices + rank) * G::V::kBytes : static_cast<uint64_t>(p.head) * G::K::kBytes;
             const int lead = a.tma ? static_cast<int>(slice & 15u) : 0;
+            const int32_t x0 = static_cast<int32_t>(slice / 16u * 4u);
             uint32_t ring_ok[NS];                      // visible keys of the loads in flight
 #pragma unroll
             for (int i = 0; i < NS; ++i) ring_ok[i] = 0;
-            // the warp's keys of a tile: 16 from `mine` on, or (V of a pair) twice 16, bits 0-15
-            // and 16-31 of a mask
             const int32_t in0 = p.in0, kend = p.kend;
-            const int32_t mine = is_v ? w4 * 16 * G::kBoxesV : static_cast<int32_t>(rank) * 64 + w4 * 16;
-            const int boxes = is_v ? G::kBoxesV : 1;
-            // the second 16 keys of a mask: V's second box, or (K of a pair) those that the peer's
-            // warp brings, of which only the visibility is wanted here
-            const int32_t second = is_v ? 16 : rank == 0 ? 64 : -64;
-            constexpr int kLooks = kCtas;
-            // TMA: lane b brings box b; its table entry is fetched while the load before is issued
+            auto box_key = [&](int32_t i) -> int32_t {     // first key of box i
+                return G::kBoxesV == 2 && is_v ? (in0 + (i >> 1)) * kKeys + mine + 16 * (i & 1) : (in0 + i) * kKeys + mine;
+            };
+            // the table entry of box i, fetched while the load before is issued
             auto entry = [&](int32_t i) -> int32_t {
-                const int32_t key0 = (in0 + i) * kKeys + mine + second * lane;
-                return lane < kLooks && i < n_tiles && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
+                const int32_t key0 = box_key(i) + theirs * lane;
+                return lane < kLooks && i < n_boxes && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
             };
             int32_t slot_next = a.tma ? entry(0) : -1;
+            // every lane gets the box's visible keys, a bit each (bits 16-31: those of lane 1's)
             auto load = [&](int32_t i) -> uint32_t {
                 uint8_t *st = ring + in_at * raw_bytes;
                 uint64_t *bar = &full[in_at];
                 if (++in_at == NS) in_at = 0;
-                const int32_t first = (in0 + i) * kKeys + mine;
+                const int32_t first = box_key(i);
                 if (a.tma) {
                     uint32_t ok = 0;
-                    const int32_t slot = slot_next, key0 = first + second * lane, left = kend - key0;
+                    const int32_t slot = slot_next, key0 = first + theirs * lane, left = kend - key0;
                     slot_next = entry(i + 1);
-                    if (lane < kLooks) {
-                        if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
-                        if (lane < boxes) {
-                            if (ok != 0) {
-                                const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
-                                mbar_arrive_expect_tx(bar, raw_bytes / boxes);
-                                tma_load_2d(st + lane * (raw_bytes / boxes), is_v ? &a.map_v : &a.map_k, static_cast<int32_t>(slice / 16u * 4u),
-                                            static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
-                            } else {
-                                mbar_arrive(bar);
-                            }
+                    if (lane < kLooks && slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                    if (lane == 0) {
+                        if (ok != 0) {
+                            const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
+                            mbar_arrive_expect_tx(bar, raw_bytes);
+                            tma_load_2d(st, is_v ? &a.map_v : &a.map_k, x0, static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
+                        } else {
+                            mbar_arrive(bar);
                         }
                     }
                     return __shfl_sync(0xffffffffu, ok, 0) | (kLooks > 1 ? __shfl_sync(0xffffffffu, ok, 1) << 16 : 0u);
                 }
-                const int rows = 16 * boxes;
-                const uint32_t key = first + (kLooks > 1 ? (lane & 15) + second * (lane >> 4) : lane & 15);
+                const int32_t key = first + (kLooks > 1 ? (lane & 15) + theirs * (lane >> 4) : lane & 15);
                 int32_t cell = -1;
-                if (static_cast<int32_t>(key) < kend) {
-                    const uint32_t blk = attend_block(a, key);
+                if (key < kend) {
+                    const uint32_t blk = attend_block(a, static_cast<uint32_t>(key));
                     const int32_t slot = trow[blk];
                     if (slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots)
                         cell = static_cast<int32_t>(slot * a.block_tokens + (key - blk * a.block_tokens));
@@ -904,10 +903,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     using S = decltype(slice_t);
                     constexpr int C = S::kBytes / 4;
 #pragma unroll 4
-                    for (int y = 0; y < (rows * C + 31) / 32; ++y) {
-                        const int x = lane + 32 * y, r = min(x / C, rows - 1), c = x - r * C;
+                    for (int y = 0; y < (kAttendBox * C + 31) / 32; ++y) {
+                        const int x = lane + 32 * y, r = min(x / C, kAttendBox - 1), c = x - r * C;
                         const int32_t cr = __shfl_sync(0xffffffffu, cell, r);
-                        if (x < rows * C)
+                        if (x < kAttendBox * C)
                             cp_async4(smem_u32(st + r * S::kStride + c * 4), base + (cr >= 0 ? cr * row_bytes + c * 4 : 0ull), cr >= 0 ? 4u : 0u);
                     }
                 };
@@ -916,60 +915,57 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 return ok;
             };
 #pragma unroll
-            for (int i = 0; i < NS - 1; ++i) {
-                if (i < n_tiles) ring_ok[i] = load(i);
+            for (int i = 0; i < NS; ++i) {
+                if (i < n_boxes) ring_ok[i] = load(i);
                 cp_async_commit();
             }
 #pragma unroll 1
-            for (int32_t i = 0; i < n_tiles; ++i, ++j) {
-                if (NS == 1) ring_ok[0] = load(i);
+            for (int32_t i = 0; i < n_boxes; ++i) {
+                const bool last = G::kBoxesV == 1 || !is_v || (i & 1);     // ... of its tile
                 if (a.tma) wait(&full[out_at], out_phase);
-                else if (NS == 1) cp_async_commit(), cp_async_wait<0>();
-                else cp_async_wait<(NS > 1 ? NS - 2 : 0)>();
+                else cp_async_wait<NS - 1>();
                 __syncwarp();
                 const uint32_t ok = ring_ok[0];
-#pragma unroll
-                for (int k = 0; k + 1 < NS; ++k) ring_ok[k] = ring_ok[k + 1];
-                if (NS > 1) {
-                    if (i + NS - 1 < n_tiles) ring_ok[NS - 2 < 0 ? 0 : NS - 2] = load(i + NS - 1);
-                    cp_async_commit();
-                }
                 uint8_t *raw = ring + out_at * raw_bytes + lead;
-                constexpr int kVD = PAIR ? D / 2 : D, kBoxV = kAttendBox * G::V::kStride;
-                if (is_v) {
-#pragma unroll
-                    for (int b = 0; b < G::kBoxesV; ++b)
-                        if (((ok >> (16 * b)) & 0xffffu) != 0xffffu) tile_clean<VT, kVD, false>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
-                } else if ((ok & 0xffffu) != 0xffffu) {
-                    tile_clean<KT, D, false>(raw, ok & 0xffffu, lane);
-                }
-                if (j >= 2) wait(&tile_free[j & 1u], (j >> 1) - 1u);
                 if (++out_at == NS) {
                     out_at = 0;
                     out_phase ^= 1u;
                 }
+                constexpr int kVD = PAIR ? D / 2 : D;
+                if ((ok & 0xffffu) != 0xffffu) {
+                    if (is_v) tile_clean<VT, kVD, false>(raw, ok & 0xffffu, lane);
+                    else tile_clean<KT, D, false>(raw, ok & 0xffffu, lane);
+                }
+                if (j >= 2 && (G::kBoxesV == 1 || !is_v || !(i & 1))) wait(&tile_free[j & 1u], (j >> 1) - 1u);
                 uint8_t *tile = smem + (is_v ? 2 * G::kOperand : 0) + (j & 1u) * G::kOperand;
                 if (is_v) {
-#pragma unroll
-                    for (int b = 0; b < G::kBoxesV; ++b)
-                        if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw + b * kBoxV, tile, mine + 16 * b, lane))) {
-                            // the epilogue adds what is not finite; the products do without it
-                            tile_clean<VT, kVD, true>(raw + b * kBoxV, (ok >> (16 * b)) & 0xffffu, lane);
-                            tile_dequant<VT, kVD, kKeys>(raw + b * kBoxV, tile, mine + 16 * b, lane);
-                            if constexpr (PAIR) {
-                                if (lane < kCtas) st_shared_at(&s_odd, 1u, lane);
-                                asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                            } else {
-                                *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
-                            }
+                    const int at = w4 * 16 * G::kBoxesV + (G::kBoxesV == 2 ? 16 * (i & 1) : 0);
+                    if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane))) {
+                        // the epilogue adds what is not finite; the products do without it
+                        tile_clean<VT, kVD, true>(raw, ok & 0xffffu, lane);
+                        tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane);
+                        if constexpr (PAIR) {
+                            if (lane < kCtas) st_shared_at(&s_odd, 1u, lane);
+                            asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                        } else {
+                            *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
                         }
+                    }
                 } else {
                     tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
-                    if (lane < kLooks) valid[(kKeys / 16) * (j & 3u) + (mine + second * lane) / 16] = (ok >> (16 * lane)) & 0xffffu;
+                    if (lane < kLooks) valid[(kKeys / 16) * (j & 3u) + (mine + theirs * lane) / 16] = (ok >> (16 * lane)) & 0xffffu;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive(&tile_full[j & 1u]);
+                if (last) {
+                    if (lane == 0) arrive(&tile_full[j & 1u]);
+                    ++j;
+                }
+                // the box is read: its slot takes the one NS ahead
+#pragma unroll
+                for (int k = 0; k + 1 < NS; ++k) ring_ok[k] = ring_ok[k + 1];
+                if (i + NS < n_boxes) ring_ok[NS - 1] = load(i + NS);
+                cp_async_commit();
             }
             cp_async_wait<0>();
             __syncwarp();
