@@ -845,7 +845,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
         uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring slot of the next load, of the next box
         // a pair's K warp also looks up the 16 keys that the peer's warp brings (their
-        // visibility is wanted here too): lane 1
+        // visibility is wanted here too)
         constexpr int kLooks = kCtas;
         const int32_t mine = is_v ? w4 * 16 * G::kBoxesV : static_cast<int32_t>(rank) * 64 + w4 * 16;
         const int32_t theirs = is_v ? 0 : rank == 0 ? 64 : -64;
@@ -862,35 +862,42 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             auto box_key = [&](int32_t i) -> int32_t {     // first key of box i
                 return G::kBoxesV == 2 && is_v ? (in0 + (i >> 1)) * kKeys + mine + 16 * (i & 1) : (in0 + i) * kKeys + mine;
             };
-            // the table entry of box i, fetched while the load before is issued
-            auto entry = [&](int32_t i) -> int32_t {
-                const int32_t key0 = box_key(i) + theirs * lane;
-                return lane < kLooks && i < n_boxes && key0 < kend ? trow[attend_block(a, static_cast<uint32_t>(key0))] : -1;
+            // rows and visible keys of 32 boxes, a box a lane: looking them up one by one exposed
+            // the table's latency at every load (900 cycles)
+            int32_t box_row = 0;
+            uint32_t box_ok = 0;
+            auto look = [&](int32_t i) {
+                box_ok = 0;
+#pragma unroll
+                for (int c = 0; c < kCtas; ++c) {
+                    const int32_t key0 = box_key(i) + (c ? theirs : 0), left = kend - key0;
+                    const uint32_t blk = attend_block(a, static_cast<uint32_t>(max(key0, 0)));
+                    const int32_t slot = i < n_boxes && left > 0 ? trow[blk] : -1;
+                    const bool here = slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots;
+                    if (here) box_ok |= (left >= 16 ? 0xffffu : (1u << left) - 1u) << (16 * c);
+                    if (c == 0 && here) box_row = static_cast<int32_t>(slot * a.block_tokens + (static_cast<uint32_t>(key0) - blk * a.block_tokens));
+                }
             };
-            int32_t slot_next = a.tma ? entry(0) : -1;
             // every lane gets the box's visible keys, a bit each (bits 16-31: those of lane 1's)
             auto load = [&](int32_t i) -> uint32_t {
                 uint8_t *st = ring + in_at * raw_bytes;
                 uint64_t *bar = &full[in_at];
                 if (++in_at == NS) in_at = 0;
-                const int32_t first = box_key(i);
                 if (a.tma) {
-                    uint32_t ok = 0;
-                    const int32_t slot = slot_next, key0 = first + theirs * lane, left = kend - key0;
-                    slot_next = entry(i + 1);
-                    if (lane < kLooks && slot >= 0 && static_cast<uint32_t>(slot) < a.n_slots) ok = left >= 16 ? 0xffffu : (1u << left) - 1u;
+                    if ((i & 31) == 0) look(i + lane);
+                    const uint32_t ok = __shfl_sync(0xffffffffu, box_ok, i & 31);
+                    const int32_t row = __shfl_sync(0xffffffffu, box_row, i & 31);
                     if (lane == 0) {
-                        if (ok != 0) {
-                            const uint32_t in_block = static_cast<uint32_t>(key0) - attend_block(a, static_cast<uint32_t>(key0)) * a.block_tokens;
+                        if (ok & 0xffffu) {
                             mbar_arrive_expect_tx(bar, raw_bytes);
-                            tma_load_2d(st, is_v ? &a.map_v : &a.map_k, x0, static_cast<int32_t>(slot * a.block_tokens + in_block), bar);
+                            tma_load_2d(st, is_v ? &a.map_v : &a.map_k, x0, row, bar);
                         } else {
                             mbar_arrive(bar);
                         }
                     }
-                    return __shfl_sync(0xffffffffu, ok, 0) | (kLooks > 1 ? __shfl_sync(0xffffffffu, ok, 1) << 16 : 0u);
+                    return ok;
                 }
-                const int32_t key = first + (kLooks > 1 ? (lane & 15) + theirs * (lane >> 4) : lane & 15);
+                const int32_t key = box_key(i) + (kLooks > 1 ? (lane & 15) + theirs * (lane >> 4) : lane & 15);
                 int32_t cell = -1;
                 if (key < kend) {
                     const uint32_t blk = attend_block(a, static_cast<uint32_t>(key));
