@@ -183,7 +183,7 @@ __device__ __forceinline__ void write_side(const RowsArgs &a, const RowsSide &s,
 }
 
 template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads) write_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, 4) write_rows_kernel(const __grid_constant__ RowsArgs a) {
     __shared__ __align__(16) uint8_t stage[kRowsThreads * kBlockBytesQ8];
     const RowsSide &s = a.side[blockIdx.y];
     if (!s.on) return;
