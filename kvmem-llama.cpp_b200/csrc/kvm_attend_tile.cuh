@@ -99,6 +99,9 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
         ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
+__device__ __forceinline__ void mbar_arrive_n(uint64_t *bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
 // Arrives on the barrier at the same offset in CTA `rank` of the cluster.  What the
 // arrival announces lies in this SM (TMEM, shared memory) and has been completed by
 // tcgen05.wait or a proxy fence before; a cluster-scope release would wait for every
@@ -601,8 +604,25 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
             return at[(wg ^ 1) * kTileRows + row];
         };
+        auto vote = [&](uint64_t *bar, uint32_t n) {
+            if constexpr (PAIR) mbar_arrive_at(bar, 0);
+            else mbar_arrive_n(bar, n);
+        };
         bool described = false;
         while (next_piece()) {
+            // Warps without a row of the piece (drafts fill one or two of the four pairs) would
+            // only take the others' issue slots: they sleep on a named barrier, and the first
+            // pair arrives for them.  A pair of CTAs is only used for longer requests.
+            const uint32_t idle = PAIR ? 0u : 4u - min(4u, (p.rows + 31u) / 32u);
+            const uint32_t votes = (warp & 3) == 0 ? 1u + idle : 1u;
+            auto sleep = [&]() {
+                if (idle) asm volatile("bar.sync 5, 256;" ::: "memory");
+            };
+            if (!PAIR && static_cast<uint32_t>(warp & 3) * 32u >= p.rows) {
+                j += static_cast<uint32_t>(max(0, p.in1 - p.in0));
+                sleep();
+                continue;
+            }
             const uint32_t item_row = rank * kTileRows + row;
             const bool in = item_row < p.rows;
             const uint32_t rr = p.first + (in ? item_row : 0), tok = rr / a.group;
@@ -669,7 +689,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             else tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0 && work) arrive(q_full);
+            if (lane == 0 && work) vote(q_full, votes);
 
             float m = kNegInf, l = 0.0f;
             const uint32_t j0 = j;
@@ -749,7 +769,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&p_full[st]);
+                if (lane == 0) vote(&p_full[st], votes);
             }
             // ---- epilogue
             const bool any = j != j0;
@@ -833,6 +853,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 desc->parts = 1u + p.more;
             }
             described = described || (p.starts && !p.ends);
+            sleep();
         }
         if (tid == 0 && rank == 0 && !described) desc->parts = 0;
     } else if (warp < 16) {
