@@ -614,8 +614,8 @@ kvm_status kvm_qk_norm_rope(kvm_stream stream, uint32_t n, const kvm_rows *q, co
  * Quantize row i of k and v (F32, F16 or BF16) into cell d_cells[i], with the
  * arithmetic and bytes of ggml's quantize_row_*_ref in 32 bits
  * (kvm_quantize_rows for F16 rows).  A cell outside [0, n_slots*block_tokens)
- * skips the row.  k or v may be NULL.  Rows that share a cell leave a mixture
- * of their blocks there.
+ * skips the row.  k or v may be NULL.  A cell named twice ends up undefined
+ * (a mixture of both rows' bytes); the others are not touched by that.
  */
 kvm_status kvm_write_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
                           const int64_t *d_cells, const kvm_rows *k, const kvm_rows *v);
@@ -638,6 +638,10 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * to no request stay as they were.  Query head h reads KV head
  * h / (n_head / n_head_kv).  q and out: F16 or BF16, head_dim 64, 128 or 256.
  * Scores, maxima and sums are F32; the weights enter the second product in F16.
+ * In requests of more than 16 rows a KV head, K and V values enter the products
+ * rounded to F16 (2^-11): quantized values beyond 65504 become infinite there.
+ * out must not overlap q, the cache or the workspace.  Waits inside the kernels
+ * are bounded (2 s); one that runs out leaves NaN, never a hang.
  * max_new: the most rows of a request, as far as the caller knows (it picks the
  * kernel; a wrong value costs time, not correctness).
  * d_work: KVM_ATTEND_WORK_BYTES of device memory, 16-byte aligned, that no

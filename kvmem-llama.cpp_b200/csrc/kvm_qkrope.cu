@@ -13,9 +13,14 @@
 // pair that a rotation mixes (8 values and their partners n_rot/2 further on), so
 // the rotation needs no exchange and the norm only a reduction over the head's
 // head_dim/16 neighbouring threads.  A CTA takes one to four tokens at a time, all
-// heads: its threads first issue the loads of up to four heads each (8 vectors in
-// flight), then form the tokens' cos / sin once for all heads, in shared memory,
-// while those loads are under way.  Weights stay in registers across the tokens.
+// heads: its threads first issue the loads of two heads each (four vectors; 64
+// registers and so four CTAs an SM, which beat eight vectors at three), then form
+// the tokens' cos / sin once for all heads, in shared memory, while those loads
+// are under way.  The query weights stay in registers across the tokens.
+//
+// 8192 tokens of 24 + 4 heads of 256, BF16, all rotated: 51 us for 235 MB = 4.6 TB/s
+// (a copy 36 us): issue slots 59 % busy, norm and rotation cost 18 instructions a
+// pair of values.  64 tokens: 4.2 us, launch and two dependent loads.
 #include <cuda_bf16.h>
 
 #include <algorithm>
