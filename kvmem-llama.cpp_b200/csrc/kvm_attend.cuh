@@ -87,11 +87,6 @@ __device__ __forceinline__ uint32_t attend_block(const AttendArgs &a, uint32_t k
     return a.block_shift < 32u ? key >> a.block_shift : key / a.block_tokens;
 }
 
-__device__ __forceinline__ float load16(const uint8_t *p, int32_t bf16) {
-    const uint16_t u = *reinterpret_cast<const uint16_t *>(p);
-    return bf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(__ushort_as_half(u));
-}
-
 __device__ __forceinline__ void store16(uint8_t *p, float x, int32_t bf16) {
     *reinterpret_cast<uint16_t *>(p) = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x))
                                             : __half_as_ushort(__float2half_rn(x));

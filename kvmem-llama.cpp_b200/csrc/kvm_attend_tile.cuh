@@ -1,13 +1,13 @@
-// kvm_attend_tile.cuh -- attend_tile_kernel: attention for many query rows a
-// sequence (prompt chunks, drafts), bound by the tensor cores.
+// kvm_attend_tile.cuh -- attend_tile_kernel, attend_pair_kernel: attention for
+// many query rows a sequence (prompt chunks, drafts).
 //
-// A work item is 128 rows (token, query head of one KV head) against the keys
-// they see, 64 keys at a time:
-//     S = Q K^T  (128 x 64, tcgen05, Q from TMEM, K from shared memory)
-//     P = exp2(S * f - m)             -> F16 in TMEM, over S
-//     O += P V   (128 x D, tcgen05, P from TMEM, V from shared memory)
+// A work item is a tile of rows (token, query head of one KV head) against the
+// keys they see, one key tile at a time:
+//     S = Q K^T              (tcgen05, K from shared memory)
+//     P = exp2(S * f - m)    -> F16 in TMEM, over S
+//     O += P V               (tcgen05, P from TMEM, V from shared memory)
 // K and V enter as F16 values code * d, rounded once: unlike the few-row kernel
-// this one is not bound by the window's bytes, and dequantizing once for 128
+// this one is not bound by the window's bytes, and dequantizing once for all
 // rows leaves the tensor cores plain F16 operands.  Q is scaled a row by a power
 // of two (exact for 16-bit inputs but for elements 2^24 below the row's
 // largest), P is F16, all sums and statistics are F32.  The running maximum is
@@ -15,25 +15,47 @@
 // rarely; P carries a factor 2^7 that cancels in the quotient, which keeps it
 // below F16's top and its bits down to 2^-31 of the row's largest weight.
 //
-// Roles (17 warps, one CTA an SM): warps 0-7 own the 128 rows (Q into TMEM,
-// softmax, epilogue), two threads a row with half the columns each; warps 8-11
-// turn raw K rows into an operand tile, warps 12-15 raw V rows, warp 16 issues
-// the products.  (One thread a row left a single softmax warp on each scheduler,
-// whose latencies alone took 2250 cycles a tile.)  Everything is double-buffered on
-// mbarriers: QK of tile j + 1 is issued before PV of tile j, so that the softmax
-// of one tile runs under the products of the other.  With D = 256: S 2 x 64,
-// O 256 and Q 128 columns are all of TMEM; Q there rather than in shared memory
-// halves what QK reads from shared memory, which would otherwise bound it at
-// N = 64 (A 4 KB + B 2 KB an instruction of 32 cycles, at 128 bytes a cycle).
+// Two shapes.
+//  - One CTA (attend_tile_kernel): 128 rows, 64 keys a tile, Q in TMEM.  With D = 256
+//    S 2 x 64, O 256 and Q 128 columns are all of TMEM; Q there rather than in
+//    shared memory halves what S = Q K^T reads from it (A 4 KB + B 2 KB an instruction
+//    otherwise, at 128 bytes a cycle).  An instruction of 128 x 64 x 16 takes 57
+//    cycles, not the 32 of its rate.
+//  - A pair of CTAs (attend_pair_kernel, quantized K and V of 128 or 256 dims, more
+//    than 128 rows): 256 rows, 128 keys a tile by cta_group::2.  128 x 128 x 16 takes
+//    65 cycles a CTA, so the pair nearly doubles the rate of S = Q K^T, and each CTA dequantizes
+//    only half of every tile (64 keys of K, half of V's dims) for 256 rows.  Q is in
+//    shared memory there: 2 x 128 columns of S and 256 of O fill TMEM.
+//    2048 tokens behind a window of 32768 keys (24 heads of 256, q4_0): 2.29 ms by
+//    single CTAs, 1.56 ms by pairs.
 //
-// Operand tiles: rows of 64 keys by 128-byte chunks of 64 dims with the 128-byte
+// Roles (17 warps, one CTA an SM): warps 0-7 own 128 rows (Q, softmax, epilogue),
+// two threads a row with half the columns each; warps 8-11 turn raw K rows into an
+// operand tile, warps 12-15 raw V rows, warp 16 issues the products.  (One thread a
+// row left a single softmax warp on each scheduler, whose latencies alone took 2250
+// cycles a tile.  25 warps leave 72 registers a thread: slower, they spill.)
+// Everything is double-buffered on mbarriers: S of tile j + 1 is issued before O of
+// tile j, so that the softmax of one tile runs under the products of the other.
+// Raw rows come through a ring a warp, 16 keys a slot, refilled as soon as a slot
+// is read; the table is looked up for 32 boxes at a time.
+//
+// What bounds it now.  Pairs: a 128-key tile takes 4100 cycles, of which the tensor
+// cores are busy for 53 %; the longest chain is a V warp's two boxes (1600 cycles
+// each: 850 of conversion, the rest barriers, fences and the load's issue), with the
+// softmax warps (3100) behind it.  Giving every dequantizing warp a box of K and
+// one of V, half the dims each, was slower (1.67 ms).  Drafts (8 requests of 4
+// tokens, 80,000 keys): 87 us against 14 for their bytes (90 while the warps without
+// rows worked and polled along).  The time hardly depends on the rows (8 tokens
+// 83 us): a 64-key tile costs 4000 cycles, 2100 of them a box's conversion.
+//
+// Operand tiles: rows of keys by 128-byte chunks of 64 dims with the 128-byte
 // swizzle; K is read K-major, V from the same layout MN-major.  Which dim a
 // position stands for is free as long as Q (for K) and the epilogue (for V)
 // agree: q4_0 and q5_0 keep the order their nibbles fall out in (position i of
 // eight holds value 0 2 1 3 4 6 5 7).
 //
 // The (item, key tile) pairs of the call form one line, shared evenly by the
-// CTAs; an item that several CTAs share leaves its pieces' maxima, sums and
+// CTAs or pairs; an item that several share leaves its pieces' maxima, sums and
 // normalised F16 outputs (one rounding as large as the output's own) for
 // attend_tile_join_kernel.
 #pragma once
