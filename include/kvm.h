@@ -632,7 +632,8 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  *     out = softmax(scale * q k^T) v   over the keys a row sees:
  * all of them, or with KVM_ATTEND_CAUSAL key j of row i (of n) when
  * j <= kv_len - n + i.  A row that sees no key is 0.  Keys beyond the table's
- * columns and keys of a block whose entry is outside [0, n_slots) are not seen.
+ * columns, keys from 2^31 - 65536 on and keys of a block whose entry is outside
+ * [0, n_slots) are not seen.
  * What hidden keys hold -- stale bytes, infinities, NaN -- reaches no output.
  * Rows of q_start outside [0, n_rows) are skipped, and rows of out that belong
  * to no request stay as they were.  Query head h reads KV head

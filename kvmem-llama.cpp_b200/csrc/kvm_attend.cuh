@@ -52,6 +52,10 @@ struct AttendArgs {
 // box_rows rows by box_bytes.  False when the driver cannot make it.
 bool attend_map(CUtensorMap *map, const void *base, uint64_t row_bytes, const AttendArgs &a, uint32_t box_bytes, uint32_t box_rows);
 
+// Keys of a request at most: a step or tile may reach some thousand keys past the
+// last one, and their numbers are 32-bit.
+constexpr int64_t kAttendMostKeys = 0x7fff0000;
+
 // A sequence as the kernels see it; nothing read from device memory is trusted
 // to stay inside the tables.
 struct AttendSeq {
@@ -71,7 +75,7 @@ __host__ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, ui
     q.n_new = (lo < 0 || n <= 0 || lo >= a.n_rows)
                   ? 0 : static_cast<int32_t>(min(n, static_cast<int64_t>(a.n_rows) - lo));
     q.shift = static_cast<int32_t>(max(kv - n, static_cast<int64_t>(-0x40000000)));
-    q.keys = static_cast<int32_t>(min(kv, min(cap, static_cast<int64_t>(0x7fffff00))));
+    q.keys = static_cast<int32_t>(min(kv, min(cap, kAttendMostKeys)));
     return q;
 }
 
@@ -79,7 +83,7 @@ __host__ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs &a, ui
 __host__ __device__ __forceinline__ int32_t attend_limit(const AttendArgs &a, const AttendSeq &q, int32_t i) {
     if (!a.causal) return q.keys;
     return max(0, min(q.keys, static_cast<int32_t>(min(static_cast<int64_t>(q.shift) + i + 1,
-                                                       static_cast<int64_t>(0x7fffff00)))));
+                                                       kAttendMostKeys))));
 }
 
 // Block of a key.

@@ -197,3 +197,24 @@ def test_cells_past_four_gigabytes(kvm_lib, T):
             outs[-1].append(out)
     assert all(torch.equal(a, b) for a, b in zip(*outs))
     assert outs[0][2].any() and (outs[0][0].float() - k.float()).abs().max() < 0.05
+
+
+@pytest.mark.parametrize("D, new", [(64, 1), (64, 20), (128, 130)])
+def test_lengths_up_to_the_last_key_number(kvm_lib, D, new):
+    """A table of 2^31 keys of which two blocks hold any, the second at its very end:
+    key numbers stay inside 32 bits, and keys from 2^31 - 65536 on are not seen."""
+    import layer_ref as ref
+    import torch
+    T, cols = 4096, 524288
+    w = Window(kvm_lib, torch, D, ("q4_0", "q4_0"), 1, D, T, [2 * T], spare=1)
+    table = np.full((1, cols), -1, np.int32)
+    table[0, 0], table[0, cols - 17], table[0, cols - 16:] = 0, 1, 2      # 17 blocks are 65536 + T keys
+    q = queries(torch, w.rng, new, 1, D, "f16")
+    got = w.run(q, [0, new], False, max_new=new, kv_len=[2 ** 31 - 1], table=table).float().cpu().numpy()
+    near = np.array([[0, 1]], np.int32)
+    w.table = near
+    same = w.check(q, [0, new], False, max_new=new, kv_len=[2 * T]).float().cpu().numpy()
+    # both sum the same keys, in other places: each is off by what the check allows
+    _, spread, _ = ref.attend(q.float().cpu().numpy(), w.raw[0], w.raw[1], w.kinds, 1, T, w.slots, near, [0, new], [2 * T],
+                              D ** -0.5, False, np.zeros(q.shape))
+    assert (np.abs(got - same) <= spread * 2.0 ** -8 + np.abs(same) * 2.0 ** -10 + 2.0 ** -24).all()
