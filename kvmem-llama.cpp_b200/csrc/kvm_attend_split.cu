@@ -25,7 +25,7 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
     attend_split_kernel<D, KT, VT, NT><<<grid, G::kThreads, smem, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || grid == 1 || a.whole) return e;
-    return launch_after_prev(attend_join_kernel<D, NT>, dim3(std::min<uint32_t>(2u * num_sms(), grid * 8u * NT * a.heads_cta)), dim3(kJoinThreads), 0, st, a, grid);
+    return launch_after_prev(attend_join_kernel<D, NT>, dim3(std::min<uint32_t>(2u * num_sms(), grid * 8u * NT * a.heads_cta * (D / 64))), dim3(kJoinThreads), 0, st, a, grid);
 }
 
 template <int D, int KT, int VT>

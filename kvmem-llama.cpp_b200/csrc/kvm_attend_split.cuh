@@ -954,7 +954,8 @@ __device__ __forceinline__ void join_list(const AttendArgs &a, uint32_t ctas, ui
     uint32_t before = 0;
     for (uint32_t base = 0; base < ctas; base += kJoinThreads) {
         const uint32_t c = base + threadIdx.x;
-        uint32_t x = c < ctas && desc[c].parts ? desc[c].rows * heads : 0u;
+        const uint32_t parts = c < ctas ? desc[c].parts : 0u, rows = c < ctas ? desc[c].rows : 0u;
+        uint32_t x = parts ? rows * heads : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -984,68 +985,90 @@ __device__ __forceinline__ uint32_t join_find(const JoinList &list, uint32_t cta
     return c;
 }
 
-// One (head, row) of a split segment at a time: the parts of a segment that
-// starts in CTA c lie in slot 2c + 1, then 2(c + 1), 2(c + 2), ...  They are
-// spread over groups of D / 4 threads, four dims a thread, and added in a fixed
-// order.
+// One (head, row) of a split segment at a time, or, while that leaves CTAs idle, 64
+// dims of it: the parts of a segment that starts in CTA c lie in slot 2c + 1, then
+// 2(c + 1), 2(c + 2), ...  They are spread over groups of threads, four dims a
+// thread, and added in a fixed order.  A decode step of one request is 24 rows of 148
+// parts: bound by the chain of dependent reads, so a part's maximum, sum and first
+// values are asked for together.
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a, uint32_t ctas) {
-    constexpr int R = 8 * NT, G = kJoinThreads / (D / 4);
-    __shared__ float weight[kAttendMaxCtas], s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
-    __shared__ float4 s_acc[G][D / 4];
+    constexpr int R = 8 * NT, W = kJoinThreads / 32, kEarly = 6;
+    static_assert(kAttendMaxCtas <= 2 * kJoinThreads, "two parts a thread");
+    __shared__ float weight[2 * kJoinThreads], s_top[W], s_sum[W];
+    __shared__ float4 s_acc[kJoinThreads];
     __shared__ JoinList list;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     join_list(a, ctas, a.heads_cta, list);
-    for (uint32_t at = blockIdx.x; at < list.total; at += gridDim.x) {
+    const uint32_t slices = list.total * (D / 64) <= gridDim.x ? D / 64 : 1u;
+    const uint32_t wide = D / 4 / slices, groups = kJoinThreads / wide;        // threads a part, parts at a time
+    const uint32_t grp = tid / wide, at_dim = tid % wide;
+    for (uint32_t item = blockIdx.x; item < list.total * slices; item += gridDim.x) {
+        const uint32_t d = item % slices * wide + at_dim;                      // of D / 4
         uint32_t hr;
-        const uint32_t c = join_find(list, ctas, at, &hr);
+        const uint32_t c = join_find(list, ctas, item / slices, &hr);
         const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + c;
         const uint32_t parts = min(desc->parts, ctas), hs = hr / desc->rows, r = hr - hs * desc->rows;
         auto part = [&](uint32_t i) { return attend_part<D, NT>(a, i ? 2u * (c + i) : 2u * c + 1u, hs); };
-        float top = -__builtin_huge_valf();
-        for (uint32_t i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, weight[i] = part(i)[r]);
+        // rows start at 2 R floats behind a multiple of 16 bytes, D floats apart
+        auto values = [&](uint32_t i) { return *reinterpret_cast<const float4 *>(part(i) + 2 * R + r * D + 4 * d); };
+        float m[2], l[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t i = tid + k * kJoinThreads;
+            m[k] = i < parts ? part(i)[r] : -__builtin_huge_valf();
+            l[k] = i < parts ? part(i)[R + r] : 0.0f;
+        }
+        float4 early[kEarly];
+#pragma unroll
+        for (int k = 0; k < kEarly; ++k) {
+            const uint32_t i = grp + k * groups;
+            early[k] = i < parts ? values(i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float top = fmaxf(m[0], m[1]);
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) s_top[warp] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, s_top[w]);
         const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
         float sum = 0.0f;
-        for (uint32_t i = tid; i < parts; i += kJoinThreads) {
-            const float f = exp2_approx(weight[i] - ref);
-            weight[i] = f;
-            sum += f * part(i)[R + r];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float f = exp2_approx(m[k] - ref);
+            weight[tid + k * kJoinThreads] = f;
+            sum += f * l[k];
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_sum[warp] = sum;
         __syncthreads();
-        const int grp = tid / (D / 4), d = tid % (D / 4);
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (uint32_t i = grp; i < parts; i += G) {
+        auto add = [&](uint32_t i, const float4 &x) {
             const float f = weight[i];
-            // rows start at 2 R floats behind a multiple of 16 bytes, D floats apart
-            const float4 x = *reinterpret_cast<const float4 *>(part(i) + 2 * R + r * D + 4 * d);
             acc.x += f * x.x;
             acc.y += f * x.y;
             acc.z += f * x.z;
             acc.w += f * x.w;
-        }
-        s_acc[grp][d] = acc;
+        };
+#pragma unroll
+        for (int k = 0; k < kEarly; ++k)
+            if (grp + k * groups < parts) add(grp + k * groups, early[k]);
+#pragma unroll 4
+        for (uint32_t i = grp + kEarly * groups; i < parts; i += groups) add(i, values(i));
+        s_acc[tid] = acc;
         __syncthreads();
-        if (tid < D) {
-            float o = 0.0f, l = 0.0f;
+        if (tid < 4 * wide) {
+            float o = 0.0f, l_all = 0.0f;
+            for (uint32_t k = 0; k < groups; ++k) o += reinterpret_cast<const float *>(s_acc + k * wide)[tid];
 #pragma unroll
-            for (int k = 0; k < G; ++k) o += reinterpret_cast<const float *>(s_acc[k])[tid];
-#pragma unroll
-            for (int w = 0; w < kJoinThreads / 32; ++w) l += s_sum[w];
-            const uint32_t rr = desc->first + r, tok = rr / a.group;
+            for (int w = 0; w < W; ++w) l_all += s_sum[w];
+            const uint32_t rr = desc->first + r, tok = rr / a.group, dim = item % slices * 4u * wide + tid;
             store16(const_cast<uint8_t *>(a.out.p) + (static_cast<uint64_t>(desc->row0) + tok) * a.out.nb_tok +
-                        (static_cast<uint64_t>(desc->head + hs) * a.group + rr % a.group) * a.out.nb_head + tid * a.out.nb_dim,
-                    l == 0.0f ? 0.0f : o / l, a.out.bf16);
+                        (static_cast<uint64_t>(desc->head + hs) * a.group + rr % a.group) * a.out.nb_head + dim * a.out.nb_dim,
+                    l_all == 0.0f ? 0.0f : o / l_all, a.out.bf16);
         }
         __syncthreads();
     }
