@@ -155,6 +155,7 @@ __device__ __forceinline__ bool mbar_wait_near(uint64_t *bar, uint32_t parity) {
 constexpr int kAttendBox = 16;                // rows of a TMA box
 constexpr int kAttendMinSteps = 4;            // steps of 16 keys that a warp takes at least
 constexpr int kAttendSegmentSteps = 24;       // steps of 16 keys that beginning a segment is worth
+constexpr int kAttendWholeSteps = 4;          // steps of a warp up to which a short window is not cut
 constexpr uint32_t kAttendMaxCtas = 592;      // descriptors in the workspace
 constexpr uint32_t kAttendDescBytes = 32;
 struct AttendDesc {                           // segment that starts in CTA c and goes on in c + 1 ...

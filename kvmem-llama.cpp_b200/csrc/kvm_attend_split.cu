@@ -18,10 +18,21 @@ cudaError_t launch(AttendArgs a, uint32_t grid, cudaStream_t st) {
         return cudaErrorInvalidValue;
     if (a.tma && !(attend_map(&a.map_k, a.k, a.row_k, a, G::K::kStride, kAttendBox) && attend_map(&a.map_v, a.v, a.row_v, a, G::V::kStride, kAttendBox)))
         a.tma = 0;
+    // Windows of a few steps a warp (kAttendWholeSteps) whose (request, head) pairs are
+    // hardly more than the SMs: a KV head a CTA, nothing cut.  A CTA then begins one or two
+    // segments instead of parts of several, and there is no join: 2 requests of 333 keys
+    // (4 heads of 256) 27 us by four heads a CTA, cut, and 13.6 us so; 64 of 1024 55 and
+    // 39 us; 2 of 1024 22.6 and 20.4.
+    const uint64_t steps = (a.max_keys + static_cast<uint64_t>(G::kStep) - 1u) / G::kStep;
+    const bool alone = steps <= static_cast<uint64_t>(kAttendWholeSteps * G::kWarps) && static_cast<uint64_t>(a.n_seq) * a.n_head_kv <= 2u * num_sms();
+    if (alone) {
+        a.heads_cta = 1;
+        grid = std::min<uint32_t>(num_sms(), kAttendMaxCtas);
+    }
     const uint64_t slot = static_cast<uint64_t>(a.heads_cta) * attend_part_floats<D, NT>() * 4u;
     grid = static_cast<uint32_t>(std::min<uint64_t>(grid, (KVM_ATTEND_WORK_BYTES - kAttendMaxCtas * kAttendDescBytes) / (2 * slot)));
     // segments that the least share would hold whole are not cut at all
-    a.whole = (a.max_keys + G::kStep - 1u) / G::kStep <= static_cast<uint32_t>(kAttendMinSteps / G::kTiles * (G::kWarps / a.heads_cta));
+    a.whole = alone || steps <= static_cast<uint64_t>(kAttendMinSteps / G::kTiles * (G::kWarps / a.heads_cta));
     attend_split_kernel<D, KT, VT, NT><<<grid, G::kThreads, smem, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || grid == 1 || a.whole) return e;

@@ -39,9 +39,10 @@
 // and q4_0 values: 78 us = 3.7 TB/s.  Not the bytes bound it (87 and 44 us) but the
 // instructions around the products: a 16-key step costs 12 warps a scheduler's 52 %
 // of issue slots and 30 % of the tensor pipe, whose m16n8k16 takes 8 cycles for 8
-// rows of N of which 6 are used.  One request of 32768 keys: 30 us, 13 of them the
-// join, the launches and the first loads.  With 16 rows (two products a code)
-// the time is 1.6 times that of 8.
+// rows of N of which 6 are used.  One request of 32768 keys: 24 us, 11 of them a
+// CTA's (queries and first rows 5, steps 3, merge 2), the rest launches and the join.
+// 2 requests of up to 333 keys (2 heads of 128): 10 us.  With 16 rows (two products a
+// code) the time is 1.6 times that of 8.
 #pragma once
 
 #include "kvm_attend.cuh"
