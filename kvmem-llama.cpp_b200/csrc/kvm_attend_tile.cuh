@@ -1111,23 +1111,40 @@ __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __
         const AttendDesc *desc = reinterpret_cast<const AttendDesc *>(a.work) + c;
         const uint32_t parts = min(desc->parts, ctas), d8 = threadIdx.x % kGroup;
         auto part = [&](uint32_t i) { return tile_part<D, ROWS>(a, i ? 2u * (c + i) : 2u * c + 1u); };
-        float top = -__builtin_huge_valf();
-        for (uint32_t i = 0; i < parts; ++i) top = fmaxf(top, reinterpret_cast<const float *>(part(i))[r]);
-        const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-        float sum = 0.0f, o[8] = {};
-#pragma unroll 2
-        for (uint32_t i = 0; i < parts; ++i) {
-            const float *f = reinterpret_cast<const float *>(part(i));
-            const float w = f[ROWS + r] * exp2_approx(f[r] - ref);
-            const uint4 v = *reinterpret_cast<const uint4 *>(part(i) + 8 * ROWS + (r * D + 8 * d8) * 2);
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-            sum += w;
-            if (w != 0.0f) {
+        // eight parts at a time, all their reads under way together, in the parts' order
+        constexpr int kBatch = 8;
+        float top = -__builtin_huge_valf(), sum = 0.0f, o[8] = {};
+        for (uint32_t i0 = 0; i0 < parts; i0 += kBatch) {
+            float m[kBatch], l[kBatch];
+            uint4 v[kBatch];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&u[k]));
-                    o[2 * k] += w * y.x;
-                    o[2 * k + 1] += w * y.y;
+            for (int k = 0; k < kBatch; ++k) {
+                const bool on = i0 + k < parts;
+                const uint8_t *at = part(on ? i0 + k : i0);
+                m[k] = on ? reinterpret_cast<const float *>(at)[r] : -__builtin_huge_valf();
+                l[k] = on ? reinterpret_cast<const float *>(at)[ROWS + r] : 0.0f;
+                v[k] = *reinterpret_cast<const uint4 *>(at + 8 * ROWS + (r * D + 8 * d8) * 2);
+            }
+            float next = top;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) next = fmaxf(next, m[k]);
+            const float ref = next == -__builtin_huge_valf() ? 0.0f : next, f = exp2_approx(top - ref);
+            top = next;
+            sum *= f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = f == 0.0f ? 0.0f : o[k] * f;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const float w = l[k] * exp2_approx(m[k] - ref);
+                const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                sum += w;
+                if (w != 0.0f) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&u[e]));
+                        o[2 * e] += w * y.x;
+                        o[2 * e + 1] += w * y.y;
+                    }
                 }
             }
         }
