@@ -151,10 +151,14 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     // requests (one, or drafts that fit a row tile with more than 8 rows on average)
     // take one kernel: the tile kernel's time hardly depends on the rows in a tile,
     // and eight drafts of 1 to 4 tokens over 16385 keys took 145 us in both.
+    // Few requests do better in row tiles of 8 (24 query and 4 KV heads of 256, us): 12 rows
+    // of 1 request of 32768 keys 34, in tiles of 16 39; 8 of 16385 94 and 103; 32 of
+    // 1024 40 and 33.  24 rows of 1 request of 32768 keys 42, in the tile kernel 55; 2 of
+    // 8192 35 and 42; 4 of 2048 31 and 27.
     const uint64_t most = static_cast<uint64_t>(b->max_new) * a.group;
     cudaError_t e;
-    if (most <= 16u) {
-        e = launch(most <= 8u ? 1 : 2, 1, 0xffffffffu);
+    if (most <= 16u || (most <= 24u && b->n_seq <= 3u)) {
+        e = launch(most <= 8u || b->n_seq <= 8u ? 1 : 2, 1, 0xffffffffu);
     } else if (b->n_seq == 1 || (most <= 128u && static_cast<uint64_t>(b->n_rows) * a.group > 8ull * b->n_seq)) {
         e = launch(most > 128u ? -1 : 0, 1, 0xffffffffu);
     } else {

@@ -44,9 +44,10 @@
 // each: 850 of conversion, the rest barriers, fences and the load's issue), with the
 // softmax warps (3100) behind it.  Giving every dequantizing warp a box of K and
 // one of V, half the dims each, was slower (1.67 ms).  Drafts (8 requests of 4
-// tokens, 80,000 keys): 87 us against 14 for their bytes (90 while the warps without
-// rows worked and polled along).  The time hardly depends on the rows (8 tokens
-// 83 us): a 64-key tile costs 4000 cycles, 2100 of them a box's conversion.
+// tokens, 80,000 keys): 85 us against 14 for their bytes (90 while the warps without
+// rows worked and polled along, 87 with a join of one part after the other).  The
+// time hardly depends on the rows: a 64-key tile costs 4000 cycles, 2100 of them a
+// box's conversion.
 //
 // Operand tiles: rows of keys by 128-byte chunks of 64 dims with the 128-byte
 // swizzle; K is read K-major, V from the same layout MN-major.  Which dim a

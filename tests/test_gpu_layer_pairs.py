@@ -218,3 +218,16 @@ def test_lengths_up_to_the_last_key_number(kvm_lib, D, new):
     _, spread, _ = ref.attend(q.float().cpu().numpy(), w.raw[0], w.raw[1], w.kinds, 1, T, w.slots, near, [0, new], [2 * T],
                               D ** -0.5, False, np.zeros(q.shape))
     assert (np.abs(got - same) <= spread * 2.0 ** -8 + np.abs(same) * 2.0 ** -10 + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("kinds", [("q4_0", "q4_0"), ("q8_0", "q4_0"), ("q5_0", "q5_0"), ("f16", "f16")])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("B, group, new", [(12, 6, 2), (3, 6, 4), (2, 3, 8)])
+def test_drafts_of_few_and_many_requests(kvm_lib, kinds, D, B, group, new):
+    """9 to 24 rows a KV head, in row tiles of 16 (many requests) and of 8 (few)."""
+    import torch
+    rng = np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(new, 700, B)]
+    w = Window(kvm_lib, torch, 40 + B, kinds, 2, D, 32, lens)
+    start = [new * i for i in range(B + 1)]
+    w.check(queries(torch, w.rng, new * B, 2 * group, D, "bf16"), start, True, max_new=new)
