@@ -640,7 +640,7 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * h / (n_head / n_head_kv).  q and out: F16 or BF16, head_dim 64, 128 or 256.
  * Scores, maxima and sums are F32; the weights enter the second product in F16.
  * In requests of more than 16 rows a KV head, K and V values may enter the products
- * rounded to F16 (2^-11): quantized values beyond 65504 become infinite there.
+ * rounded to F16 (2^-11): quantized K values beyond 65504 become infinite there.
  * out must not overlap q, the cache or the workspace.  Waits inside the kernels
  * are bounded (2 s); one that runs out leaves NaN, never a hang.
  * max_new: the most rows of a request, as far as the caller knows (it picks the

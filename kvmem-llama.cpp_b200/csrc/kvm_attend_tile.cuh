@@ -8,7 +8,10 @@
 //     O += P V               (tcgen05, P from TMEM, V from shared memory)
 // K and V enter as F16 values code * d, rounded once: unlike the few-row kernel
 // this one is not bound by the window's bytes, and dequantizing once for all
-// rows leaves the tensor cores plain F16 operands.  Q is scaled a row by a power
+// rows leaves the tensor cores plain F16 operands.  V blocks that
+// may leave F16's range (scales from 65536 / the largest code on, kTileWide), infinities
+// and NaN stay out of the products, where a weight of 0 would make NaN of them; the
+// epilogue adds them by the definition, in F32, with their own weights.  Q is scaled a row by a power
 // of two (exact for 16-bit inputs but for elements 2^24 below the row's
 // largest), P is F16, all sums and statistics are F32.  The running maximum is
 // raised only when it would grow by more than 2^8, so O in TMEM is rescaled
@@ -352,8 +355,14 @@ __host__ __device__ constexpr int tile_order(int i) {
     return Slice<T, 64>::kNibble ? (i & 4) | (i & 1) << 1 | (i & 2) >> 1 : i;
 }
 
+// Magnitude bits of the first F16 scale whose block may hold values outside F16, 65536 over
+// the largest code (8, 16 or 128), infinite and NaN scales among them; F16 rows: of the
+// first value that is not finite.
+template <int T>
+constexpr uint32_t kTileWide = T == KVM_TYPE_F16 ? 0x7c00u : 0x7c00u - (static_cast<uint32_t>(Slice<T, 64>::kOffsetLog) << 10);
+
 // Drops from a warp's 16 raw rows what must not reach a product: hidden keys (not
-// in `ok`) become zeros, and with IS_V blocks or values that are not finite.
+// in `ok`) become zeros, and with IS_V the blocks or values that are wide (kTileWide).
 template <int T, int D, bool IS_V>
 __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
     using S = Slice<T, D>;
@@ -366,7 +375,7 @@ __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
         constexpr int kStep = T == KVM_TYPE_F16 ? 2 : S::kBlock;      // halves to look at: every value, or the scales
         for (int x = lane; x < 16 * (S::kBytes / kStep); x += 32) {
             uint16_t *p = reinterpret_cast<uint16_t *>(raw + (x & 15) * S::kStride + (x >> 4) * kStep);
-            if ((*p & 0x7c00u) == 0x7c00u) *p = 0;
+            if ((*p & 0x7fffu) >= kTileWide<T>) *p = 0;
         }
         __syncwarp();
     }
@@ -376,7 +385,7 @@ __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
 // Writes 16 keys' slices as F16 values into the operand tile; `raw` is the warp's
 // 16 rows, `key0` its first row of the tile's ROWS.  An eighth of a warp takes eight
 // keys' same 16-byte chunk, so reads and swizzled stores are free of bank
-// conflicts.  Returns whether a scale (F16: a value) of this lane is not finite.
+// conflicts.  Returns whether a scale (F16: a value) of this lane is wide.
 template <int T, int D, int ROWS>
 __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
     uint32_t top = 0;              // largest magnitude bits of the scales
@@ -483,7 +492,20 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
             }
         }
     }
-    return top >= 0x7c00u;
+    return top >= kTileWide<T>;
+}
+
+// q . k of one row and one key by the definition, in F32, from the tensors in device
+// memory: for the keys whose values the tiles leave out.
+template <int T, int D>
+__device__ __noinline__ float tile_score(const uint8_t *q, uint64_t nb_dim, int32_t bf16, const uint8_t *k) {
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int e = 0; e < D; ++e) {
+        const uint32_t u = *reinterpret_cast<const uint16_t *>(q + e * nb_dim);
+        sum = fmaf(bf16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(u))), row_value<T>(k, e), sum);
+    }
+    return sum;
 }
 
 // ------------------------------------------------------------------ kernel --
@@ -821,7 +843,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 float y[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[(i & ~7) | tile_order<VT>(i & 7)] = any ? __uint_as_float(o[i]) * inv : 0.0f;
-                if (odd && in) {                       // values the tiles left out: infinities and NaN that this row sees
+                if (odd && in) {                       // values the tiles left out, of keys that this row sees
                     const int32_t hi = min(lim, p.in1 * kKeys);
                     for (int32_t key = p.in0 * kKeys; key < hi; ++key) {
                         const uint32_t blk = attend_block(a, static_cast<uint32_t>(key));
@@ -829,11 +851,19 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                         if (slot < 0 || static_cast<uint32_t>(slot) >= a.n_slots) continue;
                         const uint64_t cell = static_cast<uint64_t>(slot) * a.block_tokens + (key - blk * a.block_tokens);
                         const uint8_t *v = a.v + cell * a.row_v + static_cast<uint64_t>(p.head) * (G::kSlices * G::V::kBytes);
-                        if (VT != KVM_TYPE_F16 && (*reinterpret_cast<const uint16_t *>(v + c * G::V::kBlock) & 0x7c00u) != 0x7c00u) continue;
+                        bool wide = false;
+                        for (int i = 0; i < (VT == KVM_TYPE_F16 ? 32 : 1); ++i)
+                            wide = wide || (*reinterpret_cast<const uint16_t *>(v + c * G::V::kBlock + 2 * i) & 0x7fffu) >= kTileWide<VT>;
+                        if (!wide) continue;
+                        // the weight as the products' S gives it but for K's rounding; one that
+                        // underflows leaves the value out
+                        const float score = tile_score<KT, D>(qp, a.q.nb_dim, a.q.bf16, a.k + cell * a.row_k + static_cast<uint64_t>(p.head) * G::K::kBytes);
+                        const float weight = exp2_approx(score * a.scale_log2 + (kWeightLog - m)) * inv;
+                        if (weight == 0.0f) continue;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const float x = row_value<VT>(v, 32 * c + i);
-                            if (!isfinite(x)) y[i] += x;
+                            if (VT != KVM_TYPE_F16 || !isfinite(x)) y[i] += weight * x;
                         }
                     }
                 }
@@ -992,7 +1022,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 if (is_v) {
                     const int at = w4 * 16 * G::kBoxesV + (G::kBoxesV == 2 ? 16 * (i & 1) : 0);
                     if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane))) {
-                        // the epilogue adds what is not finite; the products do without it
+                        // the epilogue adds these values with their weights; the products do without them
                         tile_clean<VT, kVD, true>(raw, ok & 0xffffu, lane);
                         tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane);
                         if constexpr (PAIR) {

@@ -1,0 +1,85 @@
+"""Attention over values of every size, against the definition in 64 bits with a
+tolerance from each row's own |q|.|k|: blocks whose values leave F16's range, in
+keys that some rows see and others do not, in every kernel."""
+import numpy as np
+import pytest
+
+import layer_ref as ref
+from test_gpu_layer import Window, queries
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(w, q, start, lens, scale, causal=True, rows=None):
+    """(want, spread, peak, ds) of the rows of q: the definition, sum p |v| / sum p, the
+    largest |v| a row sees, and the most that an F16 rounding of K (2^-11) and an F32 sum
+    of D products move one of the row's scores."""
+    n, hq, D = q.shape
+    G = hq // w.hkv
+    k, v = (ref.row_values(r, t) for r, t in zip(w.raw, w.kinds))
+    want, spread, peak = (np.zeros((n, hq, D)) for _ in range(3))
+    ds = np.zeros((n, hq, 1))
+    for s in range(len(lens)):
+        lo, hi, kv = int(start[s]), int(start[s + 1]), int(lens[s])
+        j = np.arange(kv)
+        cell = w.table[s, j // w.T].astype(np.int64) * w.T + j % w.T
+        for r in range(lo, hi):
+            if rows is not None and r not in rows:
+                continue
+            c = cell[:kv - (hi - lo) + (r - lo) + 1] if causal else cell
+            if c.size == 0:
+                continue
+            for h in range(hq):
+                at = slice(h // G * D, h // G * D + D)
+                x = k[c, at] @ q[r, h] * scale
+                p = np.exp(x - x.max())
+                p /= p.sum()
+                want[r, h], spread[r, h] = p @ v[c, at], p @ np.abs(v[c, at])
+                peak[r, h] = np.abs(v[c, at]).max(0)
+                # the same bound for keys that weigh nothing would hide the others' errors
+                near = p > 1e-9
+                ds[r, h] = abs(scale) * (np.abs(k[c, at][near]) @ np.abs(q[r, h])).max() * (2.0 ** -11 + D * 2.0 ** -23)
+    return want, spread, peak, ds
+
+
+def agree(got, want, spread, peak, ds, keys):
+    """Two roundings of a weight to F16 and one of a V value (2^-11 each), a score moved by
+    ds in numerator and denominator, one rounding more for an item that several CTAs share,
+    weights below 2^-31 of the largest lost, the output's half step."""
+    half = 2.0 ** -8 if str(got.dtype).endswith("bfloat16") else 2.0 ** -11
+    tol = spread * (4 * 2.0 ** -11 + 2 * ds) + keys * 2.0 ** -31 * 2.0 ** -11 * peak + np.abs(want) * half
+    if half == 2.0 ** -11:
+        tol = tol + 2.0 ** -25          # half a step of F16's subnormals
+    error = np.abs(got.float().cpu().numpy().astype(np.float64) - want)
+    assert (error <= tol).all(), np.nanmax(np.where(error <= tol, 0, error / np.maximum(tol, 1e-300)))
+
+
+def rewrite(w, side, change):
+    """The window's rows of one side after `change`(values [cells, width])."""
+    w.put(side, ref.quantize(change(ref.row_values(w.raw[side], w.kinds[side])).astype(np.float32), w.kinds[side]))
+
+
+# ---------------------------------------------- values beyond F16, not seen by all --
+
+SHAPES = [(64, 2, 40), (128, 4, 20), (128, 4, 70), (256, 6, 12), (256, 6, 50)]      # head size, group, rows: single CTAs and pairs
+
+
+@pytest.mark.parametrize("kinds", [("q8_0", "q8_0"), ("q4_0", "q4_0"), ("f16", "q8_0"), ("q8_0", "q5_0"), ("q5_0", "q4_0")])
+@pytest.mark.parametrize("D, group, new", SHAPES)
+def test_a_value_beyond_f16_stays_with_the_rows_that_see_it(kvm_lib, kinds, D, group, new):
+    """The last key's V is 1e5, finite in its block's scale and codes: rows that do not see it
+    are as without it, the last one is the definition's."""
+    import torch
+    keys = 210
+    w = Window(kvm_lib, torch, D + new, kinds, 1, D, 32, [keys])
+    q = queries(torch, w.rng, new, group, D, "bf16")
+    clean = w.run(q, [0, new], True, max_new=new)
+
+    def change(v):
+        v[w.cell(0, keys - 1)] = 1e5 * np.where(np.arange(D) % 3, 1.0, -0.7)
+        return v
+    rewrite(w, 1, change)
+    got = w.run(q, [0, new], True, max_new=new)
+    assert torch.isfinite(got).all()
+    assert torch.allclose(got[:new - 1].float(), clean[:new - 1].float(), rtol=2.0 ** -8, atol=2.0 ** -9)
+    agree(got, *reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5), keys)
