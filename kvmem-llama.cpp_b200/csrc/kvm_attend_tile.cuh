@@ -60,8 +60,9 @@
 //
 // The (item, key tile) pairs of the call form one line, shared evenly by the
 // CTAs or pairs; an item that several share leaves its pieces' maxima, sums and
-// normalised F16 outputs (one rounding as large as the output's own) for
-// attend_tile_join_kernel.
+// normalised outputs for attend_tile_join_kernel: F16 values of 32 dims with a power of
+// two that brings their largest to [2^14, 2^15) (one rounding as large as the output's
+// own, whatever their size; F32 would take twice the workspace).
 #pragma once
 
 #include "kvm_attend_split.cuh"
@@ -330,9 +331,18 @@ struct WarpWalk {
     uint32_t more;
 };
 
-// A piece's results in the workspace: maxima, sums, then rows of D halves.
+// A piece's results in the workspace: maxima, sums, what 32 dims of a row were divided by,
+// then rows of D halves.
 template <int D, int ROWS>
-__host__ __device__ constexpr uint32_t tile_part_bytes() { return ROWS * (8u + 2u * D); }
+__host__ __device__ constexpr uint32_t tile_part_bytes() { return ROWS * (8u + D / 8u + 2u * D); }
+template <int D, int ROWS>
+__device__ __forceinline__ float *tile_part_unit(uint8_t *part, uint32_t row, uint32_t dim) {
+    return reinterpret_cast<float *>(part + 8 * ROWS) + row * (D / 32) + dim / 32;
+}
+template <int D, int ROWS>
+__device__ __forceinline__ uint4 *tile_part_values(uint8_t *part, uint32_t row, uint32_t dim) {
+    return reinterpret_cast<uint4 *>(part + (8 + D / 8) * ROWS + (row * D + dim) * 2);
+}
 template <int D, int ROWS>
 __device__ __forceinline__ uint8_t *tile_part(const AttendArgs &a, uint32_t slot) {
     return a.work + kAttendMaxCtas * kAttendDescBytes + static_cast<uint64_t>(slot) * tile_part_bytes<D, ROWS>();
@@ -868,11 +878,26 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     }
                 }
                 if (part && in) {
-                    uint4 *to = reinterpret_cast<uint4 *>(part + 8 * kRows + (item_row * D + 32 * c) * 2);
+                    float top = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        to[k] = make_uint4(pack_half2(y[8 * k], y[8 * k + 1]), pack_half2(y[8 * k + 2], y[8 * k + 3]),
-                                           pack_half2(y[8 * k + 4], y[8 * k + 5]), pack_half2(y[8 * k + 6], y[8 * k + 7]));
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(y[i]));
+                    if (!isfinite(top)) {              // the largest of the others
+                        top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top = fmaxf(top, isfinite(y[i]) ? fabsf(y[i]) : 0.0f);
+                    }
+                    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                    const int up = min(126, 14 - e);
+                    const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+                    *tile_part_unit<D, kRows>(part, item_row, 32 * c) = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+                    uint4 *to = tile_part_values<D, kRows>(part, item_row, 32 * c);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t u[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) u[i] = pack_half2(y[8 * k + 2 * i] * mul, y[8 * k + 2 * i + 1] * mul);
+                        to[k] = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
                 } else if (!part && in) {
                     if (a.out_vec) {
                         uint4 *to = reinterpret_cast<uint4 *>(op + 64 * c);
@@ -1146,15 +1171,16 @@ __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __
         constexpr int kBatch = 8;
         float top = -__builtin_huge_valf(), sum = 0.0f, o[8] = {};
         for (uint32_t i0 = 0; i0 < parts; i0 += kBatch) {
-            float m[kBatch], l[kBatch];
+            float m[kBatch], l[kBatch], unit[kBatch];
             uint4 v[kBatch];
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const bool on = i0 + k < parts;
-                const uint8_t *at = part(on ? i0 + k : i0);
+                uint8_t *at = part(on ? i0 + k : i0);
                 m[k] = on ? reinterpret_cast<const float *>(at)[r] : -__builtin_huge_valf();
                 l[k] = on ? reinterpret_cast<const float *>(at)[ROWS + r] : 0.0f;
-                v[k] = *reinterpret_cast<const uint4 *>(at + 8 * ROWS + (r * D + 8 * d8) * 2);
+                unit[k] = *tile_part_unit<D, ROWS>(at, r, 8 * d8);
+                v[k] = *tile_part_values<D, ROWS>(at, r, 8 * d8);
             }
             float next = top;
 #pragma unroll
@@ -1173,8 +1199,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_tile_join_kernel(const __
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&u[e]));
-                        o[2 * e] += w * y.x;
-                        o[2 * e + 1] += w * y.y;
+                        o[2 * e] += w * unit[k] * y.x;
+                        o[2 * e + 1] += w * unit[k] * y.y;
                     }
                 }
             }

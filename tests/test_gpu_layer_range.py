@@ -83,3 +83,23 @@ def test_a_value_beyond_f16_stays_with_the_rows_that_see_it(kvm_lib, kinds, D, g
     assert torch.isfinite(got).all()
     assert torch.allclose(got[:new - 1].float(), clean[:new - 1].float(), rtol=2.0 ** -8, atol=2.0 ** -9)
     agree(got, *reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5), keys)
+
+
+# ------------------------------------------- items that several CTAs share --
+
+@pytest.mark.parametrize("kinds", [("q8_0", "q8_0"), ("q4_0", "q4_0")])
+@pytest.mark.parametrize("D, group, new", [(64, 1, 20), (128, 2, 70), (256, 6, 25)])
+@pytest.mark.parametrize("size", [1e-5, 2e5])
+def test_outputs_of_every_size_from_shared_items(kvm_lib, kinds, D, group, new, size):
+    """One request over a window that many CTAs share: means far below and far above F16's
+    range keep their bits on the way through the workspace."""
+    import torch
+    keys = 1500
+    w = Window(kvm_lib, torch, D + new, kinds, 1, D, 32, [keys])
+    # every dim has a mean of its own size beside the noise, the last 32 dims a thirtieth
+    rewrite(w, 1, lambda v: (v * 0.1 + 1.0) * size * np.where(np.arange(D) >= D - 32, 0.03, 1.0))
+    q = queries(torch, w.rng, new, group, D, "bf16")
+    got = w.run(q, [0, new], True, max_new=new)
+    seen = list(range(0, new, 7))
+    want = reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5, rows=seen)
+    agree(got[seen], *(x[seen] for x in want), keys)
