@@ -639,12 +639,14 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * to no request stay as they were.  Query head h reads KV head
  * h / (n_head / n_head_kv).  q and out: F16 or BF16, head_dim 64, 128 or 256.
  * Scores, maxima and sums are F32; the weights enter the second product in F16.
- * In requests of more than 16 rows a KV head, K and V values may enter the products
- * rounded to F16 (2^-11): quantized K values beyond 65504 become infinite there.
+ * Which kernel takes a request depends on max_new and on the batch: unless max_new times
+ * the query heads of a KV head is at most 16, K and V values may enter the products
+ * rounded to F16: by 2^-11 of a value, of any size that the rows' formats hold, and where 16
+ * neighbouring keys hold values beyond 65504 also by 2^-33 of the largest of these.
  * out must not overlap q, the cache or the workspace.  Waits inside the kernels
  * are bounded (2 s); one that runs out leaves NaN, never a hang.
- * max_new: the most rows of a request, as far as the caller knows (it picks the
- * kernel; a wrong value costs time, not correctness).
+ * max_new: the most rows of a request, as far as the caller knows.  It picks the
+ * kernel: a wrong value costs time and may change the roundings, never more.
  * d_work: KVM_ATTEND_WORK_BYTES of device memory, 16-byte aligned, that no
  * other call running at the same time uses; its contents need no preparation
  * and mean nothing afterwards.

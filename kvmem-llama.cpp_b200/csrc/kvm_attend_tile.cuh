@@ -8,13 +8,14 @@
 //     O += P V               (tcgen05, P from TMEM, V from shared memory)
 // K and V enter as F16 values code * d, rounded once: unlike the few-row kernel
 // this one is not bound by the window's bytes, and dequantizing once for all
-// rows leaves the tensor cores plain F16 operands.  V blocks that
-// may leave F16's range (scales from 65536 / the largest code on, kTileWide), infinities
-// and NaN stay out of the products, where a weight of 0 would make NaN of them; the
-// epilogue adds them by the definition, in F32, with their own weights.  Q is scaled a row by a power
-// of two (exact for 16-bit inputs but for elements 2^24 below the row's
-// largest), P is F16, all sums and statistics are F32.  The running maximum is
-// raised only when it would grow by more than 2^8, so O in TMEM is rescaled
+// rows leaves the tensor cores plain F16 operands.  V blocks that may leave F16's range
+// (scales from 65536 / the largest code on, kTileWide), infinities and NaN stay out of
+// the products, where a weight of 0 would make NaN of them; the epilogue adds them by
+// the definition, in F32, with their own weights.  K boxes with such scales enter divided
+// by the largest code, a power of two, and their columns of S are multiplied by it again.
+// Q is scaled a row by a power of two (exact for 16-bit inputs but for elements 2^24
+// below the row's largest), P is F16, all sums and statistics are F32.  The running
+// maximum is raised only when it would grow by more than 2^8, so O in TMEM is rescaled
 // rarely; P carries a factor 2^7 that cancels in the quotient, which keeps it
 // below F16's top and its bits down to 2^-31 of the row's largest weight.
 //
@@ -143,6 +144,12 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
 __device__ __forceinline__ void st_shared_at(uint32_t *p, uint32_t v, uint32_t rank) {
     asm volatile(
         "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tst.shared::cluster.u32 [ra], %1;\n\t}"
+        ::"r"(smem_u32(p)), "r"(v), "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ void st_shared_at(uint8_t *p, uint32_t v, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tst.shared::cluster.u8 [ra], %1;\n\t}"
         ::"r"(smem_u32(p)), "r"(v), "r"(rank)
         : "memory");
 }
@@ -396,7 +403,9 @@ __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
 // 16 rows, `key0` its first row of the tile's ROWS.  An eighth of a warp takes eight
 // keys' same 16-byte chunk, so reads and swizzled stores are free of bank
 // conflicts.  Returns whether a scale (F16: a value) of this lane is wide.
-template <int T, int D, int ROWS>
+// LOW: the values divided by 2^kOffsetLog, which keeps those of every finite scale in F16
+// (exact but for values below 2^(kOffsetLog - 14)).
+template <int T, int D, int ROWS, bool LOW = false>
 __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
     uint32_t top = 0;              // largest magnitude bits of the scales
     using S = Slice<T, D>;
@@ -409,6 +418,10 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
         const uint32_t d = lds16(p);
         top = max(top, d & 0x7fffu);
         return __byte_perm(d, 0u, 0x1010);
+    };
+    auto value = [&](uint32_t code, uint32_t d) -> uint32_t {
+        if constexpr (LOW) code = mul_half2(code, 0x10001u * (static_cast<uint32_t>(15 - S::kOffsetLog) << 10));
+        return mul_half2(code, d);
     };
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -441,8 +454,8 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t u = x[i] ^ 0x80808080u;       // 1024 + code + 128, less 1152
-                    o[2 * i] = mul_half2(h2_sub(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u), d);
-                    o[2 * i + 1] = mul_half2(h2_sub(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u), d);
+                    o[2 * i] = value(h2_sub(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u), d);
+                    o[2 * i + 1] = value(h2_sub(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u), d);
                 }
                 put(key, 4 * b + quad, make_uint4(o[0], o[1], o[2], o[3]));
             }
@@ -485,16 +498,16 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
                         h0 |= ((c & 5u) * 0x00400100u) & 0x01000100u;
                         h1 |= ((c & 10u) * 0x00200080u) & 0x01000100u;
                         // 1024 + n less 1040; (1024 + 16 n) / 16 less 80
-                        lo[2 * i] = mul_half2(h2_sub(l0, 0x64106410u), d);
-                        lo[2 * i + 1] = mul_half2(h2_sub(l1, 0x64106410u), d);
-                        hi[2 * i] = mul_half2(h2_fma(h0, 0x2c002c00u, 0xd500d500u), d);
-                        hi[2 * i + 1] = mul_half2(h2_fma(h1, 0x2c002c00u, 0xd500d500u), d);
+                        lo[2 * i] = value(h2_sub(l0, 0x64106410u), d);
+                        lo[2 * i + 1] = value(h2_sub(l1, 0x64106410u), d);
+                        hi[2 * i] = value(h2_fma(h0, 0x2c002c00u, 0xd500d500u), d);
+                        hi[2 * i + 1] = value(h2_fma(h1, 0x2c002c00u, 0xd500d500u), d);
                     } else {
                         // 1024 + n less 1032; (1024 + 16 n) / 16 less 72
-                        lo[2 * i] = mul_half2(h2_sub(l0, 0x64086408u), d);
-                        lo[2 * i + 1] = mul_half2(h2_sub(l1, 0x64086408u), d);
-                        hi[2 * i] = mul_half2(h2_fma(h0, 0x2c002c00u, 0xd480d480u), d);
-                        hi[2 * i + 1] = mul_half2(h2_fma(h1, 0x2c002c00u, 0xd480d480u), d);
+                        lo[2 * i] = value(h2_sub(l0, 0x64086408u), d);
+                        lo[2 * i + 1] = value(h2_sub(l1, 0x64086408u), d);
+                        hi[2 * i] = value(h2_fma(h0, 0x2c002c00u, 0xd480d480u), d);
+                        hi[2 * i + 1] = value(h2_fma(h1, 0x2c002c00u, 0xd480d480u), d);
                     }
                 }
                 put(key, 8 * pr + 4 * b + h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
@@ -503,6 +516,11 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
         }
     }
     return top >= kTileWide<T>;
+}
+
+template <int T, int D, int ROWS>
+__device__ __noinline__ void tile_dequant_low(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
+    tile_dequant<T, D, ROWS, true>(raw, tile, key0, lane);
 }
 
 // q . k of one row and one key by the definition, in F32, from the tensors in device
@@ -536,6 +554,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
     __shared__ uint32_t s_seq, s_tmem, s_odd;
     __shared__ float s_swap[2][2 * kTileRows];
+    __shared__ __align__(8) uint8_t s_low[4][8];       // K boxes of a tile (16 keys each) that are LOW
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -549,6 +568,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         mbar_init(q_full, 8 * kCtas);
         for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
         s_odd = 0;
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint64_t *>(s_low[i]) = 0;
         fence_mbar_init();
     }
     __syncthreads();
@@ -765,7 +785,15 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     const uint2 ok2 = *reinterpret_cast<const uint2 *>(valid + (kKeys / 16) * (j & 3u) + wg * (kHalf / 16) + 2 * c);
                     const uint32_t ok = ok2.x | ok2.y << 16;
                     const int32_t key0 = n * kKeys + wg * kHalf + 32 * c;
-                    if (key0 + 32 > kfull || ok != 0xffffffffu) {
+                    uint32_t low = 0;
+                    if constexpr (KT != KVM_TYPE_F16) low = *reinterpret_cast<const uint16_t *>(&s_low[j & 3u][wg * (kHalf / 16) + 2 * c]);
+                    if (key0 + 32 > kfull || ok != 0xffffffffu || low != 0u) {
+                        constexpr float kUp = static_cast<float>(1 << Slice<KT, 64>::kOffsetLog);
+                        const float up0 = low & 0xffu ? kUp : 1.0f, up1 = low >> 8 ? kUp : 1.0f;
+                        if (KT != KVM_TYPE_F16 && low != 0u) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * (i < 16 ? up0 : up1));
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (key0 + i >= lim || !((ok >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
@@ -943,6 +971,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kBoxK : 0) + w4 * NS * raw_bytes;
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
         uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring slot of the next load, of the next box
+        uint32_t low_tiles = 0;                            // this K warp's marks in s_low, a bit a tile
         // a pair's K warp also looks up the 16 keys that the peer's warp brings (their
         // visibility is wanted here too)
         constexpr int kLooks = kCtas;
@@ -1058,7 +1087,20 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                         }
                     }
                 } else {
-                    tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
+                    const bool wide = tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
+                    if constexpr (KT != KVM_TYPE_F16) {
+                        const uint32_t low = __any_sync(0xffffffffu, wide) ? 1u : 0u;
+                        if (low) tile_dequant_low<KT, D, 64>(raw, tile, w4 * 16, lane);
+                        if (low != ((low_tiles >> (j & 3u)) & 1u)) {       // read beside valid[]: written as early
+                            low_tiles ^= 1u << (j & 3u);
+                            if constexpr (PAIR) {
+                                if (lane < kCtas) st_shared_at(&s_low[j & 3u][mine / 16], low, lane);
+                                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                            } else if (lane == 0) {
+                                *reinterpret_cast<volatile uint8_t *>(&s_low[j & 3u][mine / 16]) = static_cast<uint8_t>(low);
+                            }
+                        }
+                    }
                     if (lane < kLooks) valid[(kKeys / 16) * (j & 3u) + (mine + theirs * lane) / 16] = (ok >> (16 * lane)) & 0xffffu;
                 }
                 fence_proxy_async_smem();

@@ -103,3 +103,28 @@ def test_outputs_of_every_size_from_shared_items(kvm_lib, kinds, D, group, new, 
     seen = list(range(0, new, 7))
     want = reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5, rows=seen)
     agree(got[seen], *(x[seen] for x in want), keys)
+
+
+# ------------------------------------------------------------ keys beyond F16 --
+
+@pytest.mark.parametrize("kinds", [("q8_0", "q8_0"), ("q4_0", "q4_0"), ("q5_0", "f16"), ("q8_0", "q4_0")])
+@pytest.mark.parametrize("D, group, new", SHAPES + [(128, 4, 1), (64, 2, 6)])
+@pytest.mark.parametrize("T", [32, 24])
+def test_keys_beyond_f16(kvm_lib, kinds, D, group, new, T):
+    """Some keys' first block is of 1e5 where the queries are of 1e-5: finite scores, the
+    definition's, whatever kernel takes the request."""
+    import torch
+    keys = 210
+    w = Window(kvm_lib, torch, D + new, kinds, 1, D, T, [keys])
+    big = [w.cell(0, j) for j in (0, 17, 63, 64, 100, 127, 128, 129, 200, keys - 1) if j < keys]
+
+    def change(k):
+        k[big, :32] *= 1e5
+        return k
+    rewrite(w, 0, change)
+    q = queries(torch, w.rng, new, group, D, "bf16")
+    q[..., :32] *= 1e-5
+    results = [w.run(q, [0, new], True, max_new=m) for m in (1, new, 1000)]
+    want = reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5)
+    for got in results:
+        agree(got, *want, keys)
