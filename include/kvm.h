@@ -644,7 +644,8 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * rounded to F16: by 2^-11 of a value, of any size that the rows' formats hold, and where 16
  * neighbouring keys hold values beyond 65504 also by 2^-33 of the largest of these.
  * out must not overlap q, the cache or the workspace.  Waits inside the kernels
- * are bounded (2 s); one that runs out leaves NaN, never a hang.
+ * are bounded (2 s); one that runs out leaves NaN in every row that its CTA still works
+ * on, never a wrong value or a hang, and no copy is under way when the kernel ends.
  * max_new: the most rows of a request, as far as the caller knows.  It picks the
  * kernel: a wrong value costs time and may change the roundings, never more.
  * d_work: KVM_ATTEND_WORK_BYTES of device memory, 16-byte aligned, that no
@@ -652,6 +653,10 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * and mean nothing afterwards.
  */
 #define KVM_ATTEND_CAUSAL 1u
+/* Failure-path tests: the first keys of the first request's first rows and KV head stay
+ * unloaded, in K or in V, where rows come by TMA, so that a wait runs out. */
+#define KVM_ATTEND_TEST_SKIP_K 0x40000000u
+#define KVM_ATTEND_TEST_SKIP_V 0x80000000u
 #define KVM_ATTEND_WORK_BYTES 33554432u
 typedef struct kvm_attend_batch {
     const int32_t *d_table;

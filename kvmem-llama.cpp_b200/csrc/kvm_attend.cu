@@ -79,7 +79,8 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
     if ((r = rows_check(out, q->n_head, D, "kvm_attend out")) != KVM_OK) return r;
     if (q->type == KVM_TYPE_F32 || out->type == KVM_TYPE_F32)
         return layer_fail(KVM_EINVAL, "%s: q and out must be F16 or BF16", me);
-    if (b->flags & ~KVM_ATTEND_CAUSAL) return layer_fail(KVM_EINVAL, "%s: unknown flags", me);
+    constexpr uint32_t kSkips = KVM_ATTEND_TEST_SKIP_K | KVM_ATTEND_TEST_SKIP_V;
+    if (b->flags & ~(KVM_ATTEND_CAUSAL | kSkips)) return layer_fail(KVM_EINVAL, "%s: unknown flags", me);
     if (!std::isfinite(b->scale)) return layer_fail(KVM_EINVAL, "%s: scale must be finite", me);
     if (b->n_seq > 65535u) return layer_fail(KVM_EINVAL, "%s: at most 65535 requests", me);
     if (static_cast<uint64_t>(b->n_rows) * (q->n_head / c->n_head_kv) > 0x7fffffffull || b->table_cols > 0x7fffffffu)
@@ -117,6 +118,7 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
         if (c->block_tokens == 1u << s) a.block_shift = s;
     a.scale_log2 = b->scale * 1.4426950408889634f;
     a.causal = (b->flags & KVM_ATTEND_CAUSAL) ? 1u : 0u;
+    a.skip = b->flags & kSkips;
     a.q = rows_of(q);
     a.out = rows_of(out);
     a.work = static_cast<uint8_t *>(d_work);

@@ -44,6 +44,7 @@ struct AttendArgs {
     uint32_t heads_cta;        // KV heads that a CTA takes together: 1, 2 or 4
     uint32_t whole;            // split kernel: no segment is shared (all are short), so nothing is joined
     uint32_t max_keys;         // keys that the table's columns can hold, at most 2^31 - 1
+    uint32_t skip;             // the KVM_ATTEND_TEST_SKIP flags
     uint32_t min_rows, max_rows;   // query rows (tokens * group) a sequence needs to be taken by this launch
     CUtensorMap map_k, map_v;      // [cells][row bytes / 4] of 32-bit words
 };

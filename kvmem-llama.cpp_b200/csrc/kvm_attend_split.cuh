@@ -336,7 +336,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         // ---- the warp's steps: in0 + sub, + nsub, ...
         const uint32_t kstart = in0 * kStep;
         const uint32_t in1 = min(in_end, (static_cast<uint32_t>(kend) + kStep - 1u) / kStep);
-        const int n_steps = in1 > in0 + sub ? static_cast<int>((in1 - in0 - sub + nsub - 1) / nsub) : 0;
+        const int n_steps = !lost && in1 > in0 + sub ? static_cast<int>((in1 - in0 - sub + nsub - 1) / nsub) : 0;
         const int32_t *trow = a.table + seq * a.table_stride;
         const uint8_t *kbase = a.k + static_cast<uint64_t>(head) * SK::kBytes;
         const uint8_t *vbase = a.v + static_cast<uint64_t>(head) * SV::kBytes;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         // load(i, side, stage): K (side 0), then V (side 1) of step i; K's call looks the
         // cells up for both
         int32_t cell = -1;
-        auto load = [&](int i, auto side, uint32_t to) {
+        auto load = [&](int i, auto side, uint32_t to, bool skip = false) {
             constexpr bool kIsV = decltype(side)::value != 0;
             using S = std::conditional_t<kIsV, SV, SK>;
             uint8_t *dst = ring + to * G::kStage + (kIsV ? G::kRowsK : 0);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                         cell = ok ? static_cast<int32_t>(slot * a.block_tokens + in_block) : -1;
                     }
                 }
-                if (lane < MT) {
+                if (lane < MT && !skip) {
                     uint64_t *bar = (kIsV ? v_bar : k_bar) + to;
                     if (cell >= 0) {
                         mbar_arrive_expect_tx(bar, 16 * S::kStride);
@@ -424,11 +424,21 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         };
         constexpr std::integral_constant<int, 0> kSideK{};
         constexpr std::integral_constant<int, 1> kSideV{};
-        auto arrived = [&](uint64_t *bar) {
-            if (a.tma) {
-                if (!lost && !mbar_wait_near(bar, phase)) lost = true;
-            } else {
-                cp_async_wait<2 * NS - 1>();
+        auto arrived = [&](uint64_t *bar) -> bool {
+            bool ok = true;
+            if (a.tma) ok = __all_sync(0xffffffffu, mbar_wait_near(bar, phase));
+            else cp_async_wait<2 * NS - 1>();
+            __syncwarp();
+            return ok;
+        };
+        // A wait of step i ran out, behind its K rows when k_read: no more loads, no result
+        // but NaN, and what is under way lands before the merge takes the ring's memory.
+        auto give_up = [&](int i, bool k_read) {
+            lost = true;
+            for (int k = 0; k <= NS && i + k < n_steps; ++k) {
+                const uint32_t at = stage_at + k < NS ? stage_at + k : stage_at + k - NS, parity = stage_at + k < NS ? phase : phase ^ 1u;
+                if (k_read ? k > 0 : k < NS) mbar_wait_bounded(&k_bar[at], parity);
+                if (k < NS) mbar_wait_bounded(&v_bar[at], parity);
             }
             __syncwarp();
         };
@@ -443,9 +453,10 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
 #pragma unroll 1
         for (int i = 0; i < NS; ++i) {
             const uint32_t to = stage_at + i < NS ? stage_at + i : stage_at + i - NS;
-            if (i < n_steps) load(i, kSideK, to);
+            const uint32_t skip = (static_cast<uint32_t>(i + warp) | in0 | seq | seg) == 0u ? a.skip : 0u;
+            if (i < n_steps) load(i, kSideK, to, skip & KVM_ATTEND_TEST_SKIP_K);
             cp_async_commit();
-            if (i < n_steps) load(i, kSideV, to);
+            if (i < n_steps) load(i, kSideV, to, skip & KVM_ATTEND_TEST_SKIP_V);
             cp_async_commit();
         }
 
@@ -564,7 +575,10 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
             uint8_t *kr = ring + at * G::kStage + lead_k;
             uint8_t *vr = ring + at * G::kStage + G::kRowsK + lead_v;
             const int32_t key0 = static_cast<int32_t>(kstart) + (sub + i * nsub) * kStep;
-            arrived(&k_bar[at]);
+            if (!arrived(&k_bar[at])) {
+                give_up(i, false);
+                break;
+            }
             const uint32_t ok = valid[at];
             if (a.tma && ok != kAll) hidden(kr, SK{}, ok);
 
@@ -709,7 +723,10 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 }
 
             // ---- V's rows and scales
-            arrived(&v_bar[at]);
+            if (!arrived(&v_bar[at])) {
+                give_up(i, true);
+                break;
+            }
             if (a.tma && ok != kAll) hidden(vr, SV{}, ok);
             bool odd_values = false;          // an infinite or NaN V value
             if constexpr (kCodesV) {
@@ -846,7 +863,10 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         }
 
         // ---- the warps' results together
-        if (lost) l[0][0] = __int_as_float(0x7fc00000);       // no result rather than a wrong one
+        if (lost) {                           // no result rather than a wrong one
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fc00000);
+        }
         cp_async_wait<0>();
         __syncthreads();
         float *sm_m = reinterpret_cast<float *>(smem), *sm_l = sm_m + W * R, *sm_o = sm_l + W * R;

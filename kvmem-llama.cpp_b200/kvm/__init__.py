@@ -48,7 +48,8 @@ ABI_SYMBOLS = (
     "kvm_write_rows", "kvm_read_rows", "kvm_attend",
 )
 
-ATTEND_CAUSAL = 1                 # kvm_attend_batch flag
+ATTEND_CAUSAL = 1                 # kvm_attend_batch flags
+ATTEND_TEST_SKIP_K, ATTEND_TEST_SKIP_V = 1 << 30, 1 << 31
 ATTEND_WORK_BYTES = 32 << 20      # KVM_ATTEND_WORK_BYTES
 
 
