@@ -523,6 +523,49 @@ __device__ __noinline__ void tile_dequant_low(const uint8_t *raw, uint8_t *tile,
     tile_dequant<T, D, ROWS, true>(raw, tile, key0, lane);
 }
 
+// A wait ran out: results of this CTA and its peer are void from here on.
+template <bool PAIR>
+__device__ __noinline__ void tile_say_lost(uint32_t *lost) {
+    *reinterpret_cast<volatile uint32_t *>(lost) = 1u;
+    if constexpr (PAIR) {
+        st_shared_at(lost, 1u, (blockIdx.x & 1u) ^ 1u);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    } else {
+        __threadfence_block();
+    }
+}
+
+// A warp's raw rows did not come: its n loads under way, the ring's slots from `at` on, land
+// before it goes on.
+template <bool PAIR>
+__device__ __noinline__ void tile_abandon(uint32_t *lost, uint64_t *full, uint32_t at, uint32_t phase, uint32_t slots, int32_t n) {
+    tile_say_lost<PAIR>(lost);
+    for (uint32_t k = 0; k < slots && static_cast<int32_t>(k) < n; ++k) {
+        mbar_wait_bounded(&full[at], phase);
+        if (++at == slots) {
+            at = 0;
+            phase ^= 1u;
+        }
+    }
+    __syncwarp();
+}
+
+// The kernel's end behind a wait that ran out: products may be under way; TMEM is freed
+// behind them.
+template <bool PAIR>
+__device__ __noinline__ void tile_finish(uint64_t *mma_done) {
+    if (threadIdx.x / 32 == 16) {
+        if ((threadIdx.x & 31u) == 0u && (!PAIR || (blockIdx.x & 1u) == 0u)) {
+            if constexpr (PAIR) tc_commit_pair(mma_done);      // arrives in both CTAs
+            else tc_commit(mma_done);
+        }
+        mbar_wait_bounded(mma_done, 0);
+        __syncwarp();
+    }
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
+}
+
 // q . k of one row and one key by the definition, in F32, from the tensors in device
 // memory: for the keys whose values the tiles leave out.
 template <int T, int D>
@@ -548,11 +591,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBars);
     uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
-             *q_full = bars + 12, *raw_full = bars + 13;          // raw_full [8 warps][NS]
+             *q_full = bars + 12, *raw_full = bars + 13, *mma_done = bars + 13 + 8 * NS;      // raw_full [8 warps][NS]
     uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][kKeys / 16], a bit a key
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = blockIdx.x / kCtas, n_units = gridDim.x / kCtas;
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
-    __shared__ uint32_t s_seq, s_tmem, s_odd;
+    __shared__ uint32_t s_seq, s_tmem, s_odd, s_lost;  // s_lost: a wait of this CTA or its peer ran out
     __shared__ float s_swap[2][2 * kTileRows];
     __shared__ __align__(8) uint8_t s_low[4][8];       // K boxes of a tile (16 keys each) that are LOW
 
@@ -566,8 +609,12 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             mbar_init(&s_full[i], 1);
         }
         mbar_init(q_full, 8 * kCtas);
-        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], 1);
-        s_odd = 0;
+        // failure-path tests: one arrival more than will come, on the first rows of a K or V warp
+        const int skip_k = unit == 0 && rank == 0 && (a.skip & KVM_ATTEND_TEST_SKIP_K) ? 0 : -1;
+        const int skip_v = unit == 0 && rank == kCtas - 1u && (a.skip & KVM_ATTEND_TEST_SKIP_V) ? 4 * NS : -1;
+        for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], i == skip_k || i == skip_v ? 2 : 1);
+        mbar_init(mma_done, 1);
+        s_odd = s_lost = 0;
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint64_t *>(s_low[i]) = 0;
         fence_mbar_init();
     }
@@ -651,9 +698,14 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         __syncwarp();
         return mywalk.more != 0u;
     };
-    bool lost = false;                         // a bounded wait ran out: go on without waiting
+    // A bounded wait ran out: go on without waiting.  Whoever stores results learns of it
+    // through s_lost, written before the arrival that lets the others pass.
+    bool lost = false;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
-        if (!lost && !mbar_wait_near(bar, phase & 1u)) lost = true;
+        if (!lost && !mbar_wait_near(bar, phase & 1u)) {
+            lost = true;
+            tile_say_lost<PAIR>(&s_lost);
+        }
         // together: a lane that went ahead could let the phase after this one complete
         // while another still polls for this one
         __syncwarp();
@@ -860,7 +912,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 wait(&v_free[(j - 1) & 1u], (j - 1) >> 1);
                 tc_fence_after();
             }
-            if (lost) l = __int_as_float(0x7fc00000);
+            if (lost || *reinterpret_cast<volatile uint32_t *>(&s_lost)) l = __int_as_float(0x7fc00000);       // no result rather than a wrong one
             l += swap(l);
             const bool whole = p.starts && p.ends;
             const bool odd = *reinterpret_cast<volatile uint32_t *>(&s_odd) != 0;
@@ -972,6 +1024,11 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
         uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring slot of the next load, of the next box
         uint32_t low_tiles = 0;                            // this K warp's marks in s_low, a bit a tile
+        bool dead = false;                                 // rows never came: no more loads, the others are let pass
+        auto pass = [&](int32_t tiles) {
+            for (; tiles > 0; --tiles, ++j)
+                if (lane == 0) arrive(&tile_full[j & 1u]);
+        };
         // a pair's K warp also looks up the 16 keys that the peer's warp brings (their
         // visibility is wanted here too)
         constexpr int kLooks = kCtas;
@@ -979,6 +1036,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         const int32_t theirs = is_v ? 0 : rank == 0 ? 64 : -64;
         while (next_piece()) {
             const int32_t n_tiles = max(0, p.in1 - p.in0), n_boxes = n_tiles * boxes;
+            if (dead) {
+                pass(n_tiles);
+                continue;
+            }
             const int32_t *trow = a.table + p.seq * a.table_stride;
             const uint64_t slice = is_v ? (static_cast<uint64_t>(p.head) * G::kSlices + rank) * G::V::kBytes : static_cast<uint64_t>(p.head) * G::K::kBytes;
             const int lead = a.tma ? static_cast<int>(slice & 15u) : 0;
@@ -1057,8 +1118,17 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
 #pragma unroll 1
             for (int32_t i = 0; i < n_boxes; ++i) {
                 const bool last = G::kBoxesV == 1 || !is_v || (i & 1);     // ... of its tile
-                if (a.tma) wait(&full[out_at], out_phase);
-                else cp_async_wait<NS - 1>();
+                if (a.tma) {
+                    const bool there = mbar_wait_near(&full[out_at], out_phase);
+                    if (!__all_sync(0xffffffffu, there)) {
+                        tile_abandon<PAIR>(&s_lost, full, out_at, out_phase, NS, n_boxes - i);
+                        dead = true;
+                        pass(n_tiles - i / boxes);
+                        break;
+                    }
+                } else {
+                    cp_async_wait<NS - 1>();
+                }
                 __syncwarp();
                 const uint32_t ok = ring_ok[0];
                 uint8_t *raw = ring + out_at * raw_bytes + lead;
@@ -1178,6 +1248,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     }
     __syncthreads();
     if constexpr (PAIR) cluster_sync();        // no product reads the peer's memory any more
+    if (*reinterpret_cast<volatile uint32_t *>(&s_lost)) tile_finish<PAIR>(mma_done);      // alike in a pair
     if (warp == 16) {
         tc_fence_after();
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

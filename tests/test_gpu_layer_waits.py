@@ -46,10 +46,14 @@ def check(kvm, torch, w, q, start, max_new, side):
     ("k", ("q4_0", "q4_0"), 128, 2, 6, [1] * 3, [300, 80, 700]),         # whole windows: a KV head a CTA, nothing cut
     ("v", ("q8_0", "q5_0"), 256, 4, 6, [1] * 2, [9000, 20000]),          # windows that many CTAs share
     ("k", ("f16", "q8_0"), 128, 4, 12, [1] * 9, [5000] * 9),             # row tiles of 16
-    ("v", ("q4_0", "f16"), 64, 4, 3, [2, 5, 1], [200, 4000, 64])])       # several rows a request
+    ("v", ("q4_0", "f16"), 64, 4, 3, [2, 5, 1], [200, 4000, 64]),        # several rows a request
+    ("k", ("q4_0", "q4_0"), 128, 2, 4, [20, 9, 31], [300, 2000, 100]),   # single CTAs, items of many CTAs
+    ("v", ("q8_0", "q4_0"), 64, 4, 8, [90, 40], [300, 90]),              # more than one piece a CTA
+    ("k", ("q4_0", "q4_0"), 128, 2, 4, [100, 20, 70], [400, 3000, 100]), # pairs: the first CTA's keys,
+    ("v", ("q8_0", "q4_0"), 256, 1, 6, [80], [5000])])                   # the second one's values
 def test_rows_that_never_arrive(kvm_lib, side, kinds, D, hkv, group, news, lens):
     import torch
     w = Window(kvm_lib, torch, D + len(lens), kinds, hkv, D, 32, lens)
     start = np.concatenate([[0], np.cumsum(news)])
     q = queries(torch, w.rng, int(start[-1]), hkv * group, D, "f16")
-    check(kvm_lib, torch, w, q, start, 1, side)
+    check(kvm_lib, torch, w, q, start, max(news) if max(news) > 8 else 1, side)
