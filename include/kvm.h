@@ -634,7 +634,9 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * j <= kv_len - n + i.  A row that sees no key is 0.  Keys beyond the table's
  * columns, keys from 2^31 - 65536 on and keys of a block whose entry is outside
  * [0, n_slots) are not seen.
- * What hidden keys hold -- stale bytes, infinities, NaN -- reaches no output.
+ * What hidden keys hold -- stale bytes, infinities, NaN -- reaches no output.  An infinite
+ * or NaN value of a key that a row sees makes its dims of the row infinite or NaN; where the
+ * key's weight underflows to 0 it may be left out instead.
  * Rows of q_start outside [0, n_rows) are skipped, and rows of out that belong
  * to no request stay as they were.  Query head h reads KV head
  * h / (n_head / n_head_kv).  q and out: F16 or BF16, head_dim 64, 128 or 256.

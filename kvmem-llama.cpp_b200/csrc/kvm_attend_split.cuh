@@ -579,7 +579,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 give_up(i, false);
                 break;
             }
-            const uint32_t ok = valid[at];
+            const uint32_t ok = valid[at] & kAll;         // 16 keys a step: the upper half is never written
             if (a.tma && ok != kAll) hidden(kr, SK{}, ok);
 
             // ---- K's scales, laid out for the products

@@ -128,3 +128,28 @@ def test_keys_beyond_f16(kvm_lib, kinds, D, group, new, T):
     want = reference(w, q.float().cpu().numpy(), [0, new], [keys], D ** -0.5)
     for got in results:
         agree(got, *want, keys)
+
+
+# ------------------------------------------- what ran on the SM before a call --
+
+def test_f16_decode_does_not_see_what_ran_before(kvm_lib):
+    """F16 rows of 256 dims come in steps of 16 keys.  The same bits whether another kernel
+    left ones or zeros in shared memory, with an infinite value whose weight underflows."""
+    import torch
+    n, keys = 160, 300
+    w = Window(kvm_lib, torch, 7, ("f16", "f16"), 1, 256, 32, [keys] * n)
+    for side, (scale, value) in enumerate(((0.1, -30.0), (1.0, np.inf))):
+        raw = (w.raw[side].view(np.float16) * np.float16(scale)).astype(np.float16)
+        for s in range(n):
+            raw[w.cell(s, 5)] = value
+        w.put(side, raw.view(np.uint8))
+    q = torch.ones((n, 4, 256), dtype=torch.float16, device="cuda")
+    before = Window(kvm_lib, torch, 8, ("q4_0", "q4_0"), 1, 256, 32, [4000])
+    rows = queries(torch, before.rng, 1200, 8, 256, "f16")
+    got = []
+    for byte in (0xFF, 0):
+        for side in (0, 1):
+            before.put(side, np.full_like(before.raw[side], byte))
+        before.run(rows, [0, 1200], max_new=1200)
+        got.append(w.run(q, range(n + 1)))
+    assert torch.equal(got[0].view(torch.int16), got[1].view(torch.int16))
