@@ -116,6 +116,7 @@ __device__ __forceinline__ void write_block(const float (&x)[32], uint8_t *dst) 
     float vmax = 0.0f;                       // the first value of the largest magnitude
 #pragma unroll
     for (int i = 31; i >= 0; --i) vmax = fabsf(x[i]) == amax ? x[i] : vmax;
+    vmax = __fadd_rn(vmax, 0.0f);            // a block of zeros: +0, whatever the first one's sign
     constexpr bool q5 = CT == KVM_TYPE_Q5_0;
     const float d = __fmul_rn(vmax, q5 ? -0.0625f : -0.125f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
     const float off = q5 ? 16.5f : 8.5f;
