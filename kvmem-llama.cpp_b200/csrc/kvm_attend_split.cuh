@@ -18,8 +18,9 @@
 // elements 2^17 below the row's largest); p and p*d are rounded to F16 (2^-11
 // relative, as the output type), sums and statistics are F32.  To use F16's
 // range, p is carried times 2^14 (which cancels in the quotient) and the scales
-// of V times the power of two that brings the largest met so far to [1, 2):
-// weights keep all bits down to 2^-28 of the row's largest.
+// of V times a power of two for each block of 32 dims, which brings the largest met so far to
+// [1, 2): weights keep all bits down to 2^-28 of the row's largest, scales down to 2^-14 of
+// the largest of the same dims.
 //
 // Layout.  S^T = K Q^T with 16 keys as M and 8 query rows as N, then
 // O^T = V^T P^T with dims as M: the few rows fill N = 8, codes are the A operand
@@ -567,7 +568,12 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[nt][b][0][i] = o[nt][b][1][i] = 0.0f;
         }
-        int vexp = 15;                        // o holds the output times 2^(vexp - 24)
+        // o holds the output times 2^(vexp - 24), vexp from 15 down by block: lane (g, t) keeps that
+        // of blocks 2t, 2t + 1 as the F16 pair 2^vexp and the largest scale bits it covers
+        uint32_t vmul = 0x78007800u, vcap = 0x03ff03ffu;
+        auto vexp = [&](int b) -> int {
+            return 16 - static_cast<int>((((__shfl_sync(0xffffffffu, vcap, b / 2) >> (16 * (b & 1))) & 0xffffu) + 1u) >> 10);
+        };
 
 #pragma unroll 1
         for (int i = 0; i < n_steps; ++i) {
@@ -741,38 +747,44 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                     top = __vmaxu2(top, d[i8] & 0x7fff7fffu);
                 }
                 // rarely: a scale beyond the range that vexp covers, or one that is not finite
-                const uint32_t over = static_cast<uint32_t>(16 - vexp) << 10;      // the smallest scale's bits out of range
-                if (__any_sync(0xffffffffu, (top & 0xffffu) >= over || (top >> 16) >= over)) {
-                    uint32_t finite = 0;
+                if (__any_sync(0xffffffffu, __vmaxu2(top, vcap) != vcap)) {
+                    uint32_t cap = 0, mul = 0, move = 0;       // by half: new vcap, vmul; how far vexp falls
 #pragma unroll
-                    for (int i8 = 0; i8 < 2 * MT; ++i8)
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t finite = 0;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
+                        for (int i8 = 0; i8 < 2 * MT; ++i8) {
                             const uint32_t size = (d[i8] >> (16 * h)) & 0x7fffu;
                             odd_values = odd_values || size >= 0x7c00u;
                             finite = max(finite, size >= 0x7c00u ? 0u : size);
                         }
+#pragma unroll
+                        for (int x = 4; x < 32; x *= 2) finite = max(finite, __shfl_xor_sync(0xffffffffu, finite, x));
+                        const uint32_t old = (vcap >> (16 * h)) & 0xffffu, now = max(old, finite | 0x3ffu);
+                        const uint32_t exponent = (now + 1u) >> 10;           // 16 - vexp
+                        cap |= now << (16 * h);
+                        mul |= (exponent <= 30u ? (31u - exponent) << 10 : 0x0200u) << (16 * h);       // the largest so far to [1, 2)
+                        move |= (exponent - ((old + 1u) >> 10)) << (16 * h);
+                    }
                     odd_values = __any_sync(0xffffffffu, odd_values);
-                    const int need = 15 - static_cast<int>(__reduce_max_sync(0xffffffffu, finite) >> 10);
-                    if (need < vexp) {        // the largest scale so far to [1, 2)
-                        const float f = __uint_as_float(static_cast<uint32_t>(need - vexp + 127) << 23);
+                    vcap = cap;
+                    vmul = mul;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const float f = __uint_as_float((127u - ((__shfl_sync(0xffffffffu, move, b / 2) >> (16 * (b & 1))) & 0xffffu)) << 23);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    o[nt][b][0][j] *= f;
-                                    o[nt][b][1][j] *= f;
-                                }
-                        vexp = need;
+                            for (int j = 0; j < 4; ++j) {
+                                o[nt][b][0][j] *= f;
+                                o[nt][b][1][j] *= f;
+                            }
                     }
                 }
-                const uint32_t mul = 0x10001u * (vexp >= -14 ? static_cast<uint32_t>(vexp + 15) << 10 : 0x0200u);   // 2^vexp
                 if (2 * t < NB) {
 #pragma unroll
                     for (int i8 = 0; i8 < 2 * MT; ++i8) {
-                        const uint32_t ds = mul_half2(d[i8], mul);
+                        const uint32_t ds = mul_half2(d[i8], vmul);
                         // key g of the half i8 & 1 of its 16: behind the pair's other key
                         __half *to = v16 + (i8 >> 1) * kVTile + 2 * t * kVBlock + (g >> 1) * 4 + (i8 & 1) * 2 + (g & 1);
                         to[0] = __ushort_as_half(static_cast<uint16_t>(ds & 0xffffu));
@@ -828,7 +840,9 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                 }
             } else {
                 // values that are not finite: by the definition, p = 0 leaves them out
-                const float unit = kCodesV ? __uint_as_float(static_cast<uint32_t>(vexp - 24 + 127) << 23) : 1.0f;
+                float unit[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) unit[b] = kCodesV ? __uint_as_float(static_cast<uint32_t>(vexp(b) - 24 + 127) << 23) : 1.0f;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll 1
@@ -846,7 +860,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
 #pragma unroll
                                     for (int h = 0; h < 2; ++h) {
                                         const float up = SV::kNibble && tile ? 16.0f : 1.0f;
-                                        const float v = row_value<VT>(row, v_dim<VT>(b, tile, h, g)) * unit * up;
+                                        const float v = row_value<VT>(row, v_dim<VT>(b, tile, h, g)) * unit[b] * up;
                                         if (p0 != 0.0f) o[nt][b][tile][2 * h] += p0 * v;
                                         if (p1 != 0.0f) o[nt][b][tile][2 * h + 1] += p1 * v;
                                     }
@@ -871,7 +885,9 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
         __syncthreads();
         float *sm_m = reinterpret_cast<float *>(smem), *sm_l = sm_m + W * R, *sm_o = sm_l + W * R;
         constexpr int OS = D + 4;
-        const float unit = kCodesV ? __uint_as_float(static_cast<uint32_t>(24 - vexp + 127) << 23) : 1.0f;
+        float unit[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) unit[b] = kCodesV ? __uint_as_float(static_cast<uint32_t>(24 - vexp(b) + 127) << 23) : 1.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -894,7 +910,7 @@ __global__ void __launch_bounds__((SplitGeom<D, KT, VT, NT>::kThreads), 1) atten
                     for (int j = 0; j < 4; ++j) {
                         const float up = SV::kNibble && tile ? 0.0625f : 1.0f;
                         sm_o[(warp * R + nt * 8 + 2 * t + (j & 1)) * OS + v_dim<VT>(b, tile, j >> 1, g)] =
-                            o[nt][b][tile][j] * unit * up;
+                            o[nt][b][tile][j] * unit[b] * up;
                     }
         }
         __syncthreads();

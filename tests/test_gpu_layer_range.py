@@ -153,3 +153,20 @@ def test_f16_decode_does_not_see_what_ran_before(kvm_lib):
         before.run(rows, [0, 1200], max_new=1200)
         got.append(w.run(q, range(n + 1)))
     assert torch.equal(got[0].view(torch.int16), got[1].view(torch.int16))
+
+
+# ------------------------------------- value blocks of very different sizes --
+
+@pytest.mark.parametrize("kinds", [("q4_0", "q4_0"), ("q8_0", "q8_0"), ("f16", "q5_0")])
+@pytest.mark.parametrize("D, group, new", [(64, 2, 1), (128, 6, 1), (256, 6, 1), (128, 12, 1), (256, 6, 20)])
+@pytest.mark.parametrize("apart", [14, 20, 26])
+def test_value_blocks_of_very_different_sizes(kvm_lib, kinds, D, group, new, apart):
+    """Every other block of 32 dims is 2^-apart of its neighbours: each dim keeps its own
+    relative accuracy."""
+    import torch
+    keys = 260
+    w = Window(kvm_lib, torch, D + new, kinds, 1, D, 32, [keys, 90])
+    rewrite(w, 1, lambda v: v * np.where(np.arange(D) // 32 % 2, 2.0 ** (6 - apart), 2.0 ** 6))
+    q = queries(torch, w.rng, 2 * new, group, D, "bf16")
+    got = w.run(q, [0, new, 2 * new], True, max_new=new)
+    agree(got, *reference(w, q.float().cpu().numpy(), [0, new, 2 * new], [keys, 90], D ** -0.5), keys)
