@@ -194,21 +194,14 @@ constexpr uint32_t tc_idesc(int m, int n, bool b_mn_major) {
 }
 
 // ------------------------------------------------------------- work line --
-// sum_{i < n} floor((a i + b) / m), all arguments non-negative, m > 0.
-__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-    int64_t sum = 0;
-    for (;;) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const int64_t top = a * n + b;
-        if (top < m) return sum;
-        n = top / m;
-        b = top % m;
-        const int64_t x = m;
-        m = a;
-        a = x;
-    }
+// sum_{i < n} floor((2 i + e) / g), e >= 0, g > 0.  With e = g (e / g) + e0 and i = g k + r the
+// term is e / g + 2 k + floor((2 r + e0) / g), whose last part is 0, 1 or 2: it counts how
+// many of the borders g and 2 g lie at or below 2 r + e0.
+__host__ __device__ inline int64_t sum_of_halves(int64_t n, int64_t e, int64_t g) {
+    const int64_t e0 = e % g, turns = n / g, rest = n % g;
+    const int64_t one = (g - e0 + 1) / 2, two = (2 * g - e0 + 1) / 2;      // the first r past each border
+    auto part = [&](int64_t r) -> int64_t { return (r > one ? r - one : 0) + (r > two ? r - two : 0); };
+    return n * (e / g) + turns * (turns - 1) * g + turns * part(g) + 2 * turns * rest + part(rest);
 }
 
 struct TileSeq {
@@ -239,9 +232,11 @@ __host__ __device__ __forceinline__ int64_t tile_steps(const AttendArgs &a, cons
 // Key tiles of the first n row tiles.  Row tile i's last token is
 // floor((ROWS (i + 1) - 1) / group) (the sequence's last for the last tile), so its
 // count is floor((group (shift + KEYS) + ROWS (i + 1) - 1) / (KEYS group)) between the
-// tiles that need one key tile and those that see `cap` keys.
+// tiles that need one key tile and those that see `cap` keys.  ROWS is 2 KEYS, so a KEYS
+// of both can be divided out first.
 template <int ROWS, int KEYS>
 __host__ __device__ inline int64_t tile_prefix(const AttendArgs &a, const TileSeq &t, int64_t n) {
+    static_assert(ROWS == 2 * KEYS, "the sum below");
     const int64_t most = max(static_cast<int64_t>(1), (t.cap + KEYS - 1) / KEYS);
     if (!a.causal) return n * most;
     if (n <= 1) return n ? tile_steps<ROWS, KEYS>(a, t, 0) : 0;
@@ -254,7 +249,7 @@ __host__ __device__ inline int64_t tile_prefix(const AttendArgs &a, const TileSe
     const int64_t ones = first_with(KEYS + 1), full = max(ones, first_with(t.cap));
     int64_t sum = ones + (n - full) * most;
     if (full > ones)
-        sum += floor_sum(full - ones, KEYS * g, ROWS, g * (shift + KEYS) + ROWS * ones + ROWS - 1);
+        sum += sum_of_halves(full - ones, (g * (shift + KEYS) + ROWS * ones + ROWS - 1) / KEYS, g);
     return sum;
 }
 
