@@ -373,9 +373,12 @@ __host__ __device__ constexpr int tile_order(int i) {
 template <int T>
 constexpr uint32_t kTileWide = T == KVM_TYPE_F16 ? 0x7c00u : 0x7c00u - (static_cast<uint32_t>(Slice<T, 64>::kOffsetLog) << 10);
 
+// The rare paths are functions of their own, one copy a kernel (KERNEL): called by all the
+// kernels of a translation unit, they cost a prompt of 2048 tokens 1567 -> 1625 us.
+
 // Drops from a warp's 16 raw rows what must not reach a product: hidden keys (not
 // in `ok`) become zeros, and with IS_V the blocks or values that are wide (kTileWide).
-template <int T, int D, bool IS_V>
+template <int KERNEL, int T, int D, bool IS_V>
 __device__ __noinline__ void tile_clean(uint8_t *raw, uint32_t ok, int lane) {
     using S = Slice<T, D>;
     {
@@ -513,13 +516,13 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
     return top >= kTileWide<T>;
 }
 
-template <int T, int D, int ROWS>
+template <int KERNEL, int T, int D, int ROWS>
 __device__ __noinline__ void tile_dequant_low(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
     tile_dequant<T, D, ROWS, true>(raw, tile, key0, lane);
 }
 
 // A wait ran out: results of this CTA and its peer are void from here on.
-template <bool PAIR>
+template <int KERNEL, bool PAIR>
 __device__ __noinline__ void tile_say_lost(uint32_t *lost) {
     *reinterpret_cast<volatile uint32_t *>(lost) = 1u;
     if constexpr (PAIR) {
@@ -532,9 +535,9 @@ __device__ __noinline__ void tile_say_lost(uint32_t *lost) {
 
 // A warp's raw rows did not come: its n loads under way, the ring's slots from `at` on, land
 // before it goes on.
-template <bool PAIR>
+template <int KERNEL, bool PAIR>
 __device__ __noinline__ void tile_abandon(uint32_t *lost, uint64_t *full, uint32_t at, uint32_t phase, uint32_t slots, int32_t n) {
-    tile_say_lost<PAIR>(lost);
+    tile_say_lost<KERNEL, PAIR>(lost);
     for (uint32_t k = 0; k < slots && static_cast<int32_t>(k) < n; ++k) {
         mbar_wait_bounded(&full[at], phase);
         if (++at == slots) {
@@ -547,7 +550,7 @@ __device__ __noinline__ void tile_abandon(uint32_t *lost, uint64_t *full, uint32
 
 // The kernel's end behind a wait that ran out: products may be under way; TMEM is freed
 // behind them.
-template <bool PAIR>
+template <int KERNEL, bool PAIR>
 __device__ __noinline__ void tile_finish(uint64_t *mma_done) {
     if (threadIdx.x / 32 == 16) {
         if ((threadIdx.x & 31u) == 0u && (!PAIR || (blockIdx.x & 1u) == 0u)) {
@@ -563,7 +566,7 @@ __device__ __noinline__ void tile_finish(uint64_t *mma_done) {
 
 // q . k of one row and one key by the definition, in F32, from the tensors in device
 // memory: for the keys whose values the tiles leave out.
-template <int T, int D>
+template <int KERNEL, int T, int D>
 __device__ __noinline__ float tile_score(const uint8_t *q, uint64_t nb_dim, int32_t bf16, const uint8_t *k) {
     float sum = 0.0f;
 #pragma unroll 8
@@ -579,6 +582,7 @@ template <int D, int KT, int VT, bool PAIR>
 __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     using G = TileGeom<D, KT, VT, PAIR>;
     constexpr int NS = G::kStages, kKeys = G::kKeys, kRows = G::kRows, kCtas = PAIR ? 2 : 1;
+    constexpr int kKernel = 2 * VT + (PAIR ? 1 : 0);         // D and KT are alike in a translation unit
     constexpr float kNegInf = -__builtin_huge_valf(), kWeightLog = 7.0f, kSlack = 8.0f;
     constexpr uint32_t kColS = 0, kColO = 2 * kKeys, kColQ = kColO + D;       // kColQ: single CTAs only
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -699,7 +703,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     auto wait = [&](uint64_t *bar, uint32_t phase) {
         if (!lost && !mbar_wait_near(bar, phase & 1u)) {
             lost = true;
-            tile_say_lost<PAIR>(&s_lost);
+            tile_say_lost<kKernel, PAIR>(&s_lost);
         }
         // together: a lane that went ahead could let the phase after this one complete
         // while another still polls for this one
@@ -942,7 +946,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                         if (!wide) continue;
                         // the weight as the products' S gives it but for K's rounding; one that
                         // underflows leaves the value out
-                        const float score = tile_score<KT, D>(qp, a.q.nb_dim, a.q.bf16, a.k + cell * a.row_k + static_cast<uint64_t>(p.head) * G::K::kBytes);
+                        const float score = tile_score<kKernel, KT, D>(qp, a.q.nb_dim, a.q.bf16, a.k + cell * a.row_k + static_cast<uint64_t>(p.head) * G::K::kBytes);
                         const float weight = exp2_approx(score * a.scale_log2 + (kWeightLog - m)) * inv;
                         if (weight == 0.0f) continue;
 #pragma unroll
@@ -1116,7 +1120,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 if (a.tma) {
                     const bool there = mbar_wait_near(&full[out_at], out_phase);
                     if (!__all_sync(0xffffffffu, there)) {
-                        tile_abandon<PAIR>(&s_lost, full, out_at, out_phase, NS, n_boxes - i);
+                        tile_abandon<kKernel, PAIR>(&s_lost, full, out_at, out_phase, NS, n_boxes - i);
                         dead = true;
                         pass(n_tiles - i / boxes);
                         break;
@@ -1133,8 +1137,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 }
                 constexpr int kVD = PAIR ? D / 2 : D;
                 if ((ok & 0xffffu) != 0xffffu) {
-                    if (is_v) tile_clean<VT, kVD, false>(raw, ok & 0xffffu, lane);
-                    else tile_clean<KT, D, false>(raw, ok & 0xffffu, lane);
+                    if (is_v) tile_clean<kKernel, VT, kVD, false>(raw, ok & 0xffffu, lane);
+                    else tile_clean<kKernel, KT, D, false>(raw, ok & 0xffffu, lane);
                 }
                 if (j >= 2 && (G::kBoxesV == 1 || !is_v || !(i & 1))) wait(&tile_free[j & 1u], (j >> 1) - 1u);
                 uint8_t *tile = smem + (is_v ? 2 * G::kOperand : 0) + (j & 1u) * G::kOperand;
@@ -1142,7 +1146,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     const int at = w4 * 16 * G::kBoxesV + (G::kBoxesV == 2 ? 16 * (i & 1) : 0);
                     if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane))) {
                         // the epilogue adds these values with their weights; the products do without them
-                        tile_clean<VT, kVD, true>(raw, ok & 0xffffu, lane);
+                        tile_clean<kKernel, VT, kVD, true>(raw, ok & 0xffffu, lane);
                         tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane);
                         if constexpr (PAIR) {
                             if (lane < kCtas) st_shared_at(&s_odd, 1u, lane);
@@ -1155,7 +1159,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     const bool wide = tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
                     if constexpr (KT != KVM_TYPE_F16) {
                         const uint32_t low = __any_sync(0xffffffffu, wide) ? 1u : 0u;
-                        if (low) tile_dequant_low<KT, D, 64>(raw, tile, w4 * 16, lane);
+                        if (low) tile_dequant_low<kKernel, KT, D, 64>(raw, tile, w4 * 16, lane);
                         if (low != ((low_tiles >> (j & 3u)) & 1u)) {       // read beside valid[]: written as early
                             low_tiles ^= 1u << (j & 3u);
                             if constexpr (PAIR) {
@@ -1243,7 +1247,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     }
     __syncthreads();
     if constexpr (PAIR) cluster_sync();        // no product reads the peer's memory any more
-    if (*reinterpret_cast<volatile uint32_t *>(&s_lost)) tile_finish<PAIR>(mma_done);      // alike in a pair
+    if (*reinterpret_cast<volatile uint32_t *>(&s_lost)) tile_finish<kKernel, PAIR>(mma_done);      // alike in a pair
     if (warp == 16) {
         tc_fence_after();
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
