@@ -26,7 +26,7 @@ def reference(w, q, start, lens, scale, causal=True, rows=None):
         for r in range(lo, hi):
             if rows is not None and r not in rows:
                 continue
-            c = cell[:kv - (hi - lo) + (r - lo) + 1] if causal else cell
+            c = cell[:max(0, kv - (hi - lo) + (r - lo) + 1)] if causal else cell
             if c.size == 0:
                 continue
             for h in range(hq):
