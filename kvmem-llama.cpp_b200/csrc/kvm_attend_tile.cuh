@@ -591,12 +591,12 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBars);
     uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
              *q_full = bars + 12, *raw_full = bars + 13, *mma_done = bars + 13 + 8 * NS;      // raw_full [8 warps][NS]
-    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);      // [4 tiles][kKeys / 16], a bit a key
+    // [4 tiles][kKeys / 16]: a bit for each hidden one of 16 keys; byte 2: their K box is LOW
+    uint32_t *valid = reinterpret_cast<uint32_t *>(bars + 14 + 8 * NS);
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = blockIdx.x / kCtas, n_units = gridDim.x / kCtas;
     __shared__ unsigned long long s_scan[kTileThreads / 32], s_off;
     __shared__ uint32_t s_seq, s_tmem, s_odd, s_lost;  // s_lost: a wait of this CTA or its peer ran out
     __shared__ float s_swap[2][2 * kTileRows];
-    __shared__ __align__(8) uint8_t s_low[4][8];       // K boxes of a tile (16 keys each) that are LOW
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -614,7 +614,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         for (int i = 0; i < 8 * NS; ++i) mbar_init(&raw_full[i], i == skip_k || i == skip_v ? 2 : 1);
         mbar_init(mma_done, 1);
         s_odd = s_lost = 0;
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint64_t *>(s_low[i]) = 0;
+        for (int i = 0; i < 4 * kKeys / 16; ++i) valid[i] = 0;
         fence_mbar_init();
     }
     __syncthreads();
@@ -833,21 +833,19 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                 auto columns = [&](int c) {
                     tc_ld32(s, lanes + kColS + st * kKeys + wg * kHalf + 32 * c);
                     tc_wait_ld();
-                    const uint2 ok2 = *reinterpret_cast<const uint2 *>(valid + (kKeys / 16) * (j & 3u) + wg * (kHalf / 16) + 2 * c);
-                    const uint32_t ok = ok2.x | ok2.y << 16;
+                    const uint2 word = *reinterpret_cast<const uint2 *>(valid + (kKeys / 16) * (j & 3u) + wg * (kHalf / 16) + 2 * c);
                     const int32_t key0 = n * kKeys + wg * kHalf + 32 * c;
-                    uint32_t low = 0;
-                    if constexpr (KT != KVM_TYPE_F16) low = *reinterpret_cast<const uint16_t *>(&s_low[j & 3u][wg * (kHalf / 16) + 2 * c]);
-                    if (key0 + 32 > kfull || ok != 0xffffffffu || low != 0u) {
-                        constexpr float kUp = static_cast<float>(1 << Slice<KT, 64>::kOffsetLog);
-                        const float up0 = low & 0xffu ? kUp : 1.0f, up1 = low >> 8 ? kUp : 1.0f;
-                        if (KT != KVM_TYPE_F16 && low != 0u) {
+                    if (key0 + 32 > kfull || (word.x | word.y) != 0u) {
+                        if (KT != KVM_TYPE_F16 && ((word.x | word.y) >> 16) != 0u) {
+                            constexpr float kUp = static_cast<float>(1 << Slice<KT, 64>::kOffsetLog);
+                            const float up0 = word.x >> 16 ? kUp : 1.0f, up1 = word.y >> 16 ? kUp : 1.0f;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * (i < 16 ? up0 : up1));
                         }
+                        const uint32_t hidden = __byte_perm(word.x, word.y, 0x5410);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (key0 + i >= lim || !((ok >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
+                            if (key0 + i >= lim || ((hidden >> i) & 1u)) s[i] = __float_as_uint(kNegInf);
                     }
                 };
                 float x = kNegInf;
@@ -1022,7 +1020,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
         uint8_t *ring = smem + G::kRaw + (is_v ? 4 * NS * G::kBoxK : 0) + w4 * NS * raw_bytes;
         uint64_t *full = raw_full + (warp - 8) * NS, *tile_full = is_v ? v_full : k_full, *tile_free = is_v ? v_free : k_free;
         uint32_t in_at = 0, out_at = 0, out_phase = 0;     // ring slot of the next load, of the next box
-        uint32_t low_tiles = 0;                            // this K warp's marks in s_low, a bit a tile
+        [[maybe_unused]] uint32_t low_tiles = 0;                            // this K warp's LOW marks in valid[], a bit a tile
         bool dead = false;                                 // rows never came: no more loads, the others are let pass
         auto pass = [&](int32_t tiles) {
             for (; tiles > 0; --tiles, ++j)
@@ -1157,20 +1155,23 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     }
                 } else {
                     const bool wide = tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
+                    uint32_t low = 0;
                     if constexpr (KT != KVM_TYPE_F16) {
-                        const uint32_t low = __any_sync(0xffffffffu, wide) ? 1u : 0u;
+                        low = __any_sync(0xffffffffu, wide) ? 1u : 0u;
                         if (low) tile_dequant_low<kKernel, KT, D, 64>(raw, tile, w4 * 16, lane);
-                        if (low != ((low_tiles >> (j & 3u)) & 1u)) {       // read beside valid[]: written as early
+                        if (PAIR && low != ((low_tiles >> (j & 3u)) & 1u)) {       // read with the bits, so written as early
                             low_tiles ^= 1u << (j & 3u);
-                            if constexpr (PAIR) {
-                                if (lane < kCtas) st_shared_at(&s_low[j & 3u][mine / 16], low, lane);
-                                asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                            } else if (lane == 0) {
-                                *reinterpret_cast<volatile uint8_t *>(&s_low[j & 3u][mine / 16]) = static_cast<uint8_t>(low);
-                            }
+                            uint8_t *at = reinterpret_cast<uint8_t *>(valid + (kKeys / 16) * (j & 3u) + mine / 16) + 2;
+                            if (lane < kCtas) st_shared_at(at, low, lane);
+                            asm volatile("fence.acq_rel.cluster;" ::: "memory");
                         }
                     }
-                    if (lane < kLooks) valid[(kKeys / 16) * (j & 3u) + (mine + theirs * lane) / 16] = (ok >> (16 * lane)) & 0xffffu;
+                    if constexpr (PAIR) {
+                        if (lane < kLooks)
+                            *reinterpret_cast<uint16_t *>(valid + (kKeys / 16) * (j & 3u) + (mine + theirs * lane) / 16) = static_cast<uint16_t>(~(ok >> (16 * lane)));
+                    } else if (lane == 0) {
+                        valid[(kKeys / 16) * (j & 3u) + mine / 16] = low << 16 | (~ok & 0xffffu);
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
