@@ -645,9 +645,11 @@ kvm_status kvm_read_rows(kvm_stream stream, const kvm_cache *cache, uint32_t n,
  * the query heads of a KV head is at most 16, K and V values may enter the products
  * rounded to F16: by 2^-11 of a value, of any size that the rows' formats hold, and where 16
  * neighbouring keys hold values beyond 65504 also by 2^-33 of the largest of these.
- * out must not overlap q, the cache or the workspace.  Waits inside the kernels
- * are bounded (2 s); one that runs out leaves NaN in every row that its CTA still works
- * on, never a wrong value or a hang, and no copy is under way when the kernel ends.
+ * V values beyond 65504, infinities and NaN are added one by one there, some 40 us a key for
+ * the rows of a CTA: more than 40000 such keys of a request can run out a wait (below).
+ * out must not overlap q, the cache or the workspace.  Waits inside the kernels are bounded
+ * (2 s); one that runs out leaves NaN in every row that its CTA still works on, never a
+ * wrong value or a hang, and no copy is under way when the kernel ends.
  * max_new: the most rows of a request, as far as the caller knows.  It picks the
  * kernel: a wrong value costs time and may change the roundings, never more.
  * d_work: KVM_ATTEND_WORK_BYTES of device memory, 16-byte aligned, that no
