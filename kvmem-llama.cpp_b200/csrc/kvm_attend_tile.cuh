@@ -516,9 +516,9 @@ __device__ __forceinline__ bool tile_dequant(const uint8_t *raw, uint8_t *tile, 
     return top >= kTileWide<T>;
 }
 
-template <int KERNEL, int T, int D, int ROWS>
-__device__ __noinline__ void tile_dequant_low(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
-    tile_dequant<T, D, ROWS, true>(raw, tile, key0, lane);
+template <int KERNEL, int T, int D, int ROWS, bool LOW>
+__device__ __noinline__ void tile_dequant_again(const uint8_t *raw, uint8_t *tile, int key0, int lane) {
+    tile_dequant<T, D, ROWS, LOW>(raw, tile, key0, lane);
 }
 
 // A wait ran out: results of this CTA and its peer are void from here on.
@@ -530,6 +530,16 @@ __device__ __noinline__ void tile_say_lost(uint32_t *lost) {
         asm volatile("fence.acq_rel.cluster;" ::: "memory");
     } else {
         __threadfence_block();
+    }
+}
+
+// Some values stay out of the tiles: the epilogues of both CTAs look for them.
+template <int KERNEL, bool PAIR>
+__device__ __noinline__ void tile_say_odd(uint32_t *odd) {
+    *reinterpret_cast<volatile uint32_t *>(odd) = 1u;
+    if constexpr (PAIR) {
+        st_shared_at(odd, 1u, (blockIdx.x & 1u) ^ 1u);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
     }
 }
 
@@ -1187,20 +1197,15 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
                     if (__any_sync(0xffffffffu, tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane))) {
                         // the epilogue adds these values with their weights; the products do without them
                         tile_clean<kKernel, VT, kVD, true>(raw, ok & 0xffffu, lane);
-                        tile_dequant<VT, kVD, kKeys>(raw, tile, at, lane);
-                        if constexpr (PAIR) {
-                            if (lane < kCtas) st_shared_at(&s_odd, 1u, lane);
-                            asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                        } else {
-                            *reinterpret_cast<volatile uint32_t *>(&s_odd) = 1u;
-                        }
+                        tile_dequant_again<kKernel, VT, kVD, kKeys, false>(raw, tile, at, lane);
+                        tile_say_odd<kKernel, PAIR>(&s_odd);
                     }
                 } else {
                     const bool wide = tile_dequant<KT, D, 64>(raw, tile, w4 * 16, lane);
                     uint32_t low = 0;
                     if constexpr (KT != KVM_TYPE_F16) {
                         low = __any_sync(0xffffffffu, wide) ? 1u : 0u;
-                        if (low) tile_dequant_low<kKernel, KT, D, 64>(raw, tile, w4 * 16, lane);
+                        if (low) tile_dequant_again<kKernel, KT, D, 64, true>(raw, tile, w4 * 16, lane);
                         if (PAIR && low != ((low_tiles >> (j & 3u)) & 1u)) {       // read with the bits, so written as early
                             low_tiles ^= 1u << (j & 3u);
                             uint8_t *at = reinterpret_cast<uint8_t *>(valid + (kKeys / 16) * (j & 3u) + mine / 16) + 2;
