@@ -149,14 +149,17 @@ extern "C" kvm_status kvm_attend(kvm_stream stream, const kvm_cache *c, const kv
         return launch_d<256>(a, c->type_k, c->type_v, nt, grid, st);
     };
     // Requests of up to 16 query rows go to the split kernel, longer ones to the tile
-    // kernel; the device sorts them, so a wrong max_new only costs time.  Alike
-    // requests (one, or drafts that fit a row tile with more than 8 rows on average)
-    // take one kernel: the tile kernel's time hardly depends on the rows in a tile,
-    // and eight drafts of 1 to 4 tokens over 16385 keys took 145 us in both.
-    // Few requests do better in row tiles of 8 (24 query and 4 KV heads of 256, us): 12 rows
-    // of 1 request of 32768 keys 34, in tiles of 16 39; 8 of 16385 94 and 103; 32 of
-    // 1024 40 and 33.  24 rows of 1 request of 32768 keys 42, in the tile kernel 55; 2 of
-    // 8192 35 and 42; 4 of 2048 31 and 27.
+    // kernel; the device sorts them, so a wrong max_new costs time and the tile kernel's
+    // roundings, nothing else.  Alike requests (one, or drafts that fit a row tile with more
+    // than 8 rows on average) take one kernel, since the tile kernel's time hardly depends
+    // on the rows in a tile: 24 rows of 32 alike requests of 2048 keys 89 us, in row tiles of
+    // 8 112, of 16 135.
+    // Few requests do better in row tiles of 8 (24 query and 4 KV heads of 256, us; the borders
+    // were set on this layer): 12 rows of 1 request of 32768 keys 34, in tiles of 16 39; 8 of
+    // 16385 94 and 103; 32 of 1024 42 and 33.  24 rows of 1 request of 32768 keys 42, in the tile
+    // kernel 60; 2 of up to 8192 30 and 43; 4 alike of 2048 31 and 27, 8 alike of 16384 138 and
+    // 134, but 8 of all lengths up to that 76 and 87.  8 KV heads of 128, q8_0, 24 rows of 8
+    // alike requests of 2048: 49 and 40.
     const uint64_t most = static_cast<uint64_t>(b->max_new) * a.group;
     cudaError_t e;
     if (most <= 16u || (most <= 24u && b->n_seq <= 3u)) {

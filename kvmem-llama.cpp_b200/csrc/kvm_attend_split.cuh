@@ -16,7 +16,8 @@
 // Rounding: q enters in F16, scaled by a power of two a row so that its largest
 // element is near the top of the range (exact for F16 and BF16 inputs but for
 // elements 2^17 below the row's largest); p and p*d are rounded to F16 (2^-11
-// relative, as the output type), sums and statistics are F32.  To use F16's
+// relative, as the output type), sums and statistics are F32; the two terms of o_e cancel
+// where values are small beside their block's largest, to some 2^-18 of that.  To use F16's
 // range, p is carried times 2^14 (which cancels in the quotient) and the scales
 // of V times a power of two for each block of 32 dims, which brings the largest met so far to
 // [1, 2): weights keep all bits down to 2^-28 of the row's largest, scales down to 2^-14 of
@@ -36,14 +37,15 @@
 // block and rows are multiples of 16 bytes, else by cp.async.
 //
 // Measured (24 query and 4 KV heads of 256).  32 requests over ragged windows of up
-// to 32768 keys, q4_0: 162 us for 569 MB = 3.5 TB/s; 16 of up to 20001, q8_0 keys
-// and q4_0 values: 78 us = 3.7 TB/s.  Not the bytes bound it (87 and 44 us) but the
-// instructions around the products: a 16-key step costs 12 warps a scheduler's 52 %
-// of issue slots and 30 % of the tensor pipe, whose m16n8k16 takes 8 cycles for 8
-// rows of N of which 6 are used.  One request of 32768 keys: 24 us, 11 of them a
+// to 32768 keys, q4_0: 164 us for 569 MB = 3.5 TB/s (q5_0 275, q8_0 207, F16 333 us, the last
+// the bytes' own 328); 16 of up to 20001, q8_0 keys and q4_0 values: 76 us = 3.8 TB/s.  No unit
+// is full: three warps a scheduler, each a chain of dependent steps, take 52 % of the issue
+// slots and 29 % of the tensor pipe, whose m16n8k16 takes 8 cycles for 8 rows of N of which 6
+// are used; of 49 products a 16-key step 16 are the offset's.  168 registers, 78 bytes of
+// spills.  One request of 32768 keys (38 MB, in L2 when repeated): 25 us, 11 of them a
 // CTA's (queries and first rows 5, steps 3, merge 2), the rest launches and the join.
 // 2 requests of up to 333 keys (2 heads of 128): 10 us.  With 16 rows (two products a
-// code) the time is 1.6 times that of 8.
+// code; 255 registers, 580 bytes of spills) the time is 1.6 times that of 8.
 #pragma once
 
 #include "kvm_attend.cuh"

@@ -31,13 +31,14 @@
 //    only half of every tile (64 keys of K, half of V's dims) for 256 rows.  Q is in
 //    shared memory there: 2 x 128 columns of S and 256 of O fill TMEM.
 //    2048 tokens behind a window of 32768 keys (24 heads of 256, q4_0): 2.29 ms by
-//    single CTAs, 1.56 ms by pairs.
+//    single CTAs, 1.54 ms by pairs (1.54 to 1.79 ms by the card's power cap).
 //
 // Roles (17 warps, one CTA an SM): warps 0-7 own 128 rows (Q, softmax, epilogue),
 // two threads a row with half the columns each; warps 8-11 turn raw K rows into an
 // operand tile, warps 12-15 raw V rows, warp 16 issues the products.  (One thread a
 // row left a single softmax warp on each scheduler, whose latencies alone took 2250
-// cycles a tile.  25 warps leave 72 registers a thread: slower, they spill.)
+// cycles a tile.  All warps have the same 96 registers and spill 340 bytes (pairs 500)
+// at 256 dims; 25 warps would have 72 and were slower.)
 // Everything is double-buffered on mbarriers: S of tile j + 1 is issued before O of
 // tile j, so that the softmax of one tile runs under the products of the other.
 // Raw rows come through a ring a warp, 16 keys a slot, refilled as soon as a slot
@@ -48,10 +49,10 @@
 // each: 850 of conversion, the rest barriers, fences and the load's issue), with the
 // softmax warps (3100) behind it.  Giving every dequantizing warp a box of K and
 // one of V, half the dims each, was slower (1.67 ms).  Drafts (8 requests of 4
-// tokens, 80,000 keys): 85 us against 14 for their bytes (90 while the warps without
-// rows worked and polled along, 87 with a join of one part after the other).  The
-// time hardly depends on the rows: a 64-key tile costs 4000 cycles, 2100 of them a
-// box's conversion.
+// tokens, 80,000 keys): 87 us against 14 for their bytes.  The time hardly depends on the
+// rows: a 64-key tile costs 4000 cycles, 2100 of them a box's conversion, while six of the
+// eight softmax warps sleep (their polling cost 3 us); 1.5 stalls an issue are
+// instruction fetch.  F16 K and V, by single CTAs: 2.67 ms for the prompt.
 //
 // Operand tiles: rows of keys by 128-byte chunks of 64 dims with the 128-byte
 // swizzle; K is read K-major, V from the same layout MN-major.  Which dim a

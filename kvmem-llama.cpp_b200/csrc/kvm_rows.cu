@@ -12,12 +12,13 @@
 // shared memory and leave as words, two blocks (always a whole number of words)
 // at a time.  Read: a thread 16 values, two 16-byte stores.
 //
-// 8191 rows of 4 heads of 256 on both sides (q8_0 keys, q4_0 values): 11 us to write
-// (F16 in), 11 us to read (BF16 out), 47 MB each = 4.3 TB/s; a copy of those bytes
-// takes 7.  Issue slots are 60 % busy, with 20 to 35 % of the cycles in waits for the
-// loads.  64 rows: 2.3 us each.  Types as template arguments and divisions as
-// products took it from 33 us for both to 24, 64 instead of 74 registers (four
-// CTAs an SM) to 22.
+// 8191 rows of 4 heads of 256 on both sides (q8_0 keys, q4_0 values), F16 in and BF16 out:
+// 26 us to write and read them, 94 MB = 3.6 TB/s, over tensors larger than L2 together (22 us
+// where a graph repeats one call, whose 94 MB stay in L2); a copy of those bytes takes 14.
+// Issue slots are 60 % busy, with 20 to 35 % of the cycles in waits for the loads.  64 rows:
+// 2.3 us each.  Types as template arguments and divisions as products took the repeated call
+// from 33 us to 24, 64 instead of 74 registers (four CTAs an SM) to 22.  F16 cache
+// rows move in 2-byte accesses: 144 us for 8191.
 #include <cuda_bf16.h>
 
 #include "kvm_layer.cuh"
