@@ -352,6 +352,7 @@ def _layer_stream(stream, dev):
 _PACK_ROWS = struct.Struct("=QiIIIQQQ").pack
 _PACK_MAP = struct.Struct("=QQQQQIIIIIIQQQQQQ").pack
 _PACK_ATTEND = struct.Struct("=QQIIQQIIIf").pack
+_UNFIT = (struct.error, OverflowError)       # a number that does not fit its field
 
 
 def _act(t, what, dev):
@@ -414,11 +415,14 @@ def map_batch(past, new, free_slots, block_tokens, table, q_start, kv_len, cells
     dev = _device(past, "past")
     i32, n, rows = _Torch.i32, past.numel(), cells.numel()
     tab, stride, cols = _table(table, n, dev)
-    m = _PACK_MAP(_index(past, i32, n, "past", dev), _index(new, i32, n, "new", dev),
-                  _index(free_slots, i32, 0, "free_slots", dev), tab, stride, cols, n, free_slots.numel(), block_tokens,
-                  rows, 0, _index(q_start, i32, n + 1, "q_start", dev), _index(kv_len, i32, n, "kv_len", dev),
-                  _index(cells, _Torch.i64, rows, "cells", dev), _index(pos, i32, rows, "pos", dev),
-                  _index(seq, i32, rows, "seq", dev), _index(info, i32, 4, "info", dev))
+    try:
+        m = _PACK_MAP(_index(past, i32, n, "past", dev), _index(new, i32, n, "new", dev),
+                      _index(free_slots, i32, 0, "free_slots", dev), tab, stride, cols, n, free_slots.numel(), block_tokens,
+                      rows, 0, _index(q_start, i32, n + 1, "q_start", dev), _index(kv_len, i32, n, "kv_len", dev),
+                      _index(cells, _Torch.i64, rows, "cells", dev), _index(pos, i32, rows, "pos", dev),
+                      _index(seq, i32, rows, "seq", dev), _index(info, i32, 4, "info", dev))
+    except _UNFIT as e:
+        _bad(f"block_tokens {block_tokens!r}: {e}")
     _layer_check(lib().kvm_map_batch(_layer_stream(stream, dev), m))
 
 
@@ -490,8 +494,11 @@ def attend(cache, q, q_start, kv_len, table, out, work, scale, causal=True, max_
         _bad(f"work: a contiguous tensor on cuda:{dev}")
     tab, stride, cols = _table(table, n, dev)
     i32 = _Torch.i32
-    batch = _PACK_ATTEND(tab, stride, cols, n, _index(q_start, i32, n + 1, "q_start", dev),
-                         _index(kv_len, i32, n, "kv_len", dev), shape[0], max_new, ATTEND_CAUSAL if causal else 0, scale)
+    try:
+        batch = _PACK_ATTEND(tab, stride, cols, n, _index(q_start, i32, n + 1, "q_start", dev),
+                             _index(kv_len, i32, n, "kv_len", dev), shape[0], max_new, ATTEND_CAUSAL if causal else 0, scale)
+    except _UNFIT as e:
+        _bad(f"scale {scale!r}, max_new {max_new!r}: {e}")
     _layer_check(lib().kvm_attend(_layer_stream(stream, dev), C.byref(cache), batch, a, b,
                                   work.data_ptr(), work.numel() * work.element_size()))
 
