@@ -810,6 +810,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             else mbar_arrive_n(bar, n);
         };
         bool described = false;
+        bool together = true;                  // every row warp is done with the pieces before this one
         while (next_piece()) {
             // Warps without a row of the piece (drafts fill one or two of the four pairs) would
             // only take the others' issue slots: they sleep on a named barrier, and the first
@@ -819,6 +820,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs &a) {
             auto sleep = [&]() {
                 if (idle) asm volatile("bar.sync 5, 256;" ::: "memory");
             };
+            // The votes for sleeping warps let the products go over O's rows: not before those
+            // warps have read there what the piece before left.
+            if (!together) sleep();
+            together = idle != 0u;
             if (!PAIR && static_cast<uint32_t>(warp & 3) * 32u >= p.rows) {
                 j += static_cast<uint32_t>(max(0, p.in1 - p.in0));
                 sleep();

@@ -170,3 +170,33 @@ def test_value_blocks_of_very_different_sizes(kvm_lib, kinds, D, group, new, apa
     q = queries(torch, w.rng, 2 * new, group, D, "bf16")
     got = w.run(q, [0, new, 2 * new], True, max_new=new)
     agree(got, *reference(w, q.float().cpu().numpy(), [0, new, 2 * new], [keys, 90], D ** -0.5), keys)
+
+
+# --------------------------------------- row tiles of different fill behind one another --
+
+@pytest.mark.parametrize("kinds", [("q8_0", "q5_0"), ("q4_0", "f16")])
+def test_short_row_tiles_behind_full_ones(kvm_lib, kinds):
+    """A CTA's next row tile may fill two of its four pairs of warps while the others still
+    store the last one, which V blocks beyond F16 make long: every row as the definition
+    has it, and the same bits on every run."""
+    import torch
+    news, lens = [66, 44, 109, 65, 34, 71, 97, 92], [94, 61, 110, 81, 33, 69, 113, 91]
+    w = Window(kvm_lib, torch, 3, kinds, 4, 128, 32, lens)
+
+    def change(v):
+        v[np.random.default_rng(0).random(v.shape[0]) < 0.05] *= 6e4 if kinds[1] == "f16" else 75000.0
+        return np.clip(v, -6e4, 6e4) if kinds[1] == "f16" else np.clip(v, -4e5, 4e5)
+    rewrite(w, 1, change)
+    if kinds[1] == "f16":                      # infinities are what F16 rows have to add apart
+        raw = w.raw[1].copy()
+        raw.view(np.float16)[w.cell(2, 3)] = np.inf
+        w.put(1, raw)
+    start = np.concatenate([[0], np.cumsum(news)])
+    q = queries(torch, w.rng, int(start[-1]), 48, 128, "bf16")
+    got = w.run(q, start, True, max_new=7)
+    for _ in range(5):
+        assert torch.equal(w.run(q, start, True, max_new=7).view(torch.int16), got.view(torch.int16))
+    with np.errstate(invalid="ignore"):
+        want = reference(w, q.float().cpu().numpy(), start, lens, 128 ** -0.5, rows=range(0, int(start[-1]), 5))
+    pick = [r for r in range(0, int(start[-1]), 5) if not (start[2] <= r < start[3] and kinds[1] == "f16")]
+    agree(got[pick], *(x[pick] for x in want), max(lens))
